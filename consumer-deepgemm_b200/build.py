@@ -50,7 +50,7 @@ def build_lib(force: bool = False, extra=()) -> str:
     if force or _stale(LIB, LIB_SOURCES):
         _run([NVCC, *ARCH_FLAGS, "-lineinfo", "-O3", "-std=c++17", "-Xcompiler", "-fPIC", "-shared",
               "-cudart", "shared", "-Xptxas", "-v", "-I", INCLUDE, "-I", CSRC,
-              "-o", LIB, os.path.join(CSRC, "cdg_abi.cu"), os.path.join(CSRC, "cdg_moe.cu"), *extra])
+              "-o", LIB, "-t", "0", *(f for f in LIB_SOURCES if f.endswith(".cu")), *extra])
     return LIB
 
 

@@ -1,0 +1,558 @@
+// Root-mean-square norm with the residual's addition, an e4m3 output with 1x128 scales, and
+// its gradient.
+//
+//   h = x + r                      (32 bits; stored once in x's type)
+//   s = 1 / sqrt(mean(h^2) + eps)
+//   y = h * s * w                  (from the 32-bit h; stored once in x's type)
+//   q, scale = 1x128 e4m3 quantisation of the 32-bit y (the recipes of cdg_quant_fp8_rows)
+//
+//   u = w * dy,  dx = dh + s * (u - h * s^2 * mean(u * h)),  dw[c] = sum_t dy[t, c] * h[t, c] * s[t]
+//
+// Both directions are bound by memory: the forward pass reads x and r once and writes h, y, q and
+// the scales once, the backward pass reads dy, h and dh once and writes dx once.  A row stays in
+// its CTA's registers between the sum of squares and the stores.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_fp8.h>
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <cstdint>
+
+#include "cdg_b200.h"
+
+namespace cdg {
+namespace {
+
+template <typename T>
+__device__ __forceinline__ float to_f(T v);
+template <>
+__device__ __forceinline__ float to_f(float v) { return v; }
+template <>
+__device__ __forceinline__ float to_f(__nv_bfloat16 v) { return __bfloat162float(v); }
+template <>
+__device__ __forceinline__ float to_f(__half v) { return __half2float(v); }
+
+template <typename T>
+__device__ __forceinline__ T from_f(float v);
+template <>
+__device__ __forceinline__ float from_f(float v) { return v; }
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_f(float v) { return __float2bfloat16_rn(v); }
+template <>
+__device__ __forceinline__ __half from_f(float v) { return __float2half_rn(v); }
+
+__device__ __forceinline__ float2 unpack2(uint32_t v, __nv_bfloat16) {
+  return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&v));
+}
+__device__ __forceinline__ float2 unpack2(uint32_t v, __half) {
+  return __half22float2(*reinterpret_cast<const __half2*>(&v));
+}
+__device__ __forceinline__ uint32_t pack2(float a, float b, __nv_bfloat16) {
+  const __nv_bfloat162 p = __floats2bfloat162_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&p);
+}
+__device__ __forceinline__ uint32_t pack2(float a, float b, __half) {
+  const __half2 p = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&p);
+}
+
+// A warp takes 256 columns at a time, eight per lane.  Wide (rows on 16-byte boundaries, H a
+// multiple of 8): lane l holds columns 8l .. 8l+7, one 128-column scale block per half warp.
+// Narrow (anything else): lane l holds columns l, l + 32, ..., so that each load of the warp
+// stays contiguous; the first four are in the first scale block, the others in the second.
+template <bool WIDE>
+__device__ __forceinline__ int64_t column(int64_t chunk, int lane, int j) {
+  return chunk * 256 + (WIDE ? lane * 8 + j : j * 32 + lane);
+}
+
+// The lane's eight elements of a chunk as they lie in memory.
+template <typename T>
+struct Raw {
+  static constexpr int kWords = static_cast<int>(sizeof(T)) * 2;
+  uint32_t w[kWords];
+};
+
+template <typename T>
+__device__ __forceinline__ void unpack8(const Raw<T>& raw, float (&v)[8]) {
+  if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = __uint_as_float(raw.w[j]);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float2 f = unpack2(raw.w[j], T());
+      v[2 * j] = f.x;
+      v[2 * j + 1] = f.y;
+    }
+  }
+}
+
+template <typename T, bool WIDE>
+__device__ __forceinline__ Raw<T> load8(const T* row, int64_t chunk, int lane, int64_t H) {
+  Raw<T> raw;
+#pragma unroll
+  for (int j = 0; j < Raw<T>::kWords; ++j) raw.w[j] = 0;
+  if constexpr (WIDE) {
+    const int64_t c = column<true>(chunk, lane, 0);
+    if (c < H) {
+      const uint4* p = reinterpret_cast<const uint4*>(row + c);
+#pragma unroll
+      for (int k = 0; k < Raw<T>::kWords / 4; ++k) {
+        const uint4 t = p[k];
+        raw.w[4 * k] = t.x; raw.w[4 * k + 1] = t.y; raw.w[4 * k + 2] = t.z; raw.w[4 * k + 3] = t.w;
+      }
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const int64_t c = column<false>(chunk, lane, j);
+      if (c < H) {
+        if constexpr (sizeof(T) == 4)
+          raw.w[j] = reinterpret_cast<const uint32_t*>(row)[c];
+        else
+          raw.w[j / 2] |= static_cast<uint32_t>(reinterpret_cast<const uint16_t*>(row)[c]) << (16 * (j & 1));
+      }
+    }
+  }
+  return raw;
+}
+
+template <typename T, bool WIDE>
+__device__ __forceinline__ void store8(T* row, int64_t chunk, int lane, int64_t H, const float (&v)[8]) {
+  if constexpr (WIDE) {
+    const int64_t c = column<true>(chunk, lane, 0);
+    if (c >= H) return;
+    uint4* p = reinterpret_cast<uint4*>(row + c);
+    if constexpr (sizeof(T) == 4) {
+      p[0] = make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
+      p[1] = make_uint4(__float_as_uint(v[4]), __float_as_uint(v[5]), __float_as_uint(v[6]), __float_as_uint(v[7]));
+    } else {
+      p[0] = make_uint4(pack2(v[0], v[1], T()), pack2(v[2], v[3], T()), pack2(v[4], v[5], T()), pack2(v[6], v[7], T()));
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const int64_t c = column<false>(chunk, lane, j);
+      if (c < H) row[c] = from_f<T>(v[j]);
+    }
+  }
+}
+
+// The norm's weights: of the rows' type or FP32.
+template <typename T, bool WIDE>
+__device__ __forceinline__ void load_weight8(const void* w, bool w_f32, int64_t chunk, int lane, int64_t H,
+                                             float (&v)[8]) {
+  if (w_f32) {
+    unpack8<float>(load8<float, WIDE>(static_cast<const float*>(w), chunk, lane, H), v);
+  } else {
+    unpack8<T>(load8<T, WIDE>(static_cast<const T*>(w), chunk, lane, H), v);
+  }
+}
+
+// Sum over the CTA's warps of one value per thread (every thread gets it).  `slot` holds one
+// value per warp; one barrier, so a caller that comes again alternates between two slots.
+__device__ __forceinline__ float cta_sum(float v, float* slot, int warps) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  if (warps == 1) return v;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (lane == 0) slot[warp] = v;
+  __syncthreads();
+  float t = lane < warps ? slot[lane] : 0.0f;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
+  return t;
+}
+
+// Scale and reciprocal factor of a 128-column block with the largest magnitude `amax`.  A NaN
+// among the values does not reach the scale (fmaxf passes over it); its own code is NaN.
+__device__ __forceinline__ float block_scale(float amax, int pow2, float& factor) {
+  amax = fmaxf(amax, 1e-12f);
+  float scale = amax / 448.0f;
+  if (pow2) {
+    uint32_t b = __float_as_uint(scale);
+    if (b & 0x007FFFFFu) b = (b & 0xFF800000u) + 0x00800000u;
+    scale = __uint_as_float(b);
+    factor = 1.0f / scale;
+  } else {
+    factor = 448.0f / amax;
+  }
+  return scale;
+}
+
+struct NormFwd {
+  const void *x, *r, *w;
+  void *h, *y;
+  uint8_t* q;
+  float* s;
+  int64_t x_stride, r_stride, h_stride, y_stride, q_stride, s_stride_m, s_stride_k;
+  int64_t T, H;
+  float eps;
+  int w_f32, pow2;
+};
+
+// Quantise one chunk of y and store codes and scales.
+template <bool WIDE>
+__device__ __forceinline__ void quant_chunk(const NormFwd& a, int64_t row, int64_t chunk, int lane,
+                                            const float (&y)[8]) {
+  uint8_t* q = a.q + row * a.q_stride;
+  float* s = a.s + row * a.s_stride_m;
+  const int64_t kb = chunk * 2;
+  if constexpr (WIDE) {
+    float m = 0.0f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) m = fmaxf(m, fabsf(y[j]));
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    float f;
+    const float scale = block_scale(m, a.pow2, f);
+    const int64_t c = column<true>(chunk, lane, 0);
+    if (c >= a.H) return;
+    uint32_t p[2];
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(y[4 * k] * f, y[4 * k + 1] * f), __NV_SATFINITE, __NV_E4M3);
+      const uint32_t hi =
+          __nv_cvt_float2_to_fp8x2(make_float2(y[4 * k + 2] * f, y[4 * k + 3] * f), __NV_SATFINITE, __NV_E4M3);
+      p[k] = lo | (hi << 16);
+    }
+    *reinterpret_cast<uint2*>(q + c) = make_uint2(p[0], p[1]);
+    if ((lane & 15) == 0) s[(kb + (lane >> 4)) * a.s_stride_k] = scale;
+  } else {
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+      float m = 0.0f;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) m = fmaxf(m, fabsf(y[4 * b + j]));
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+      float f;
+      const float scale = block_scale(m, a.pow2, f);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int64_t c = column<false>(chunk, lane, 4 * b + j);
+        if (c < a.H) q[c] = __nv_cvt_float_to_fp8(y[4 * b + j] * f, __NV_SATFINITE, __NV_E4M3);
+      }
+      if (lane == 0 && (kb + b) * 128 < a.H) s[(kb + b) * a.s_stride_k] = scale;
+    }
+  }
+}
+
+// One row per CTA (one per warp where a warp holds a whole row: warps_per_row == 1); warp w of a
+// row's warps takes chunks w, w + warps, ... and keeps its ITER chunks of h in registers.
+template <typename T, bool WIDE, int ITER, int THREADS>
+__global__ void __launch_bounds__(THREADS) add_rms_norm_kernel(const NormFwd a, int warps_per_row) {
+  __shared__ float slot[32];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  int64_t row = blockIdx.x;
+  int w = warp;
+  if (warps_per_row == 1) {
+    row = row * (blockDim.x >> 5) + warp;
+    w = 0;
+    if (row >= a.T) return;  // no barrier follows where a warp holds the row
+  }
+  const T* x = static_cast<const T*>(a.x) + row * a.x_stride;
+  Raw<T> rx[ITER], rr[ITER];
+#pragma unroll
+  for (int i = 0; i < ITER; ++i) rx[i] = load8<T, WIDE>(x, i * warps_per_row + w, lane, a.H);
+  if (a.r) {
+    const T* r = static_cast<const T*>(a.r) + row * a.r_stride;
+#pragma unroll
+    for (int i = 0; i < ITER; ++i) rr[i] = load8<T, WIDE>(r, i * warps_per_row + w, lane, a.H);
+  }
+  float h[ITER][8];
+  float sum = 0.0f;
+#pragma unroll
+  for (int i = 0; i < ITER; ++i) {
+    unpack8<T>(rx[i], h[i]);
+    if (a.r) {
+      float b[8];
+      unpack8<T>(rr[i], b);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) h[i][j] += b[j];
+    }
+    float part = 0.0f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) part = fmaf(h[i][j], h[i][j], part);
+    sum += part;
+  }
+  if (a.h) {
+#pragma unroll
+    for (int i = 0; i < ITER; ++i)
+      store8<T, WIDE>(static_cast<T*>(a.h) + row * a.h_stride, i * warps_per_row + w, lane, a.H, h[i]);
+  }
+  sum = cta_sum(sum, slot, warps_per_row);
+  const float rstd = 1.0f / sqrtf(sum / static_cast<float>(a.H) + a.eps);
+#pragma unroll
+  for (int i = 0; i < ITER; ++i) {
+    const int64_t chunk = i * warps_per_row + w;
+    if (chunk * 256 >= a.H) break;  // warp-uniform
+    float wv[8];
+    load_weight8<T, WIDE>(a.w, a.w_f32, chunk, lane, a.H, wv);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) wv[j] *= h[i][j] * rstd;
+    if (a.y) store8<T, WIDE>(static_cast<T*>(a.y) + row * a.y_stride, chunk, lane, a.H, wv);
+    if (a.q) quant_chunk<WIDE>(a, row, chunk, lane, wv);
+  }
+}
+
+struct NormBwd {
+  const void *dy, *h, *w, *dh;
+  void* dx;
+  float* partial;  // [gridDim.x][H]: each CTA's sum over its rows of dy * h * s
+  int64_t dy_stride, h_stride, dh_stride, dx_stride;
+  int64_t T, H;
+  float eps;
+  int w_f32;
+};
+
+// CTA b takes rows b, b + grid, ...; warp w of it takes chunks w, w + warps, ... of every row and
+// sums their weight gradients in registers.  The next row's loads are issued before this row's
+// barrier, so that they cross it.  Both sums over the row (h^2 and u * h) share one barrier.
+template <typename T, bool WIDE, int ITER, int THREADS>
+__global__ void __launch_bounds__(THREADS) rms_norm_backward_kernel(const NormBwd a) {
+  __shared__ float2 slot[2][32];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
+  const T* dy = static_cast<const T*>(a.dy);
+  const T* h = static_cast<const T*>(a.h);
+  const T* dh = static_cast<const T*>(a.dh);
+  float acc[ITER][8] = {};
+  Raw<T> rdy[ITER], rh[ITER], rdh[ITER];
+  auto load_row = [&](int64_t row) {
+#pragma unroll
+    for (int i = 0; i < ITER; ++i) {
+      const int64_t chunk = i * warps + warp;
+      rh[i] = load8<T, WIDE>(h + row * a.h_stride, chunk, lane, a.H);
+      rdy[i] = load8<T, WIDE>(dy + row * a.dy_stride, chunk, lane, a.H);
+      if (dh) rdh[i] = load8<T, WIDE>(dh + row * a.dh_stride, chunk, lane, a.H);
+    }
+  };
+  int64_t row = blockIdx.x;
+  if (row < a.T) load_row(row);
+  for (int turn = 0; row < a.T; row += gridDim.x, turn ^= 1) {
+    Raw<T> cdy[ITER], ch[ITER], cdh[ITER];
+    float sq = 0.0f, uh = 0.0f;
+#pragma unroll
+    for (int i = 0; i < ITER; ++i) {
+      cdy[i] = rdy[i]; ch[i] = rh[i]; cdh[i] = rdh[i];
+    }
+    if (row + gridDim.x < a.T) load_row(row + gridDim.x);
+#pragma unroll
+    for (int i = 0; i < ITER; ++i) {
+      float hv[8], g[8], wv[8];
+      unpack8<T>(ch[i], hv);
+      unpack8<T>(cdy[i], g);
+      load_weight8<T, WIDE>(a.w, a.w_f32, i * warps + warp, lane, a.H, wv);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        sq = fmaf(hv[j], hv[j], sq);
+        uh = fmaf(g[j] * wv[j], hv[j], uh);
+      }
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      sq += __shfl_xor_sync(0xffffffffu, sq, o);
+      uh += __shfl_xor_sync(0xffffffffu, uh, o);
+    }
+    if (lane == 0) slot[turn][warp] = make_float2(sq, uh);
+    __syncthreads();
+    const float2 t = lane < warps ? slot[turn][lane] : make_float2(0.0f, 0.0f);
+    sq = t.x;
+    uh = t.y;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      sq += __shfl_xor_sync(0xffffffffu, sq, o);
+      uh += __shfl_xor_sync(0xffffffffu, uh, o);
+    }
+    const float inv = 1.0f / static_cast<float>(a.H);
+    const float rstd = 1.0f / sqrtf(sq * inv + a.eps);
+    const float k = uh * inv * rstd * rstd;
+#pragma unroll
+    for (int i = 0; i < ITER; ++i) {
+      const int64_t chunk = i * warps + warp;
+      float hv[8], g[8], wv[8];
+      unpack8<T>(ch[i], hv);
+      unpack8<T>(cdy[i], g);
+      load_weight8<T, WIDE>(a.w, a.w_f32, chunk, lane, a.H, wv);
+      float out[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        acc[i][j] = fmaf(g[j], hv[j] * rstd, acc[i][j]);
+        out[j] = rstd * fmaf(-hv[j], k, g[j] * wv[j]);
+      }
+      if (dh) {
+        float d[8];
+        unpack8<T>(cdh[i], d);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) out[j] += d[j];
+      }
+      store8<T, WIDE>(static_cast<T*>(a.dx) + row * a.dx_stride, chunk, lane, a.H, out);
+    }
+  }
+  float* partial = a.partial + static_cast<int64_t>(blockIdx.x) * a.H;
+#pragma unroll
+  for (int i = 0; i < ITER; ++i) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const int64_t c = column<WIDE>(i * warps + warp, lane, j);
+      if (c < a.H) partial[c] = acc[i][j];
+    }
+  }
+}
+
+// dw[c] = the sum of the CTAs' partial sums, in CTA order per thread and then over the eight
+// threads of a column: the same order every time.
+template <typename W>
+__global__ void __launch_bounds__(256) rms_norm_dw_kernel(const float* partial, int parts, int64_t H, W* dw) {
+  __shared__ float sums[8][33];
+  const int lane = threadIdx.x & 31, g = threadIdx.x >> 5;
+  const int64_t c = static_cast<int64_t>(blockIdx.x) * 32 + lane;
+  float v = 0.0f;
+  if (c < H)
+    for (int p = g; p < parts; p += 8) v += partial[static_cast<int64_t>(p) * H + c];
+  sums[g][lane] = v;
+  __syncthreads();
+  if (g == 0 && c < H) {
+#pragma unroll
+    for (int i = 1; i < 8; ++i) v += sums[i][lane];
+    dw[c] = from_f<W>(v);
+  }
+}
+
+int launched() { return cudaGetLastError() == cudaSuccess ? CDG_OK : CDG_ERR_CUDA; }
+
+int sm_count() {
+  int dev = 0, n = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
+    return 148;
+  return n > 0 ? n : 148;
+}
+}  // namespace
+
+// Row widths up to this one fit the registers of one CTA (32 warps of four 256-column chunks).
+constexpr int64_t kNormMaxH = 32768;
+
+namespace {
+
+int element_size(int dtype) { return dtype == CDG_DTYPE_F32 ? 4 : 2; }
+
+bool row_dtype(int dtype) { return dtype == CDG_DTYPE_BF16 || dtype == CDG_DTYPE_F16 || dtype == CDG_DTYPE_F32; }
+
+// Whether every row of a tensor starts on a 16-byte boundary (absent tensors do).
+bool wide_rows(const void* p, int64_t stride, int64_t bytes) {
+  return !p || (reinterpret_cast<uintptr_t>(p) % 16 == 0 && stride * bytes % 16 == 0);
+}
+
+template <typename T, bool WIDE>
+int launch_norm(const NormFwd& a, cudaStream_t st) {
+  const int chunks = static_cast<int>((a.H + 255) / 256);
+  // Rows of few tokens are spread over as many warps as they have chunks (latency); otherwise a
+  // warp holds four chunks, so that one barrier and one reduction serve more loads.
+  // Rows of more than 8192 columns take up to 32 warps, whose registers then hold four chunks
+  // with some spilling.
+  const int iter = chunks <= 32 && a.T <= 2 * sm_count() ? 1 : chunks >= 4 ? 4 : chunks >= 2 ? 2 : 1;
+  const int warps = (chunks + iter - 1) / iter;
+  const int rows = warps == 1 ? 4 : 1;  // rows per CTA
+  const unsigned grid = static_cast<unsigned>((a.T + rows - 1) / rows);
+  auto kernel = iter == 1    ? add_rms_norm_kernel<T, WIDE, 1, 1024>
+                : iter == 2  ? add_rms_norm_kernel<T, WIDE, 2, 128>
+                : warps <= 8 ? add_rms_norm_kernel<T, WIDE, 4, 256>
+                             : add_rms_norm_kernel<T, WIDE, 4, 1024>;
+  kernel<<<grid, warps * rows * 32, 0, st>>>(a, warps);
+  return launched();
+}
+
+// CTAs of the backward kernel: every SM filled, each CTA taking several rows where there are
+// that many, because each writes one row of partial weight gradients.
+struct BwdShape {
+  int iter, warps, grid;
+};
+
+BwdShape backward_shape(int64_t T, int64_t H) {
+  const int chunks = static_cast<int>((H + 255) / 256);
+  BwdShape s;
+  s.iter = chunks <= 4 ? 1 : chunks <= 32 ? 2 : 4;
+  s.warps = (chunks + s.iter - 1) / s.iter;
+  const int per_sm = std::max(1, std::min(16, 16 / s.warps));
+  s.grid = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(T, int64_t(sm_count()) * per_sm)));
+  return s;
+}
+
+template <typename T, bool WIDE>
+int launch_norm_backward(const NormBwd& a, const BwdShape& s, cudaStream_t st) {
+  auto kernel = s.iter == 1   ? rms_norm_backward_kernel<T, WIDE, 1, 128>
+                : s.iter == 2 ? rms_norm_backward_kernel<T, WIDE, 2, 512>
+                              : rms_norm_backward_kernel<T, WIDE, 4, 1024>;
+  kernel<<<s.grid, s.warps * 32, 0, st>>>(a);
+  return launched();
+}
+
+}  // namespace
+}  // namespace cdg
+
+extern "C" {
+
+int cdg_add_rms_norm(const cdg_norm_args* g, cdg_stream_t stream) {
+  using namespace cdg;
+  if (!g || g->T < 0 || g->H <= 0 || !row_dtype(g->dtype)) return CDG_ERR_INVALID_ARGUMENT;
+  if (g->w_dtype != g->dtype && g->w_dtype != CDG_DTYPE_F32) return CDG_ERR_INVALID_ARGUMENT;
+  if (g->scale_fmt != CDG_SCALE_FP32 && g->scale_fmt != CDG_SCALE_POW2) return CDG_ERR_INVALID_ARGUMENT;
+  if (!(g->eps >= 0.0f)) return CDG_ERR_INVALID_ARGUMENT;
+  if (g->H > kNormMaxH || g->T >= int64_t(1) << 31) return CDG_ERR_UNSUPPORTED;
+  if (g->T == 0) return CDG_OK;
+  if (!g->x || !g->w || (g->q && !g->s) || (!g->y && !g->q && !g->h)) return CDG_ERR_INVALID_ARGUMENT;
+  NormFwd a{g->x, g->r, g->w, g->h, g->y, g->q, g->s, g->x_stride, g->r_stride, g->h_stride, g->y_stride, g->q_stride,
+            g->s_stride_m, g->s_stride_k, g->T, g->H, g->eps, g->w_dtype == CDG_DTYPE_F32, g->scale_fmt};
+  const int64_t e = element_size(g->dtype);
+  const bool wide = g->H % 8 == 0 && wide_rows(a.x, a.x_stride, e) && wide_rows(a.r, a.r_stride, e) &&
+                    wide_rows(a.h, a.h_stride, e) && wide_rows(a.y, a.y_stride, e) && wide_rows(a.w, 0, e) &&
+                    (!a.q || (reinterpret_cast<uintptr_t>(a.q) % 8 == 0 && a.q_stride % 8 == 0));
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  if (g->dtype == CDG_DTYPE_BF16)
+    return wide ? launch_norm<__nv_bfloat16, true>(a, st) : launch_norm<__nv_bfloat16, false>(a, st);
+  if (g->dtype == CDG_DTYPE_F16) return wide ? launch_norm<__half, true>(a, st) : launch_norm<__half, false>(a, st);
+  return wide ? launch_norm<float, true>(a, st) : launch_norm<float, false>(a, st);
+}
+
+size_t cdg_rms_norm_backward_workspace_bytes(int64_t T, int64_t H) {
+  if (T < 0 || H <= 0 || H > cdg::kNormMaxH) return 0;
+  return static_cast<size_t>(cdg::backward_shape(T, H).grid) * H * sizeof(float);
+}
+
+int cdg_rms_norm_backward(const cdg_norm_backward_args* g, void* workspace, size_t workspace_bytes,
+                          cdg_stream_t stream) {
+  using namespace cdg;
+  if (!g || g->T < 0 || g->H <= 0 || !row_dtype(g->dtype)) return CDG_ERR_INVALID_ARGUMENT;
+  if (g->w_dtype != g->dtype && g->w_dtype != CDG_DTYPE_F32) return CDG_ERR_INVALID_ARGUMENT;
+  if (!(g->eps >= 0.0f) || !g->w || !g->dw) return CDG_ERR_INVALID_ARGUMENT;
+  if (g->H > kNormMaxH || g->T >= int64_t(1) << 31) return CDG_ERR_UNSUPPORTED;
+  if (g->T > 0 && (!g->dy || !g->h || !g->dx)) return CDG_ERR_INVALID_ARGUMENT;
+  if (!workspace || workspace_bytes < cdg_rms_norm_backward_workspace_bytes(g->T, g->H)) return CDG_ERR_WORKSPACE;
+  if (reinterpret_cast<uintptr_t>(workspace) % 4) return CDG_ERR_ALIGNMENT;
+  NormBwd a{g->dy, g->h, g->w, g->dh, g->dx, static_cast<float*>(workspace), g->dy_stride, g->h_stride, g->dh_stride,
+            g->dx_stride, g->T, g->H, g->eps, g->w_dtype == CDG_DTYPE_F32};
+  const int64_t e = element_size(g->dtype);
+  const bool wide = g->H % 8 == 0 && wide_rows(a.dy, a.dy_stride, e) && wide_rows(a.h, a.h_stride, e) &&
+                    wide_rows(a.dh, a.dh_stride, e) && wide_rows(a.dx, a.dx_stride, e) && wide_rows(a.w, 0, e);
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  const BwdShape s = backward_shape(g->T, g->H);
+  int rc;
+  if (g->dtype == CDG_DTYPE_BF16)
+    rc = wide ? launch_norm_backward<__nv_bfloat16, true>(a, s, st) : launch_norm_backward<__nv_bfloat16, false>(a, s, st);
+  else if (g->dtype == CDG_DTYPE_F16)
+    rc = wide ? launch_norm_backward<__half, true>(a, s, st) : launch_norm_backward<__half, false>(a, s, st);
+  else
+    rc = wide ? launch_norm_backward<float, true>(a, s, st) : launch_norm_backward<float, false>(a, s, st);
+  if (rc != CDG_OK) return rc;
+  const unsigned grid = static_cast<unsigned>((g->H + 31) / 32);
+  if (g->w_dtype == CDG_DTYPE_BF16)
+    rms_norm_dw_kernel<__nv_bfloat16><<<grid, 256, 0, st>>>(a.partial, s.grid, g->H, static_cast<__nv_bfloat16*>(g->dw));
+  else if (g->w_dtype == CDG_DTYPE_F16)
+    rms_norm_dw_kernel<__half><<<grid, 256, 0, st>>>(a.partial, s.grid, g->H, static_cast<__half*>(g->dw));
+  else
+    rms_norm_dw_kernel<float><<<grid, 256, 0, st>>>(a.partial, s.grid, g->H, static_cast<float*>(g->dw));
+  return launched();
+}
+
+}  // extern "C"

@@ -30,6 +30,7 @@ int32_t dtype_code(const torch::Tensor& t) {
   switch (t.scalar_type()) {
     case torch::kFloat8_e4m3fn: return CDG_DTYPE_E4M3;
     case torch::kBFloat16: return CDG_DTYPE_BF16;
+    case torch::kFloat16: return CDG_DTYPE_F16;
     case torch::kFloat32: return CDG_DTYPE_F32;
     case torch::kUInt8: return CDG_DTYPE_UE8M0;
     case torch::kInt32: return CDG_DTYPE_I32;
@@ -611,6 +612,123 @@ torch::Tensor ep_unpermute_combine(const torch::Tensor& Y, const torch::Tensor& 
   return y;
 }
 
+// ------------------------------------------------------------------ around the experts: norm, router, dense product
+// A [rows, columns] tensor with unit stride along its columns, on `dev`.
+void check_rows(const torch::Tensor& t, const char* name, const torch::Device& dev, int64_t rows, int64_t cols) {
+  check_cuda(t, name, dev);
+  TORCH_CHECK_VALUE(t.dim() == 2 && t.size(0) == rows && t.size(1) == cols, name, " must be [", rows, ", ", cols,
+                    "], got ", t.sizes());
+  TORCH_CHECK_VALUE(cols <= 1 || t.stride(1) == 1, name, " must have unit stride along its last dim");
+}
+
+void check_vector(const torch::Tensor& t, const char* name, const torch::Device& dev, int64_t n) {
+  check_cuda(t, name, dev);
+  TORCH_CHECK_VALUE(t.dim() == 1 && t.size(0) == n && (n <= 1 || t.stride(0) == 1), name,
+                    " must be a contiguous vector of ", n, ", got ", t.sizes());
+}
+
+bool float_rows(const torch::Tensor& t) {
+  return t.scalar_type() == torch::kBFloat16 || t.scalar_type() == torch::kFloat16 ||
+         t.scalar_type() == torch::kFloat32;
+}
+
+// (h, y, q, scale), None where not asked for; h only with a residual.
+py::tuple add_rms_norm(const torch::Tensor& x, const torch::Tensor& w, const c10::optional<torch::Tensor>& residual,
+                       double eps, bool quantize, bool ue8m0, bool normed) {
+  const auto dev = x.device();
+  check_cuda(x, "x", dev);
+  TORCH_CHECK_VALUE(x.dim() == 2 && x.size(1) > 0, "x must be [T, H] with H > 0, got ", x.sizes());
+  TORCH_CHECK_VALUE(float_rows(x), "x must be BF16/FP16/FP32, got ", x.scalar_type());
+  TORCH_CHECK_VALUE(normed || quantize, "nothing to compute: normed and quantize are both off");
+  TORCH_CHECK_VALUE(eps >= 0, "eps must not be negative");
+  const int64_t T = x.size(0), H = x.size(1);
+  check_rows(x, "x", dev, T, H);
+  check_vector(w, "weight", dev, H);
+  TORCH_CHECK_VALUE(w.scalar_type() == x.scalar_type() || w.scalar_type() == torch::kFloat32,
+                    "weight must have x's dtype or FP32, got ", w.scalar_type());
+  cdg_norm_args g{};
+  torch::Tensor h, y, q, s;
+  const c10::cuda::CUDAGuard guard(dev);
+  if (residual.has_value()) {
+    check_rows(*residual, "residual", dev, T, H);
+    TORCH_CHECK_VALUE(residual->scalar_type() == x.scalar_type(), "residual must have x's dtype");
+    g.r = residual->data_ptr();
+    g.r_stride = residual->stride(0);
+    h = torch::empty({T, H}, x.options());
+    g.h = h.data_ptr();
+    g.h_stride = H;
+  }
+  if (normed) {
+    y = torch::empty({T, H}, x.options());
+    g.y = y.data_ptr();
+    g.y_stride = H;
+  }
+  if (quantize) {
+    q = torch::empty({T, H}, x.options().dtype(torch::kFloat8_e4m3fn));
+    s = torch::empty({T, (H + 127) / 128}, x.options().dtype(torch::kFloat32));
+    g.q = reinterpret_cast<uint8_t*>(q.data_ptr());
+    g.q_stride = H;
+    g.s = s.data_ptr<float>();
+    g.s_stride_m = s.size(1);
+    g.s_stride_k = 1;
+  }
+  g.x = x.data_ptr();
+  g.x_stride = x.stride(0);
+  g.w = w.data_ptr();
+  g.dtype = dtype_code(x);
+  g.w_dtype = dtype_code(w);
+  g.T = T;
+  g.H = H;
+  g.eps = static_cast<float>(eps);
+  g.scale_fmt = ue8m0 ? CDG_SCALE_POW2 : CDG_SCALE_FP32;
+  check_status(cdg_add_rms_norm(&g, cur_stream(x)), "add_rms_norm");
+  auto give = [](const torch::Tensor& t) -> py::object { return t.defined() ? py::cast(t) : py::none(); };
+  return py::make_tuple(give(h), give(y), give(q), give(s));
+}
+
+std::vector<torch::Tensor> rms_norm_backward(const torch::Tensor& dy, const torch::Tensor& h, const torch::Tensor& w,
+                                             const c10::optional<torch::Tensor>& dh, double eps) {
+  const auto dev = h.device();
+  check_cuda(h, "h", dev);
+  TORCH_CHECK_VALUE(h.dim() == 2 && h.size(1) > 0, "h must be [T, H] with H > 0, got ", h.sizes());
+  TORCH_CHECK_VALUE(float_rows(h), "h must be BF16/FP16/FP32, got ", h.scalar_type());
+  TORCH_CHECK_VALUE(eps >= 0, "eps must not be negative");
+  const int64_t T = h.size(0), H = h.size(1);
+  check_rows(h, "h", dev, T, H);
+  check_rows(dy, "dy", dev, T, H);
+  check_vector(w, "weight", dev, H);
+  TORCH_CHECK_VALUE(dy.scalar_type() == h.scalar_type(), "dy must have h's dtype");
+  TORCH_CHECK_VALUE(w.scalar_type() == h.scalar_type() || w.scalar_type() == torch::kFloat32,
+                    "weight must have h's dtype or FP32, got ", w.scalar_type());
+  cdg_norm_backward_args g{};
+  if (dh.has_value()) {
+    check_rows(*dh, "dh", dev, T, H);
+    TORCH_CHECK_VALUE(dh->scalar_type() == h.scalar_type(), "dh must have h's dtype");
+    g.dh = dh->data_ptr();
+    g.dh_stride = dh->stride(0);
+  }
+  const c10::cuda::CUDAGuard guard(dev);
+  auto dx = torch::empty({T, H}, h.options());
+  auto dw = torch::empty({H}, w.options());
+  const size_t ws_bytes = cdg_rms_norm_backward_workspace_bytes(T, H);
+  auto ws = torch::empty({static_cast<int64_t>(ws_bytes)}, h.options().dtype(torch::kUInt8));
+  g.dy = dy.data_ptr();
+  g.dy_stride = dy.stride(0);
+  g.h = h.data_ptr();
+  g.h_stride = h.stride(0);
+  g.w = w.data_ptr();
+  g.dtype = dtype_code(h);
+  g.w_dtype = dtype_code(w);
+  g.T = T;
+  g.H = H;
+  g.eps = static_cast<float>(eps);
+  g.dx = dx.data_ptr();
+  g.dx_stride = H;
+  g.dw = dw.data_ptr();
+  check_status(cdg_rms_norm_backward(&g, ws.data_ptr(), ws_bytes, cur_stream(h)), "add_rms_norm_backward");
+  return {dx, dw};
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -710,4 +828,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("ep_combine", &ep_combine, py::arg("rows"), py::arg("send_index"), py::arg("topk_w"));
   m.def("ep_unpermute_combine", &ep_unpermute_combine, py::arg("y"), py::arg("perm_pos"), py::arg("send_index"),
         py::arg("topk_w"));
+  m.def("add_rms_norm", &add_rms_norm, py::arg("x"), py::arg("weight"), py::arg("residual"), py::arg("eps"),
+        py::arg("quantize"), py::arg("ue8m0"), py::arg("normed"));
+  m.def("rms_norm_backward", &rms_norm_backward, py::arg("dy"), py::arg("h"), py::arg("weight"), py::arg("dh"),
+        py::arg("eps"));
 }

@@ -59,6 +59,7 @@ typedef enum cdg_dtype {
   CDG_DTYPE_UE8M0_X4 = 7, /* int32 words of four UE8M0 activation scales: the scale of 128-wide K
                             block kb is byte kb % 4 of word kb / 4 (the packed format of DeepGEMM's
                             UE8M0 recipe, e.g. vLLM's silu_mul_quant_fp8_packed) */
+  CDG_DTYPE_F16 = 9,    /* IEEE half (the norm, the router and the dense product) */
   CDG_DTYPE_E4M3_PLANES = 8 /* activations given as the two e4m3 planes the tensor cores read: `a` is
                                uint8 [2][M][K] (hi plane, then lo plane; a_row_stride = K, M a multiple
                                of 128), `sa` is int32 [M] row exponents E (sa_dtype = CDG_DTYPE_I32),
@@ -480,6 +481,66 @@ int cdg_ep_unpermute_combine(const void* Y, int64_t y_stride, const int32_t* per
 
 /* Human-readable name of a cdg_status value. */
 const char* cdg_status_string(int status);
+
+/* ---------------------------------------------------------------------------------------------
+ * What stands around the experts in a mixture-of-experts block: the norm before them, the router
+ * and dense products.  None of these exist in the reference (it ships the GEMM only).
+ * Strides are in elements; last dimensions have unit stride.
+ * ------------------------------------------------------------------------------------------- */
+
+/* RMS norm with the residual's addition and an e4m3 output.  For each of T rows of H columns:
+ *   h = x + r (32 bits),  y = h / sqrt(mean(h^2) + eps) * w,
+ *   q, s = the 1x128 e4m3 quantisation of the 32-bit y (scale_fmt; the last block of a row may be
+ *   shorter than 128 columns).
+ * x, r, h, y are of `dtype` (BF16, F16 or F32); w of `dtype` or F32.  r may be NULL (no addition);
+ * h, y and q may each be NULL (not written), not all three.  h may be x or r itself.
+ * H up to 32,768. */
+typedef struct cdg_norm_args {
+  const void* x;
+  int64_t x_stride;
+  const void* r;
+  int64_t r_stride;
+  const void* w;
+  int32_t dtype, w_dtype;
+  int64_t T, H;
+  float eps;
+  int32_t scale_fmt; /* CDG_SCALE_* */
+  void* h;
+  int64_t h_stride;
+  void* y;
+  int64_t y_stride;
+  uint8_t* q;
+  int64_t q_stride;
+  float* s; /* [T, ceil(H / 128)] */
+  int64_t s_stride_m, s_stride_k;
+} cdg_norm_args;
+
+int cdg_add_rms_norm(const cdg_norm_args* args, cdg_stream_t stream);
+
+/* Gradient of the norm at h (the sum x + r as stored): with u = w * dy and
+ * s = 1 / sqrt(mean(h^2) + eps),
+ *   dx = dh + s * (u - h * s^2 * mean(u * h)),   dw[c] = sum over rows of dy * h * s.
+ * dh (the gradient that reaches h by the residual stream) may be NULL.  dx is the gradient of x
+ * and of r alike.  dw is of w's type and summed in a fixed order. */
+typedef struct cdg_norm_backward_args {
+  const void* dy;
+  int64_t dy_stride;
+  const void* h;
+  int64_t h_stride;
+  const void* w;
+  const void* dh;
+  int64_t dh_stride;
+  int32_t dtype, w_dtype;
+  int64_t T, H;
+  float eps;
+  void* dx;
+  int64_t dx_stride;
+  void* dw;
+} cdg_norm_backward_args;
+
+size_t cdg_rms_norm_backward_workspace_bytes(int64_t T, int64_t H);
+int cdg_rms_norm_backward(const cdg_norm_backward_args* args, void* workspace, size_t workspace_bytes,
+                          cdg_stream_t stream);
 
 #ifdef __cplusplus
 }
