@@ -20,6 +20,7 @@ from .native import build_info as native_build_info
 from .native import check_device_status, read_device_status
 from .native import is_available as native_is_available
 from .norm import add_rms_norm, add_rms_norm_backward
+from .router import moe_route, moe_route_backward
 from .utils import get_num_sms, get_pdl, get_tc_util, set_num_sms, set_pdl, set_tc_util
 
 __version__ = "0.2.0"
@@ -31,6 +32,8 @@ __all__ = [
     "transform_weights_for_mega_moe",
     "add_rms_norm",
     "add_rms_norm_backward",
+    "moe_route",
+    "moe_route_backward",
     "get_symm_buffer_for_mega_moe",
     "fp8_fp4_mega_moe",
     "get_mn_major_tma_aligned_tensor",

@@ -1,0 +1,503 @@
+// Router of a mixture-of-experts block: top-k gate, rows per expert and balance loss from the
+// router's logits in one pass over them, and the gradient with respect to the logits.
+//
+// For each token t (a row of E logits l) that is not masked and has an expert above -inf:
+//   score = softmax(l) or sigmoid(l),  p = score / sum(score)
+//   ids   = the k largest of l (of score + bias where a bias is given), ties to the lowest index
+//   w_j   = scale * score[ids_j]   (divided by the sum of the k chosen scores if renormalised)
+// Over the V valid tokens: counts[e] = how often e was chosen and
+//   loss  = E / (k V^2) * sum_e counts[e] * sum_t p[t, e].
+// Gradient, with g_j = dL/dw_j * scale, a_e = dL/dloss * E counts[e] / (k V^2) (counts held fixed):
+//   renormalised: g_j <- (g_j - sum_i g_i c_i / C) / C with c the chosen scores, C their sum
+//   softmax: dl_i = p_i (d_i - sum_j d_j p_j),  d = scatter(g) + a
+//   sigmoid: dl_i = (scatter(g)_i + (a_i - sum_j a_j p_j) / S) s_i (1 - s_i),  S = sum s
+//
+// A warp takes a row, lane l the experts l, l + 32, ...; a row is read once and its next row's
+// loads are in flight meanwhile.  Bound by instructions rather than memory: k rounds of a
+// warp-wide maximum per row.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <cfloat>
+#include <cstdint>
+
+#include "cdg_b200.h"
+
+namespace cdg {
+namespace {
+
+constexpr int kRouteMaxExperts = 1024;
+constexpr int kRouteMaxTopk = 32;  // lane j keeps the row's j-th choice
+constexpr unsigned kAll = 0xffffffffu;
+
+template <typename T>
+__device__ __forceinline__ float load_logit(const T* p);
+template <>
+__device__ __forceinline__ float load_logit(const float* p) { return __ldg(p); }
+template <>
+__device__ __forceinline__ float load_logit(const __nv_bfloat16* p) { return __bfloat162float(*p); }
+template <>
+__device__ __forceinline__ float load_logit(const __half* p) { return __half2float(*p); }
+
+// NaN counts as -inf (never chosen), +inf as the largest finite value, -0 as 0.
+__device__ __forceinline__ float clean_logit(float v) {
+  return v == v ? fminf(v, FLT_MAX) + 0.0f : -INFINITY;
+}
+
+// Keys whose unsigned order is the values' order; 0 stands for "cannot be chosen" (-inf).
+__device__ __forceinline__ uint32_t order_key(float v) {
+  const uint32_t b = __float_as_uint(v);
+  const uint32_t key = b ^ (b & 0x80000000u ? 0xFFFFFFFFu : 0x80000000u);
+  return v == -INFINITY ? 0u : key;
+}
+__device__ __forceinline__ float key_value(uint32_t key) {
+  return __uint_as_float(key ^ (key & 0x80000000u ? 0x80000000u : 0xFFFFFFFFu));
+}
+
+__device__ __forceinline__ float warp_sum(float v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(kAll, v, o);
+  return v;
+}
+
+// Fast exponential and division (errors of a few units in the last place): the gate's weights
+// and gradients stay within 1e-6 of the exact ones.
+__device__ __forceinline__ float sigmoid_fast(float v) { return __fdividef(1.0f, 1.0f + __expf(-v)); }
+
+struct Route {
+  const void* logits;
+  int64_t stride;
+  const uint8_t* mask;
+  const float* bias;
+  int64_t T;
+  int E, k;
+  int sigmoid, renormalize, balance;
+  float scale;
+  float* weights;
+  int32_t *ids, *counts, *tokens;
+  float* loss;
+  // zeroed before the launch (several CTAs): sum of p per expert in units of 2^-40, rows per
+  // expert, valid tokens, finished CTAs
+  unsigned long long* psum;
+  int32_t *acc_counts, *acc_tokens, *ticket;
+};
+
+// Sums of p leave a CTA as 64-bit integers in units of 2^-40, so that the order in which the
+// CTAs add them does not change the result.  2^23 tokens fit.
+constexpr float kFixed = 1099511627776.0f;
+constexpr int64_t kRouteMaxTokens = int64_t(1) << 23;
+
+__device__ float balance_loss(const Route& a, int32_t tokens, const volatile unsigned long long* psum,
+                              const volatile int32_t* counts, double* scratch) {
+  double v = 0.0;
+  for (int e = threadIdx.x; e < a.E; e += blockDim.x)
+    v += static_cast<double>(counts[e]) * (static_cast<double>(psum[e]) / static_cast<double>(kFixed));
+  scratch[threadIdx.x] = v;
+  __syncthreads();
+  for (int o = blockDim.x / 2; o > 0; o >>= 1) {
+    if (threadIdx.x < static_cast<unsigned>(o)) scratch[threadIdx.x] += scratch[threadIdx.x + o];
+    __syncthreads();
+  }
+  const double n = tokens > 0 ? tokens : 1;
+  return static_cast<float>(scratch[0] * a.E / a.k / n / n);
+}
+
+// N experts per lane.  Dynamic shared memory: E counts, then one row of E sums of p per warp.
+template <typename T, int N, int WARPS>
+__global__ void __launch_bounds__(WARPS * 32) moe_route_kernel(const Route a) {
+  extern __shared__ int32_t route_smem[];
+  __shared__ double scratch[WARPS * 32];
+  __shared__ int32_t s_tokens, s_last;
+  int32_t* s_counts = route_smem;
+  float* s_psum = reinterpret_cast<float*>(route_smem + a.E);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  for (int e = threadIdx.x; e < a.E; e += blockDim.x) s_counts[e] = 0;
+  if (threadIdx.x == 0) s_tokens = 0;
+  __syncthreads();
+
+  const T* logits = static_cast<const T*>(a.logits);
+  float psum[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) psum[i] = 0.0f;
+  int32_t tokens = 0;
+  const int64_t step = static_cast<int64_t>(gridDim.x) * WARPS;
+  float next[N];
+  auto load_row = [&](int64_t row) {
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      next[i] = i * 32 + lane < a.E ? load_logit<T>(logits + row * a.stride + i * 32 + lane) : -INFINITY;
+  };
+  int64_t row = static_cast<int64_t>(blockIdx.x) * WARPS + warp;
+  if (row < a.T) load_row(row);
+  for (; row < a.T; row += step) {
+    uint32_t key[N];
+    float v[N];
+    uint32_t top = 0;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      v[i] = clean_logit(next[i]);
+      key[i] = order_key(v[i]);
+      top = max(top, key[i]);
+    }
+    if (row + step < a.T) load_row(row + step);
+    top = __reduce_max_sync(kAll, top);
+    int32_t id = -1;
+    float w = 0.0f;
+    if (top != 0 && (!a.mask || a.mask[row])) {  // warp-uniform
+      const float m = a.sigmoid ? 0.0f : key_value(top);
+      float inv = 1.0f;   // 1 / sum of exponentials (softmax)
+      float part = 0.0f;  // 1 / sum of scores
+      if (a.balance || a.bias || !a.renormalize) {
+        float total = 0.0f;
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+          v[i] = a.sigmoid ? sigmoid_fast(v[i]) : __expf(v[i] - m);
+          total += v[i];
+        }
+        total = warp_sum(total);
+        part = total > 0.0f ? 1.0f / total : 0.0f;
+        if (!a.sigmoid) inv = part;
+        if (a.bias) {
+#pragma unroll
+          for (int i = 0; i < N; ++i)
+            if (key[i] != 0) key[i] = order_key(clean_logit(v[i] * inv + __ldg(a.bias + i * 32 + lane)));
+        }
+      }
+      // k rounds: the largest key, of equal ones the lowest expert
+      uint32_t mine = 0;
+#pragma unroll
+      for (int i = 0; i < N; ++i) mine = max(mine, key[i]);
+      const bool valid = __any_sync(kAll, mine != 0);  // a bias of -inf may have left nothing
+      if (valid) {
+        ++tokens;
+        if (a.balance) {
+#pragma unroll
+          for (int i = 0; i < N; ++i) psum[i] = fmaf(v[i], part, psum[i]);
+        }
+      }
+      for (int j = 0; j < a.k; ++j) {
+        const uint32_t best = __reduce_max_sync(kAll, mine);
+        if (best == 0) break;
+        int e = 0x7fffffff;
+        if (mine == best) {
+#pragma unroll
+          for (int i = N - 1; i >= 0; --i)
+            if (key[i] == best) e = i * 32 + lane;
+        }
+        const int winner = static_cast<int>(__reduce_min_sync(kAll, static_cast<unsigned>(e)));
+        if (e == winner) {
+          mine = 0;
+#pragma unroll
+          for (int i = 0; i < N; ++i) {
+            if (i * 32 + lane == winner) key[i] = 0;
+            mine = max(mine, key[i]);
+          }
+        }
+        if (lane == j) id = winner;
+      }
+      if (id >= 0) {
+        const float l = clean_logit(load_logit<T>(logits + row * a.stride + id));
+        w = a.sigmoid ? sigmoid_fast(l) : __expf(l - m) * inv;
+        atomicAdd(&s_counts[id], 1);
+      }
+      if (a.renormalize) {
+        const float total = warp_sum(w);
+        w = total > 0.0f ? w / total : 0.0f;
+      }
+      w *= a.scale;
+    }
+    if (lane < a.k) {
+      a.ids[row * a.k + lane] = id;
+      a.weights[row * a.k + lane] = w;
+    }
+  }
+
+  if (lane == 0 && tokens) atomicAdd(&s_tokens, tokens);
+  if (a.balance) {
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      if (i * 32 + lane < a.E) s_psum[warp * a.E + i * 32 + lane] = psum[i];
+  }
+  __syncthreads();
+  for (int e = threadIdx.x; e < a.E; e += blockDim.x) {
+    if (s_counts[e]) atomicAdd(&a.acc_counts[e], s_counts[e]);
+    if (a.balance) {
+      float p = 0.0f;
+      for (int i = 0; i < WARPS; ++i) p += s_psum[i * a.E + e];
+      atomicAdd(&a.psum[e], static_cast<unsigned long long>(__float2ull_rn(p * kFixed)));
+    }
+  }
+  if (threadIdx.x == 0 && s_tokens) atomicAdd(a.acc_tokens, s_tokens);
+  __threadfence();
+  __syncthreads();
+  if (threadIdx.x == 0) s_last = atomicAdd(a.ticket, 1) == static_cast<int>(gridDim.x) - 1;
+  __syncthreads();
+  if (!s_last) return;
+  __threadfence();
+  const volatile int32_t* counts = a.acc_counts;
+  for (int e = threadIdx.x; e < a.E; e += blockDim.x) a.counts[e] = counts[e];
+  const int32_t n = *static_cast<const volatile int32_t*>(a.acc_tokens);
+  if (threadIdx.x == 0) *a.tokens = n;
+  if (a.balance) {
+    const float loss = balance_loss(a, n, a.psum, counts, scratch);
+    if (threadIdx.x == 0) *a.loss = loss;
+  }
+}
+
+struct RouteBwd {
+  const void* logits;
+  int64_t stride;
+  const int32_t* ids;
+  const float* gw;     // [T, k] or null
+  const float* gloss;  // [1] or null
+  const int32_t *counts, *tokens;
+  int64_t T;
+  int E, k;
+  int sigmoid, renormalize;
+  float scale;
+  void* dlogits;
+  int64_t d_stride;
+};
+
+template <typename T>
+__device__ __forceinline__ T grad_cast(float v);
+template <>
+__device__ __forceinline__ float grad_cast(float v) { return v; }
+template <>
+__device__ __forceinline__ __nv_bfloat16 grad_cast(float v) { return __float2bfloat16_rn(v); }
+template <>
+__device__ __forceinline__ __half grad_cast(float v) { return __float2half_rn(v); }
+
+// Dynamic shared memory: one row of E floats per warp, the scattered gradient of the chosen
+// scores (zero between rows).
+template <typename T, int N, int WARPS>
+__global__ void __launch_bounds__(WARPS * 32) moe_route_backward_kernel(const RouteBwd a) {
+  extern __shared__ float s_grad[];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  float* sg = s_grad + warp * a.E;
+  for (int e = lane; e < a.E; e += 32) sg[e] = 0.0f;
+  __syncwarp();
+  float load[N];  // a_e of the lane's experts
+#pragma unroll
+  for (int i = 0; i < N; ++i) load[i] = 0.0f;
+  if (a.gloss) {
+    const float n = static_cast<float>(max(*a.tokens, 1));
+    const float f = *a.gloss * (static_cast<float>(a.E) / static_cast<float>(a.k)) / n / n;
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      if (i * 32 + lane < a.E) load[i] = f * static_cast<float>(a.counts[i * 32 + lane]);
+  }
+  const T* logits = static_cast<const T*>(a.logits);
+  const int64_t step = static_cast<int64_t>(gridDim.x) * WARPS;
+  float next[N];
+  int32_t next_id = -1;
+  float next_g = 0.0f;
+  auto load_row = [&](int64_t row) {
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      next[i] = i * 32 + lane < a.E ? load_logit<T>(logits + row * a.stride + i * 32 + lane) : -INFINITY;
+    if (lane < a.k) {
+      next_id = __ldg(a.ids + row * a.k + lane);
+      if (a.gw) next_g = __ldg(a.gw + row * a.k + lane);
+    }
+  };
+  int64_t row = static_cast<int64_t>(blockIdx.x) * WARPS + warp;
+  if (row < a.T) load_row(row);
+  for (; row < a.T; row += step) {
+    float s[N];
+    float m = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      s[i] = clean_logit(next[i]);
+      m = fmaxf(m, s[i]);
+    }
+    const int32_t id = next_id >= 0 && next_id < a.E ? next_id : -1;
+    float g = id >= 0 ? next_g * a.scale : 0.0f;
+    if (row + step < a.T) load_row(row + step);
+    T* out = static_cast<T*>(a.dlogits) + row * a.d_stride;
+    if (!__any_sync(kAll, id >= 0)) {  // masked token: no gradient
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+        if (i * 32 + lane < a.E) out[i * 32 + lane] = grad_cast<T>(0.0f);
+      continue;
+    }
+    m = a.sigmoid ? 0.0f : key_value(__reduce_max_sync(kAll, order_key(m)));
+    float total = 0.0f;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      s[i] = a.sigmoid ? sigmoid_fast(s[i]) : __expf(s[i] - m);
+      total += s[i];
+    }
+    total = warp_sum(total);
+    const float inv = total > 0.0f ? 1.0f / total : 0.0f;
+    if (!a.sigmoid) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) s[i] *= inv;  // the scores are the probabilities
+    }
+    if (a.gw) {
+      if (a.renormalize) {
+        float c = 0.0f;
+        if (id >= 0) {
+          const float l = clean_logit(load_logit<T>(logits + row * a.stride + id));
+          c = a.sigmoid ? sigmoid_fast(l) : __expf(l - m) * inv;
+        }
+        float chosen = warp_sum(c);
+        chosen = chosen > 0.0f ? 1.0f / chosen : 1.0f;
+        g = (g - warp_sum(g * c) * chosen) * chosen;
+      }
+      if (id >= 0) atomicAdd(&sg[id], g);
+      __syncwarp();
+    }
+    float d[N];
+    float dot = 0.0f;  // of what meets the probabilities: everything (softmax) or the loss alone
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      d[i] = a.gw && i * 32 + lane < a.E ? sg[i * 32 + lane] : 0.0f;
+      dot = fmaf(a.sigmoid ? load[i] : d[i] + load[i], s[i], dot);
+    }
+    dot = warp_sum(dot);
+    if (a.gw) {
+      __syncwarp();
+      if (id >= 0) sg[id] = 0.0f;
+      __syncwarp();
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      float v;
+      if (a.sigmoid)
+        v = (d[i] + (load[i] - dot * inv) * inv) * s[i] * (1.0f - s[i]);
+      else
+        v = s[i] * (d[i] + load[i] - dot);
+      if (i * 32 + lane < a.E) out[i * 32 + lane] = grad_cast<T>(v);
+    }
+  }
+}
+
+constexpr int kRouteWarps = 8;
+
+int route_sms() {
+  int dev = 0, n = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
+    return 148;
+  return n > 0 ? n : 148;
+}
+
+// CTAs per SM by registers: N experts per lane take about 4N registers of a thread.
+int route_ctas_per_sm(int n) { return n <= 8 ? 6 : n <= 16 ? 4 : 2; }
+
+template <typename T, int N>
+int launch_route(const Route& a, cudaStream_t st) {
+  const int64_t ctas = (a.T + kRouteWarps - 1) / kRouteWarps;
+  const unsigned grid = static_cast<unsigned>(std::min<int64_t>(ctas, int64_t(route_sms()) * route_ctas_per_sm(N)));
+  const size_t smem = a.E * 4 + (a.balance ? size_t(kRouteWarps) * a.E * 4 : 0);
+  moe_route_kernel<T, N, kRouteWarps><<<grid, kRouteWarps * 32, smem, st>>>(a);
+  return cudaGetLastError() == cudaSuccess ? CDG_OK : CDG_ERR_CUDA;
+}
+
+template <typename T, int N>
+int launch_route_backward(const RouteBwd& a, cudaStream_t st) {
+  const int64_t ctas = (a.T + kRouteWarps - 1) / kRouteWarps;
+  const unsigned grid = static_cast<unsigned>(std::min<int64_t>(ctas, int64_t(route_sms()) * route_ctas_per_sm(N)));
+  moe_route_backward_kernel<T, N, kRouteWarps><<<grid, kRouteWarps * 32, size_t(kRouteWarps) * a.E * 4, st>>>(a);
+  return cudaGetLastError() == cudaSuccess ? CDG_OK : CDG_ERR_CUDA;
+}
+
+template <typename T>
+int dispatch_route(const Route& a, cudaStream_t st) {
+  const int n = (a.E + 31) / 32;
+  if (n <= 1) return launch_route<T, 1>(a, st);
+  if (n <= 2) return launch_route<T, 2>(a, st);
+  if (n <= 4) return launch_route<T, 4>(a, st);
+  if (n <= 8) return launch_route<T, 8>(a, st);
+  if (n <= 16) return launch_route<T, 16>(a, st);
+  return launch_route<T, 32>(a, st);
+}
+
+template <typename T>
+int dispatch_route_backward(const RouteBwd& a, cudaStream_t st) {
+  const int n = (a.E + 31) / 32;
+  if (n <= 1) return launch_route_backward<T, 1>(a, st);
+  if (n <= 2) return launch_route_backward<T, 2>(a, st);
+  if (n <= 4) return launch_route_backward<T, 4>(a, st);
+  if (n <= 8) return launch_route_backward<T, 8>(a, st);
+  if (n <= 16) return launch_route_backward<T, 16>(a, st);
+  return launch_route_backward<T, 32>(a, st);
+}
+
+bool logit_dtype(int dtype) { return dtype == CDG_DTYPE_BF16 || dtype == CDG_DTYPE_F16 || dtype == CDG_DTYPE_F32; }
+
+}  // namespace
+}  // namespace cdg
+
+extern "C" {
+
+size_t cdg_moe_route_workspace_bytes(int64_t E) {
+  if (E <= 0 || E > cdg::kRouteMaxExperts) return 0;
+  return static_cast<size_t>(E) * 12 + 8;
+}
+
+int cdg_moe_route(const cdg_route_args* g, void* workspace, size_t workspace_bytes, cdg_stream_t stream) {
+  using namespace cdg;
+  if (!g || g->T < 0 || g->E <= 0 || g->topk <= 0 || g->topk > g->E || !logit_dtype(g->dtype))
+    return CDG_ERR_INVALID_ARGUMENT;
+  if (g->scoring != CDG_SCORE_SOFTMAX && g->scoring != CDG_SCORE_SIGMOID) return CDG_ERR_INVALID_ARGUMENT;
+  if (g->E > kRouteMaxExperts || g->topk > kRouteMaxTopk || g->T > kRouteMaxTokens) return CDG_ERR_UNSUPPORTED;
+  if (!g->counts || !g->tokens || (g->T > 0 && (!g->logits || !g->weights || !g->ids))) return CDG_ERR_INVALID_ARGUMENT;
+  if (!workspace || workspace_bytes < cdg_moe_route_workspace_bytes(g->E)) return CDG_ERR_WORKSPACE;
+  if (reinterpret_cast<uintptr_t>(workspace) % 8) return CDG_ERR_ALIGNMENT;
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  if (g->T == 0) {
+    if (cudaMemsetAsync(g->counts, 0, g->E * sizeof(int32_t), st) != cudaSuccess ||
+        cudaMemsetAsync(g->tokens, 0, sizeof(int32_t), st) != cudaSuccess ||
+        (g->loss && cudaMemsetAsync(g->loss, 0, sizeof(float), st) != cudaSuccess))
+      return CDG_ERR_CUDA;
+    return CDG_OK;
+  }
+  if (cudaMemsetAsync(workspace, 0, cdg_moe_route_workspace_bytes(g->E), st) != cudaSuccess) return CDG_ERR_CUDA;
+  Route a{};
+  a.logits = g->logits;
+  a.stride = g->stride;
+  a.mask = g->token_mask;
+  a.bias = g->bias;
+  a.T = g->T;
+  a.E = static_cast<int>(g->E);
+  a.k = static_cast<int>(g->topk);
+  a.sigmoid = g->scoring == CDG_SCORE_SIGMOID;
+  a.renormalize = g->renormalize != 0;
+  a.balance = g->loss != nullptr;
+  a.scale = g->scale;
+  a.weights = g->weights;
+  a.ids = g->ids;
+  a.counts = g->counts;
+  a.tokens = g->tokens;
+  a.loss = g->loss;
+  a.psum = static_cast<unsigned long long*>(workspace);
+  a.acc_counts = reinterpret_cast<int32_t*>(a.psum + a.E);
+  a.acc_tokens = a.acc_counts + a.E;
+  a.ticket = a.acc_tokens + 1;
+  if (g->dtype == CDG_DTYPE_BF16) return dispatch_route<__nv_bfloat16>(a, st);
+  if (g->dtype == CDG_DTYPE_F16) return dispatch_route<__half>(a, st);
+  return dispatch_route<float>(a, st);
+}
+
+int cdg_moe_route_backward(const cdg_route_backward_args* g, cdg_stream_t stream) {
+  using namespace cdg;
+  if (!g || g->T < 0 || g->E <= 0 || g->topk <= 0 || g->topk > g->E || !logit_dtype(g->dtype))
+    return CDG_ERR_INVALID_ARGUMENT;
+  if (g->scoring != CDG_SCORE_SOFTMAX && g->scoring != CDG_SCORE_SIGMOID) return CDG_ERR_INVALID_ARGUMENT;
+  if (g->E > kRouteMaxExperts || g->topk > kRouteMaxTopk || g->T > kRouteMaxTokens) return CDG_ERR_UNSUPPORTED;
+  if (g->grad_loss && (!g->counts || !g->tokens)) return CDG_ERR_INVALID_ARGUMENT;
+  if (g->T == 0) return CDG_OK;
+  if (!g->logits || !g->ids || !g->dlogits || (!g->grad_weights && !g->grad_loss)) return CDG_ERR_INVALID_ARGUMENT;
+  RouteBwd a{g->logits, g->stride, g->ids, g->grad_weights, g->grad_loss, g->counts, g->tokens, g->T,
+             static_cast<int>(g->E), static_cast<int>(g->topk), g->scoring == CDG_SCORE_SIGMOID, g->renormalize != 0,
+             g->scale, g->dlogits, g->d_stride};
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  if (g->dtype == CDG_DTYPE_BF16) return dispatch_route_backward<__nv_bfloat16>(a, st);
+  if (g->dtype == CDG_DTYPE_F16) return dispatch_route_backward<__half>(a, st);
+  return dispatch_route_backward<float>(a, st);
+}
+
+}  // extern "C"

@@ -729,6 +729,113 @@ std::vector<torch::Tensor> rms_norm_backward(const torch::Tensor& dy, const torc
   return {dx, dw};
 }
 
+void check_logits(const torch::Tensor& t, const torch::Device& dev) {
+  check_cuda(t, "logits", dev);
+  TORCH_CHECK_VALUE(t.dim() == 2 && t.size(1) > 0, "logits must be [T, E] with E > 0, got ", t.sizes());
+  TORCH_CHECK_VALUE(float_rows(t), "logits must be BF16/FP16/FP32, got ", t.scalar_type());
+  check_rows(t, "logits", dev, t.size(0), t.size(1));
+}
+
+// (weights, ids, counts, tokens, loss or None)
+py::tuple moe_route(const torch::Tensor& logits, int64_t topk, bool sigmoid, bool renormalize, double scale,
+                    const c10::optional<torch::Tensor>& bias, const c10::optional<torch::Tensor>& mask, bool balance) {
+  const auto dev = logits.device();
+  check_logits(logits, dev);
+  const int64_t T = logits.size(0), E = logits.size(1);
+  TORCH_CHECK_VALUE(topk > 0 && topk <= E, "topk must lie in [1, E], got ", topk);
+  cdg_route_args g{};
+  if (bias.has_value()) {
+    check_vector(*bias, "bias", dev, E);
+    TORCH_CHECK_VALUE(bias->scalar_type() == torch::kFloat32, "bias must be FP32, got ", bias->scalar_type());
+    g.bias = bias->data_ptr<float>();
+  }
+  if (mask.has_value()) {
+    check_vector(*mask, "token_mask", dev, T);
+    TORCH_CHECK_VALUE(mask->scalar_type() == torch::kBool || mask->scalar_type() == torch::kUInt8,
+                      "token_mask must be bool or uint8, got ", mask->scalar_type());
+    g.token_mask = static_cast<const uint8_t*>(mask->data_ptr());
+  }
+  const c10::cuda::CUDAGuard guard(dev);
+  auto f32 = logits.options().dtype(torch::kFloat32);
+  auto i32 = logits.options().dtype(torch::kInt32);
+  auto weights = torch::empty({T, topk}, f32);
+  auto ids = torch::empty({T, topk}, i32);
+  auto counts = torch::empty({E}, i32);
+  auto tokens = torch::empty({1}, i32);
+  torch::Tensor loss;
+  if (balance) {
+    loss = torch::empty({1}, f32);
+    g.loss = loss.data_ptr<float>();
+  }
+  const size_t ws_bytes = cdg_moe_route_workspace_bytes(E);
+  auto ws = torch::empty({static_cast<int64_t>(ws_bytes)}, logits.options().dtype(torch::kUInt8));
+  g.logits = logits.data_ptr();
+  g.stride = logits.stride(0);
+  g.dtype = dtype_code(logits);
+  g.scoring = sigmoid ? CDG_SCORE_SIGMOID : CDG_SCORE_SOFTMAX;
+  g.T = T;
+  g.E = E;
+  g.topk = topk;
+  g.renormalize = renormalize ? 1 : 0;
+  g.scale = static_cast<float>(scale);
+  g.weights = weights.data_ptr<float>();
+  g.ids = ids.data_ptr<int32_t>();
+  g.counts = counts.data_ptr<int32_t>();
+  g.tokens = tokens.data_ptr<int32_t>();
+  check_status(cdg_moe_route(&g, ws_bytes ? ws.data_ptr() : nullptr, ws_bytes, cur_stream(logits)), "moe_route");
+  return py::make_tuple(weights, ids, counts, tokens, balance ? py::cast(loss) : py::none());
+}
+
+torch::Tensor moe_route_backward(const torch::Tensor& logits, const torch::Tensor& ids,
+                                 const c10::optional<torch::Tensor>& gw, const c10::optional<torch::Tensor>& gl,
+                                 const c10::optional<torch::Tensor>& counts, const c10::optional<torch::Tensor>& tokens,
+                                 bool sigmoid, bool renormalize, double scale) {
+  const auto dev = logits.device();
+  check_logits(logits, dev);
+  const int64_t T = logits.size(0), E = logits.size(1);
+  check_cuda(ids, "ids", dev);
+  TORCH_CHECK_VALUE(ids.dim() == 2 && ids.size(0) == T && ids.is_contiguous() && ids.scalar_type() == torch::kInt32 &&
+                        ids.size(1) > 0 && ids.size(1) <= E,
+                    "ids must be contiguous int32 [T, topk]");
+  TORCH_CHECK_VALUE(gw.has_value() || gl.has_value(), "nothing to go back from: grad_weights and grad_loss are both None");
+  cdg_route_backward_args g{};
+  if (gw.has_value()) {
+    check_cuda(*gw, "grad_weights", dev);
+    TORCH_CHECK_VALUE(gw->sizes() == ids.sizes() && gw->is_contiguous() && gw->scalar_type() == torch::kFloat32,
+                      "grad_weights must be contiguous FP32 [T, topk]");
+    g.grad_weights = gw->data_ptr<float>();
+  }
+  if (gl.has_value()) {
+    check_cuda(*gl, "grad_loss", dev);
+    TORCH_CHECK_VALUE(gl->numel() == 1 && gl->scalar_type() == torch::kFloat32, "grad_loss must be one FP32 value");
+    TORCH_CHECK_VALUE(counts.has_value() && tokens.has_value(), "grad_loss needs the forward call's counts and tokens");
+    check_vector(*counts, "counts", dev, E);
+    check_cuda(*tokens, "tokens", dev);
+    TORCH_CHECK_VALUE(counts->scalar_type() == torch::kInt32 && tokens->scalar_type() == torch::kInt32 &&
+                          tokens->numel() == 1,
+                      "counts must be int32 [E], tokens one int32");
+    g.grad_loss = gl->data_ptr<float>();
+    g.counts = counts->data_ptr<int32_t>();
+    g.tokens = tokens->data_ptr<int32_t>();
+  }
+  const c10::cuda::CUDAGuard guard(dev);
+  auto out = torch::empty({T, E}, logits.options());
+  g.logits = logits.data_ptr();
+  g.stride = logits.stride(0);
+  g.dtype = dtype_code(logits);
+  g.scoring = sigmoid ? CDG_SCORE_SIGMOID : CDG_SCORE_SOFTMAX;
+  g.ids = ids.data_ptr<int32_t>();
+  g.T = T;
+  g.E = E;
+  g.topk = ids.size(1);
+  g.renormalize = renormalize ? 1 : 0;
+  g.scale = static_cast<float>(scale);
+  g.dlogits = out.data_ptr();
+  g.d_stride = E;
+  check_status(cdg_moe_route_backward(&g, cur_stream(logits)), "moe_route_backward");
+  return out;
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -832,4 +939,9 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         py::arg("quantize"), py::arg("ue8m0"), py::arg("normed"));
   m.def("rms_norm_backward", &rms_norm_backward, py::arg("dy"), py::arg("h"), py::arg("weight"), py::arg("dh"),
         py::arg("eps"));
+  m.def("moe_route", &moe_route, py::arg("logits"), py::arg("topk"), py::arg("sigmoid"), py::arg("renormalize"),
+        py::arg("scale"), py::arg("bias"), py::arg("token_mask"), py::arg("balance"));
+  m.def("moe_route_backward", &moe_route_backward, py::arg("logits"), py::arg("ids"), py::arg("grad_weights"),
+        py::arg("grad_loss"), py::arg("counts"), py::arg("tokens"), py::arg("sigmoid"), py::arg("renormalize"),
+        py::arg("scale"));
 }

@@ -542,6 +542,63 @@ size_t cdg_rms_norm_backward_workspace_bytes(int64_t T, int64_t H);
 int cdg_rms_norm_backward(const cdg_norm_backward_args* args, void* workspace, size_t workspace_bytes,
                           cdg_stream_t stream);
 
+/* Router: top-k gate, rows per expert and balance loss.  For each token (row of E logits) that
+ * token_mask keeps and that has an expert above -inf (logit, and bias where given):
+ *   score = softmax(logits) or sigmoid(logits), p = score / sum(score);
+ *   ids = the topk largest logits (with a bias: the topk largest score + bias), ties to the lowest
+ *   index; weights = scale * score[ids], divided by their sum before scaling if renormalize.
+ * A masked token, and a slot for which no logit above -inf is left, gets id -1 and weight 0 (the
+ * MoE layer's "no expert").  NaN logits count as -inf, +inf as the largest finite value.
+ * counts[e] = tokens that chose e, *tokens = V = valid tokens, and, unless loss is NULL,
+ *   *loss = E / (topk V^2) * sum over e of counts[e] * (sum over valid tokens of p[e]),
+ * 1 where the experts share rows and probabilities evenly, 0 without a valid token.  The sums
+ * over tokens do not depend on the order in which CTAs finish.
+ * E up to 1024, topk up to 32, T up to 2^23. */
+#define CDG_SCORE_SOFTMAX 0
+#define CDG_SCORE_SIGMOID 1
+
+typedef struct cdg_route_args {
+  const void* logits; /* [T, E] of dtype (BF16, F16 or F32) */
+  int64_t stride;
+  int32_t dtype, scoring; /* CDG_SCORE_* */
+  const uint8_t* token_mask; /* [T], nonzero = a token; NULL = all */
+  const float* bias;         /* [E]; NULL = none.  For the choice alone */
+  int64_t T, E, topk;
+  int32_t renormalize;
+  float scale;
+  float* weights;  /* [T, topk] */
+  int32_t* ids;    /* [T, topk] */
+  int32_t* counts; /* [E] */
+  int32_t* tokens; /* [1] */
+  float* loss;     /* [1] or NULL */
+} cdg_route_args;
+
+size_t cdg_moe_route_workspace_bytes(int64_t E);
+int cdg_moe_route(const cdg_route_args* args, void* workspace, size_t workspace_bytes, cdg_stream_t stream);
+
+/* Gradient of the router with respect to the logits, from the gradients of the weights
+ * (grad_weights, [T, topk], may be NULL) and of the loss (grad_loss, [1] on the device, may be
+ * NULL; then counts and tokens are not read).  ids, counts and tokens are the forward call's; the
+ * choice and the counts are held fixed.  A row whose ids are all -1 gets zeros, and so does an
+ * expert whose logit is -inf; ids outside [0, E) are passed over. */
+typedef struct cdg_route_backward_args {
+  const void* logits;
+  int64_t stride;
+  int32_t dtype, scoring;
+  const int32_t* ids;
+  const float* grad_weights;
+  const float* grad_loss;
+  const int32_t* counts;
+  const int32_t* tokens;
+  int64_t T, E, topk;
+  int32_t renormalize;
+  float scale;
+  void* dlogits; /* [T, E] of dtype */
+  int64_t d_stride;
+} cdg_route_backward_args;
+
+int cdg_moe_route_backward(const cdg_route_backward_args* args, cdg_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif
