@@ -15,6 +15,7 @@ from .layout import (
     set_mk_alignment_for_contiguous_layout,
     transform_sf_into_required_layout,
 )
+from .linear import linear, linear_backward
 from .mega import fp8_fp4_mega_moe, get_symm_buffer_for_mega_moe, transform_weights_for_mega_moe
 from .native import build_info as native_build_info
 from .native import check_device_status, read_device_status
@@ -32,6 +33,8 @@ __all__ = [
     "transform_weights_for_mega_moe",
     "add_rms_norm",
     "add_rms_norm_backward",
+    "linear",
+    "linear_backward",
     "moe_route",
     "moe_route_backward",
     "get_symm_buffer_for_mega_moe",

@@ -1,0 +1,428 @@
+// Host side of the dense product (cdg_linear, cdg_linear_backward) and its elementwise kernels.
+//
+//   forward   y = act(x W^T + b) + r                                   one product
+//   backward  dz = dy * act'(z), db = sum over rows of dz, dx = dz W, dW = dz^T x
+//             one elementwise pass (dz in the operands' 16 bits, since it is an operand of both
+//             products; db from its 32-bit values), then two products that read W and dz across
+//             their rows (MN-major operands), so nothing is transposed in memory
+//
+// Operands whose rows do not start on 16-byte boundaries cannot be loaded by TMA: they are copied
+// once into the workspace with padded rows.
+#include <cuda.h>
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <cstdint>
+#include <mutex>
+
+#include "cdg_b200.h"
+#include "cdg_linear.cuh"
+
+namespace cdg {
+namespace {
+
+using EncodeTiledFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                                   const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                                   CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+EncodeTiledFn encode_tiled() {
+  static EncodeTiledFn fn = [] {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult q{};
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) != cudaSuccess ||
+        q != cudaDriverEntryPointSuccess)
+      p = nullptr;
+    return reinterpret_cast<EncodeTiledFn>(p);
+  }();
+  return fn;
+}
+
+// Copies rows of 16-bit values to rows of `out_stride` columns, zeros past `cols`.
+__global__ void __launch_bounds__(256) repack_rows_kernel(const uint16_t* in, int64_t in_stride, int64_t rows,
+                                                          int64_t cols, uint16_t* out, int64_t out_stride) {
+  const int64_t words = out_stride / 8, total = rows * words;
+  for (int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; i < total;
+       i += static_cast<int64_t>(gridDim.x) * blockDim.x) {
+    const int64_t r = i / words, c = (i - r * words) * 8;
+    const uint16_t* p = in + r * in_stride + c;
+    uint32_t w[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const uint32_t lo = c + 2 * j < cols ? p[2 * j] : 0, hi = c + 2 * j + 1 < cols ? p[2 * j + 1] : 0;
+      w[j] = lo | (hi << 16);
+    }
+    *reinterpret_cast<uint4*>(out + r * out_stride + c) = make_uint4(w[0], w[1], w[2], w[3]);
+  }
+}
+
+// dz = dy * act'(z) and partial column sums of it.  A CTA takes 256 columns (eight per lane of
+// each of its eight warps) and every gridDim.y-th group of eight rows; its sums go to
+// partial[blockIdx.y][N].  dz or partial may be NULL.
+template <typename T, bool WIDE>
+__global__ void __launch_bounds__(256) linear_dz_kernel(const T* dy, int64_t dy_stride, const T* z, int64_t z_stride,
+                                                        int act, int64_t M, int64_t N, T* dz, int64_t dz_stride,
+                                                        float* partial) {
+  __shared__ float sums[8][256];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int64_t chunk = blockIdx.x;
+  float acc[8] = {};
+  for (int64_t m = static_cast<int64_t>(blockIdx.y) * 8 + warp; m < M; m += static_cast<int64_t>(gridDim.y) * 8) {
+    float g[8];
+    unpack8<T>(load8<T, WIDE>(dy + m * dy_stride, chunk, lane, N), g);
+    if (z) {
+      float v[8];
+      unpack8<T>(load8<T, WIDE>(z + m * z_stride, chunk, lane, N), v);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) g[j] *= activate_slope(v[j], act);
+    }
+    if (dz) store8<T, WIDE>(dz + m * dz_stride, chunk, lane, N, g);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) acc[j] += g[j];
+  }
+  if (!partial) return;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) sums[warp][column<WIDE>(0, lane, j)] = acc[j];
+  __syncthreads();
+  const int64_t n = chunk * 256 + threadIdx.x;
+  if (n < N) {
+    float v = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v += sums[i][threadIdx.x];
+    partial[static_cast<int64_t>(blockIdx.y) * N + n] = v;
+  }
+}
+
+// ------------------------------------------------------------------ host
+constexpr int kMaxDevices = 64;
+
+template <typename T, typename O, int BN, bool PROMOTE>
+bool allow_smem() {
+  return cudaFuncSetAttribute(cdg_linear_tile_kernel<T, O, BN, PROMOTE>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                              TileSmem<BN, PROMOTE>::kBytes) == cudaSuccess;
+}
+
+template <typename T>
+bool allow_smem_of() {
+  return allow_smem<T, T, 64, false>() && allow_smem<T, T, 128, false>() && allow_smem<T, float, 64, true>() &&
+         allow_smem<T, float, 128, true>();
+}
+
+// Compute capability and kernel attributes, once per device.
+int device_ready() {
+  static std::once_flag flags[kMaxDevices];
+  static int state[kMaxDevices];
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) return CDG_ERR_CUDA;
+  std::call_once(flags[dev], [dev] {
+    int major = 0;
+    if (cudaDeviceGetAttribute(&major, cudaDevAttrComputeCapabilityMajor, dev) != cudaSuccess)
+      state[dev] = CDG_ERR_CUDA;
+    else if (major != 10)
+      state[dev] = CDG_ERR_NO_SM100;
+    else
+      state[dev] = allow_smem_of<__nv_bfloat16>() && allow_smem_of<__half>() ? CDG_OK : CDG_ERR_CUDA;
+  });
+  return state[dev];
+}
+
+// A 16-bit matrix as it lies in memory: `rows` rows of `cols` columns.
+struct Matrix {
+  const void* p;
+  int64_t stride, rows, cols;
+};
+
+int64_t padded(int64_t cols) { return (cols + 7) / 8 * 8; }
+
+// Rows that TMA can load: on 16-byte boundaries and apart (a broadcast row has stride 0).
+bool tma_rows(const Matrix& m) {
+  return m.rows == 0 || (reinterpret_cast<uintptr_t>(m.p) % 16 == 0 &&
+                         (m.rows == 1 || (m.stride % 8 == 0 && m.stride >= m.cols)));
+}
+
+size_t repack_bytes(const Matrix& m) {
+  return tma_rows(m) ? 0 : (static_cast<size_t>(m.rows) * padded(m.cols) * 2 + 255) / 256 * 256;
+}
+
+int repack(Matrix& m, uint8_t*& ws, cudaStream_t st) {
+  if (tma_rows(m)) return CDG_OK;
+  const size_t bytes = repack_bytes(m);
+  const int64_t stride = padded(m.cols), total = m.rows * stride / 8;
+  const unsigned grid = static_cast<unsigned>(std::min<int64_t>((total + 255) / 256, int64_t(sm_count()) * 16));
+  repack_rows_kernel<<<grid, 256, 0, st>>>(static_cast<const uint16_t*>(m.p), m.stride, m.rows, m.cols,
+                                           reinterpret_cast<uint16_t*>(ws), stride);
+  m.p = ws;
+  m.stride = stride;
+  ws += bytes;
+  return launched();
+}
+
+int make_map(CUtensorMap* map, const Matrix& m, bool bf16, uint32_t box_rows) {
+  EncodeTiledFn enc = encode_tiled();
+  if (!enc) return CDG_ERR_CUDA;
+  cuuint64_t dims[2] = {static_cast<cuuint64_t>(m.cols), static_cast<cuuint64_t>(m.rows)};
+  // one row may have any stride; the map wants a multiple of 16 bytes all the same
+  cuuint64_t strides[1] = {static_cast<cuuint64_t>(m.rows > 1 ? m.stride : padded(m.cols)) * 2};
+  cuuint32_t box[2] = {64, box_rows};
+  cuuint32_t estr[2] = {1, 1};
+  return enc(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2,
+             const_cast<void*>(m.p), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+             CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS
+             ? CDG_OK
+             : CDG_ERR_CUDA;
+}
+
+template <typename T, typename O, int BN, bool PROMOTE>
+int launch_tiles(const CUtensorMap& ta, const CUtensorMap& tb, const LinearShape& s, const Epilogue& e, int splits,
+                 cudaStream_t st) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(static_cast<unsigned>(s.m_tiles) * s.n_tiles * splits);
+  cfg.blockDim = dim3(kTileThreads);
+  cfg.dynamicSmemBytes = TileSmem<BN, PROMOTE>::kBytes;
+  cfg.stream = st;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = splits;
+  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, cdg_linear_tile_kernel<T, O, BN, PROMOTE>, ta, tb, s, e, splits) == cudaSuccess
+             ? CDG_OK
+             : CDG_ERR_CUDA;
+}
+
+// D [M, N] = epilogue(sum over K of A and B); a_mn: A lies as [K, M], else [M, K]; b_mn: B lies as
+// [K, N], else [N, K].  Rows of both on 16-byte boundaries.
+template <typename T, typename O>
+int product(const Matrix& A, bool a_mn, const Matrix& B, bool b_mn, int64_t M, int64_t N, int64_t K,
+            const Epilogue& e, cudaStream_t st) {
+  constexpr bool kPromote = sizeof(O) == 4;
+  constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
+  if (M == 0 || N == 0) return CDG_OK;
+  LinearShape s{};
+  s.M = M;
+  s.N = N;
+  s.k_steps = static_cast<int>((K + 63) / 64);
+  s.a_mn = a_mn;
+  s.b_mn = b_mn;
+  s.bf16 = kBf16;
+  s.a_rows = static_cast<int>(std::min<int64_t>(128, (M + 7) / 8 * 8));
+  const int64_t m_tiles = (M + 127) / 128;
+  const int sms = sm_count();
+  const int bn = m_tiles * ((N + 127) / 128) >= sms ? 128 : 64;
+  const int64_t n_tiles = (N + bn - 1) / bn;
+  if (m_tiles * n_tiles * 8 > 0x7fffffff) return CDG_ERR_UNSUPPORTED;
+  s.m_tiles = static_cast<int>(m_tiles);
+  s.n_tiles = static_cast<int>(n_tiles);
+  // K is split while the tiles leave SMs without work and each part keeps four K steps
+  int splits = 1;
+  while (splits < 8 && m_tiles * n_tiles * splits * 2 <= 2 * sms && s.k_steps / (splits * 2) >= 4) splits *= 2;
+  CUtensorMap ta{}, tb{};
+  if (K > 0) {
+    int rc = make_map(&ta, A, kBf16, a_mn ? 64 : s.a_rows);
+    if (rc == CDG_OK) rc = make_map(&tb, B, kBf16, b_mn ? 64 : bn);
+    if (rc != CDG_OK) return rc;
+  }
+  return bn == 128 ? launch_tiles<T, O, 128, kPromote>(ta, tb, s, e, splits, st)
+                   : launch_tiles<T, O, 64, kPromote>(ta, tb, s, e, splits, st);
+}
+
+bool operand_dtype(int dtype) { return dtype == CDG_DTYPE_BF16 || dtype == CDG_DTYPE_F16; }
+
+bool sizes_ok(int64_t M, int64_t N, int64_t K) {
+  return M <= (int64_t(1) << 30) && N <= (int64_t(1) << 30) && K <= (int64_t(1) << 30);
+}
+
+// 16-byte rows of an output or residual that the epilogue reads and writes eight columns at a time.
+bool wide_columns(const void* p, int64_t stride, int64_t bytes) { return wide_rows(p, stride, bytes); }
+
+template <typename T>
+int forward(const cdg_linear_args* g, uint8_t* ws, cudaStream_t st) {
+  Matrix x{g->x, g->x_stride, g->M, g->K}, w{g->w, g->w_stride, g->N, g->K};
+  int rc = CDG_OK;
+  if (g->K > 0) {
+    rc = repack(x, ws, st);
+    if (rc == CDG_OK) rc = repack(w, ws, st);
+    if (rc != CDG_OK) return rc;
+  }
+  Epilogue e{};
+  e.bias = g->bias;
+  e.bias_f32 = g->bias_dtype == CDG_DTYPE_F32;
+  e.residual = g->residual;
+  e.residual_stride = g->residual_stride;
+  e.residual_f32 = g->residual_dtype == CDG_DTYPE_F32;
+  e.act = g->activation;
+  e.y = g->y;
+  e.y_stride = g->y_stride;
+  e.z = g->z_out;
+  e.z_stride = g->z_stride;
+  e.wide = wide_columns(e.y, e.y_stride, element_size(g->out_dtype)) && wide_columns(e.z, e.z_stride, 2) &&
+           wide_columns(e.residual, e.residual_stride, e.residual_f32 ? 4 : 2);
+  return g->out_dtype == CDG_DTYPE_F32 ? product<T, float>(x, false, w, false, g->M, g->N, g->K, e, st)
+                                       : product<T, T>(x, false, w, false, g->M, g->N, g->K, e, st);
+}
+
+// Row groups of the elementwise backward pass: a few CTAs per SM, each summing many rows.
+int dz_groups(int64_t M, int64_t N) {
+  const int64_t chunks = std::max<int64_t>(1, (N + 255) / 256);
+  const int64_t want = std::max<int64_t>(1, int64_t(sm_count()) * 4 / chunks);
+  return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({want, (M + 7) / 8, 1024})));
+}
+
+bool needs_dz(const cdg_linear_backward_args* g) {
+  return g->activation != CDG_ACT_NONE || !tma_rows(Matrix{g->dy, g->dy_stride, g->M, g->N});
+}
+
+size_t align256(size_t n) { return (n + 255) / 256 * 256; }
+
+template <typename T>
+int backward(const cdg_linear_backward_args* g, uint8_t* ws, cudaStream_t st) {
+  Matrix x{g->x, g->x_stride, g->M, g->K}, w{g->w, g->w_stride, g->N, g->K};
+  Matrix dz{g->dy, g->dy_stride, g->M, g->N};
+  const bool store = needs_dz(g) && (g->dx || g->dw);
+  if ((store || g->db) && g->M > 0) {
+    T* out = nullptr;
+    const int64_t stride = padded(g->N);
+    if (store) {
+      out = reinterpret_cast<T*>(ws);
+      ws += align256(static_cast<size_t>(g->M) * stride * 2);
+    }
+    const int groups = dz_groups(g->M, g->N);
+    float* partial = nullptr;
+    if (g->db) {
+      partial = reinterpret_cast<float*>(ws);
+      ws += align256(static_cast<size_t>(groups) * g->N * 4);
+    }
+    const T* z = g->activation != CDG_ACT_NONE ? static_cast<const T*>(g->z) : nullptr;
+    const bool wide = g->N % 8 == 0 && wide_rows(g->dy, g->dy_stride, 2) && (!z || wide_rows(z, g->z_stride, 2));
+    const dim3 grid(static_cast<unsigned>((g->N + 255) / 256), static_cast<unsigned>(groups));
+    if (wide)
+      linear_dz_kernel<T, true><<<grid, 256, 0, st>>>(static_cast<const T*>(g->dy), g->dy_stride, z, g->z_stride,
+                                                      g->activation, g->M, g->N, out, stride, partial);
+    else
+      linear_dz_kernel<T, false><<<grid, 256, 0, st>>>(static_cast<const T*>(g->dy), g->dy_stride, z, g->z_stride,
+                                                       g->activation, g->M, g->N, out, stride, partial);
+    int rc = launched();
+    if (rc != CDG_OK) return rc;
+    if (g->db) {
+      const unsigned blocks = static_cast<unsigned>((g->N + 31) / 32);
+      if (g->db_dtype == CDG_DTYPE_F32)
+        column_sum_kernel<float><<<blocks, 256, 0, st>>>(partial, groups, g->N, static_cast<float*>(g->db));
+      else
+        column_sum_kernel<T><<<blocks, 256, 0, st>>>(partial, groups, g->N, static_cast<T*>(g->db));
+      rc = launched();
+      if (rc != CDG_OK) return rc;
+    }
+    if (store) {
+      dz.p = out;
+      dz.stride = stride;
+    }
+  } else if (g->db) {
+    if (cudaMemsetAsync(g->db, 0, g->N * element_size(g->db_dtype), st) != cudaSuccess) return CDG_ERR_CUDA;
+  }
+  if (g->dx) {
+    int rc = g->N > 0 && g->M > 0 ? repack(w, ws, st) : CDG_OK;
+    Epilogue e{};
+    e.y = g->dx;
+    e.y_stride = g->dx_stride;
+    e.wide = wide_columns(e.y, e.y_stride, 2);
+    if (rc == CDG_OK) rc = product<T, T>(dz, false, w, true, g->M, g->K, g->N, e, st);
+    if (rc != CDG_OK) return rc;
+  }
+  if (g->dw) {
+    int rc = g->M > 0 ? repack(x, ws, st) : CDG_OK;
+    Epilogue e{};
+    e.y = g->dw;
+    e.y_stride = g->dw_stride;
+    e.wide = wide_columns(e.y, e.y_stride, 2);
+    if (rc == CDG_OK) rc = product<T, T>(dz, true, x, true, g->N, g->K, g->M, e, st);
+    if (rc != CDG_OK) return rc;
+  }
+  return CDG_OK;
+}
+
+int check_forward(const cdg_linear_args* g) {
+  if (!g || g->M < 0 || g->N < 0 || g->K < 0 || !operand_dtype(g->dtype)) return CDG_ERR_INVALID_ARGUMENT;
+  if (g->out_dtype != g->dtype && g->out_dtype != CDG_DTYPE_F32) return CDG_ERR_INVALID_ARGUMENT;
+  if (g->activation < CDG_ACT_NONE || g->activation > CDG_ACT_GELU_TANH) return CDG_ERR_INVALID_ARGUMENT;
+  if (g->bias && g->bias_dtype != g->dtype && g->bias_dtype != CDG_DTYPE_F32) return CDG_ERR_INVALID_ARGUMENT;
+  if (g->residual && g->residual_dtype != g->dtype && g->residual_dtype != CDG_DTYPE_F32)
+    return CDG_ERR_INVALID_ARGUMENT;
+  if (g->M > 0 && g->N > 0 && (!g->y || (g->K > 0 && (!g->x || !g->w)))) return CDG_ERR_INVALID_ARGUMENT;
+  return sizes_ok(g->M, g->N, g->K) ? CDG_OK : CDG_ERR_UNSUPPORTED;
+}
+
+int check_backward(const cdg_linear_backward_args* g) {
+  if (!g || g->M < 0 || g->N < 0 || g->K < 0 || !operand_dtype(g->dtype)) return CDG_ERR_INVALID_ARGUMENT;
+  if (g->activation < CDG_ACT_NONE || g->activation > CDG_ACT_GELU_TANH) return CDG_ERR_INVALID_ARGUMENT;
+  if (g->db && g->db_dtype != g->dtype && g->db_dtype != CDG_DTYPE_F32) return CDG_ERR_INVALID_ARGUMENT;
+  if (g->M > 0 && g->N > 0 && (!g->dy || (g->activation != CDG_ACT_NONE && !g->z))) return CDG_ERR_INVALID_ARGUMENT;
+  if (g->dx && g->N > 0 && g->K > 0 && g->M > 0 && !g->w) return CDG_ERR_INVALID_ARGUMENT;
+  if (g->dw && g->M > 0 && g->K > 0 && g->N > 0 && !g->x) return CDG_ERR_INVALID_ARGUMENT;
+  return sizes_ok(g->M, g->N, g->K) ? CDG_OK : CDG_ERR_UNSUPPORTED;
+}
+
+}  // namespace
+
+// This unit's record of waits that gave up (cdg_device_status reads it with the others').
+int linear_sticky_status(int clear, int32_t* out) {
+  if (cudaMemcpyFromSymbol(out, g_sticky_status, 2 * sizeof(int32_t)) != cudaSuccess) return CDG_ERR_CUDA;
+  if (clear && (out[0] || out[1])) {
+    const int32_t z[2] = {0, 0};
+    if (cudaMemcpyToSymbol(g_sticky_status, z, sizeof(z)) != cudaSuccess) return CDG_ERR_CUDA;
+  }
+  return CDG_OK;
+}
+
+}  // namespace cdg
+
+extern "C" {
+
+size_t cdg_linear_workspace_bytes(const cdg_linear_args* g) {
+  using namespace cdg;
+  if (check_forward(g) != CDG_OK) return 0;
+  return repack_bytes(Matrix{g->x, g->x_stride, g->M, g->K}) + repack_bytes(Matrix{g->w, g->w_stride, g->N, g->K});
+}
+
+int cdg_linear(const cdg_linear_args* g, void* workspace, size_t workspace_bytes, cdg_stream_t stream) {
+  using namespace cdg;
+  int rc = check_forward(g);
+  if (rc != CDG_OK) return rc;
+  if (g->M == 0 || g->N == 0) return CDG_OK;
+  const size_t need = cdg_linear_workspace_bytes(g);
+  if (need && (!workspace || workspace_bytes < need)) return CDG_ERR_WORKSPACE;
+  if (need && reinterpret_cast<uintptr_t>(workspace) % 16) return CDG_ERR_ALIGNMENT;
+  rc = device_ready();
+  if (rc != CDG_OK) return rc;
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  return g->dtype == CDG_DTYPE_BF16 ? forward<__nv_bfloat16>(g, ws, st) : forward<__half>(g, ws, st);
+}
+
+size_t cdg_linear_backward_workspace_bytes(const cdg_linear_backward_args* g) {
+  using namespace cdg;
+  if (check_backward(g) != CDG_OK) return 0;
+  size_t n = 0;
+  if (g->M > 0 && needs_dz(g) && (g->dx || g->dw)) n += align256(static_cast<size_t>(g->M) * padded(g->N) * 2);
+  if (g->M > 0 && g->db) n += align256(static_cast<size_t>(dz_groups(g->M, g->N)) * g->N * 4);
+  if (g->dx) n += repack_bytes(Matrix{g->w, g->w_stride, g->N, g->K});
+  if (g->dw) n += repack_bytes(Matrix{g->x, g->x_stride, g->M, g->K});
+  return n;
+}
+
+int cdg_linear_backward(const cdg_linear_backward_args* g, void* workspace, size_t workspace_bytes,
+                        cdg_stream_t stream) {
+  using namespace cdg;
+  int rc = check_backward(g);
+  if (rc != CDG_OK) return rc;
+  const size_t need = cdg_linear_backward_workspace_bytes(g);
+  if (need && (!workspace || workspace_bytes < need)) return CDG_ERR_WORKSPACE;
+  if (need && reinterpret_cast<uintptr_t>(workspace) % 16) return CDG_ERR_ALIGNMENT;
+  rc = device_ready();
+  if (rc != CDG_OK) return rc;
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  return g->dtype == CDG_DTYPE_BF16 ? backward<__nv_bfloat16>(g, ws, st) : backward<__half>(g, ws, st);
+}
+
+}  // extern "C"

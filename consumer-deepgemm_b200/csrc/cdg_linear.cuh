@@ -1,0 +1,425 @@
+// Dense product on the tensor cores with a fused epilogue: D = epilogue(A . B^T), A [M, K] and
+// B [N, K] BF16 or FP16, FP32 accumulation.
+//
+//   z = sum_k A[m, k] B[n, k] + bias[n];   y = act(z) + residual[m, n]
+//
+// Each operand lies in memory either K-major (rows of K) or MN-major (K rows of M or N), so that
+// one kernel serves x . W^T, dz . W and dz^T . x.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "cdg_ptx.cuh"
+#include "cdg_rows.cuh"
+
+namespace cdg {
+namespace {
+
+// ---------------------------------------------------------------- instructions
+// D[tmem] (+)= A[smem] . B[smem], 16-bit operands, by the lane elect.sync picks of a whole warp.
+__device__ __forceinline__ void tc_mma_f16_warp(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
+                                                uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p, e;\n\t"
+      "elect.sync _|e, 0xffffffff;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+      ::"r"(d_tmem), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
+__device__ __forceinline__ void tc_commit_warp(uint64_t* bar) {
+  asm volatile(
+      "{\n\t.reg .pred e;\n\t"
+      "elect.sync _|e, 0xffffffff;\n\t"
+      "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}"
+      ::"r"(smem_u32(bar))
+      : "memory");
+}
+
+// Load 32 consecutive 32-bit TMEM columns of this warp's 32 lanes.
+__device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
+        "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
+        "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr));
+}
+
+// Operand tiles of one K step (64 columns of K) in shared memory, 128-byte swizzle:
+//   K-major:  [rows][64 k], 8-row groups 1024 bytes apart;
+//   MN-major: chunks of 64 rows, each [64 k][64 rows] (8192 bytes); the 8-k groups of a chunk
+//             are 1024 bytes apart, the chunks 8192.
+// One MMA takes 16 of K: 32 bytes further on in the swizzled rows, or two 8-k groups.
+__device__ __forceinline__ uint64_t operand_desc(uint32_t addr, bool mn_major) {
+  uint64_t d = smem_desc_sw128(addr);
+  if (mn_major) d |= static_cast<uint64_t>((8192u >> 4) & 0x3FFFu) << 16;  // leading byte offset: chunk to chunk
+  return d;
+}
+
+__device__ __forceinline__ uint32_t operand_k_step(bool mn_major) { return mn_major ? 2048u >> 4 : 32u >> 4; }
+
+// Instruction descriptor of tcgen05.mma kind::f16 with FP32 accumulation.
+__host__ __device__ __forceinline__ uint32_t idesc_f16(bool bf16, bool a_mn, bool b_mn, uint32_t m, uint32_t n) {
+  uint32_t d = 1u << 4;  // D is FP32
+  d |= (bf16 ? 1u : 0u) << 7;
+  d |= (bf16 ? 1u : 0u) << 10;
+  d |= (a_mn ? 1u : 0u) << 15;
+  d |= (b_mn ? 1u : 0u) << 16;
+  d |= ((n >> 3) & 0x3Fu) << 17;
+  d |= ((m >> 4) & 0x1Fu) << 24;
+  return d;
+}
+
+// ---------------------------------------------------------------- epilogue arithmetic
+// Activations in FP32.  The exponentials are the fast ones: their error (a few units in the last
+// place) is far below the 16-bit outputs' rounding and stays within 1e-6 for 32-bit outputs.
+__device__ __forceinline__ float fast_sigmoid(float v) { return __fdividef(1.0f, 1.0f + __expf(-v)); }
+
+__device__ __forceinline__ float activate(float z, int act) {
+  switch (act) {
+    case CDG_ACT_RELU: return z > 0.0f || z != z ? z : 0.0f;
+    case CDG_ACT_SILU: return __fdividef(z, 1.0f + __expf(-z));
+    case CDG_ACT_GELU: return 0.5f * z * (1.0f + erff(z * 0.70710678118654752f));
+    case CDG_ACT_GELU_TANH: {
+      // 0.5 (1 + tanh u) = sigmoid(2u), u = sqrt(2 / pi) (z + 0.044715 z^3)
+      const float u2 = 1.5957691216057308f * (z + 0.044715f * z * z * z);
+      return __fdividef(z, 1.0f + __expf(-u2));
+    }
+    default: return z;
+  }
+}
+
+// d act(z) / dz
+__device__ __forceinline__ float activate_slope(float z, int act) {
+  switch (act) {
+    case CDG_ACT_RELU: return z > 0.0f ? 1.0f : 0.0f;
+    case CDG_ACT_SILU: {
+      const float s = fast_sigmoid(z);
+      return s * (1.0f + z * (1.0f - s));
+    }
+    case CDG_ACT_GELU:
+      return 0.5f * (1.0f + erff(z * 0.70710678118654752f)) + z * __expf(-0.5f * z * z) * 0.39894228040143268f;
+    case CDG_ACT_GELU_TANH: {
+      // with s = sigmoid(2u): z s' + s, s' = s (1 - s) d(2u)/dz
+      const float s = fast_sigmoid(1.5957691216057308f * (z + 0.044715f * z * z * z));
+      return s + z * s * (1.0f - s) * 1.5957691216057308f * (1.0f + 0.134145f * z * z);
+    }
+    default: return 1.0f;
+  }
+}
+
+struct Epilogue {
+  const void* bias;
+  const void* residual;
+  void* y;
+  void* z;  // the value before the activation, in the operands' type; NULL = not stored
+  int64_t residual_stride, y_stride, z_stride;
+  int bias_f32, residual_f32, act;
+  int wide;  // y, z and residual rows on 16-byte boundaries
+};
+
+template <typename T>
+__device__ __forceinline__ float load_any(const void* p, int64_t i, int f32) {
+  return f32 ? static_cast<const float*>(p)[i] : to_f(static_cast<const T*>(p)[i]);
+}
+
+// Eight consecutive columns [n, n + 8) of row m, clipped at N.
+template <typename T, typename O>
+__device__ __forceinline__ void finish8(const Epilogue& e, int64_t m, int64_t n, int64_t N, float (&v)[8]) {
+  const bool full = e.wide && n + 8 <= N;
+  if (e.bias) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (n + j < N) v[j] += load_any<T>(e.bias, n + j, e.bias_f32);
+  }
+  if (e.z) {
+    T* z = static_cast<T*>(e.z) + m * e.z_stride + n;
+    if (full) {
+      *reinterpret_cast<uint4*>(z) = make_uint4(pack2(v[0], v[1], T()), pack2(v[2], v[3], T()),
+                                                pack2(v[4], v[5], T()), pack2(v[6], v[7], T()));
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (n + j < N) z[j] = from_f<T>(v[j]);
+    }
+  }
+  if (e.act != CDG_ACT_NONE) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = activate(v[j], e.act);
+  }
+  if (e.residual) {
+    if (full && !e.residual_f32) {
+      const uint4 r = __ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(e.residual) + m * e.residual_stride + n));
+      const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float2 f = unpack2(w[j], T());
+        v[2 * j] += f.x;
+        v[2 * j + 1] += f.y;
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (n + j < N) v[j] += load_any<T>(e.residual, m * e.residual_stride + n + j, e.residual_f32);
+    }
+  }
+  O* y = static_cast<O*>(e.y) + m * e.y_stride + n;
+  if (full) {
+    if constexpr (sizeof(O) == 4) {
+      reinterpret_cast<float4*>(y)[0] = make_float4(v[0], v[1], v[2], v[3]);
+      reinterpret_cast<float4*>(y)[1] = make_float4(v[4], v[5], v[6], v[7]);
+    } else {
+      *reinterpret_cast<uint4*>(y) = make_uint4(pack2(v[0], v[1], O()), pack2(v[2], v[3], O()),
+                                                pack2(v[4], v[5], O()), pack2(v[6], v[7], O()));
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (n + j < N) y[j] = from_f<O>(v[j]);
+  }
+}
+
+struct LinearShape {
+  int64_t M, N;
+  int k_steps;         // of 64 columns of K
+  int m_tiles, n_tiles;
+  int a_rows;          // rows of A's box: 128, or M rounded up to 8 where M is smaller (K-major)
+  int a_mn, b_mn, bf16;
+};
+
+// ---------------------------------------------------------------- one tile per CTA, K split over a cluster
+// Tile 128 x BN.  gridDim.x = tiles * splits; the CTAs of a cluster share a tile and take
+// consecutive parts of K, then each sums a share of the tile's columns over all of them through
+// distributed shared memory, in rank order (deterministic).  Two CTAs fit an SM, so that one's
+// epilogue overlaps another's products.
+// PROMOTE (32-bit outputs): the tensor core's running sum loses about one part in 2^20 over a
+// few thousand terms (its additions truncate), which 16-bit outputs do not see; here a sum
+// covers 512 of K at most, and FP32 registers add those up.
+// Warps: 0-3 epilogue (one per TMEM lane quadrant), 4 TMA producer, 5 MMA issuer and TMEM owner.
+template <int BN, bool PROMOTE>
+struct TileSmem {
+  static constexpr int kA = 128 * 128;
+  static constexpr int kB = BN * 128;
+  static constexpr int kStageBytes = kA + kB;
+  static constexpr int kStages = BN >= 128 ? 3 : 4;
+  static constexpr int kBars = kStages * kStageBytes;  // full, empty [kStages]; tfull, tempty [2]; TMEM address
+  static constexpr int kBytes = kBars + (2 * kStages + 4) * 8 + 16 + 1024;
+  static constexpr int kAccs = PROMOTE ? 2 : 1;
+  static constexpr int kTmemCols = kAccs * BN < 32 ? 32 : kAccs * BN;
+  static_assert(128 * BN * 4 <= kStages * kStageBytes, "the split's partial sums reuse the stages");
+  static_assert(2 * kBytes <= 228 * 1024, "two CTAs per SM");
+};
+
+constexpr int kTileThreads = 192;
+constexpr int kPromoteSteps = 8;  // K steps of 64 per running sum
+
+template <typename T, typename O, int BN, bool PROMOTE>
+__global__ void __launch_bounds__(kTileThreads)
+    cdg_linear_tile_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_b,
+                           const LinearShape s, const Epilogue e, const int splits) {
+  using L = TileSmem<BN, PROMOTE>;
+  constexpr int S = L::kStages;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + L::kBars);
+  uint64_t* empty = full + S;
+  uint64_t* tfull = empty + S;
+  uint64_t* tempty = tfull + 2;
+  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(tempty + 2);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int tile = static_cast<int>(blockIdx.x) / splits, split = static_cast<int>(blockIdx.x) % splits;
+  const int m0 = (tile % s.m_tiles) * 128, n0 = (tile / s.m_tiles) * BN;
+  const int k_first = static_cast<int>(static_cast<int64_t>(s.k_steps) * split / splits);
+  const int k_last = static_cast<int>(static_cast<int64_t>(s.k_steps) * (split + 1) / splits);
+  const int sums = PROMOTE ? (k_last - k_first + kPromoteSteps - 1) / kPromoteSteps : (k_last > k_first ? 1 : 0);
+
+  if (warp == 4 && lane == 0) {
+    prefetch_tmap(&tmap_a);
+    prefetch_tmap(&tmap_b);
+    for (int i = 0; i < S; ++i) {
+      mbar_init(&full[i], 1);
+      mbar_init(&empty[i], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&tfull[i], 1);
+      mbar_init(&tempty[i], 128);
+    }
+    fence_mbarrier_init();
+  }
+  if (warp == 5) {
+    tmem_alloc(tmem_holder, L::kTmemCols);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_holder;
+  bool ok = true;
+  float acc[PROMOTE ? BN : 1];
+
+  if (warp == 4) {
+    if (lane == 0) {
+      int stage = 0;
+      uint32_t phase = 0;
+      // boxes past M (MN-major, in chunks of 64) are not loaded: their rows of the result are not stored
+      const int a_chunks = s.a_mn ? (s.M - m0 > 64 ? 2 : 1) : 0;
+      const uint32_t bytes = (s.a_mn ? a_chunks * 8192u : static_cast<uint32_t>(s.a_rows) * 128u) + L::kB;
+      for (int k = k_first; k < k_last; ++k) {
+        if (!mbar_wait_cta(&empty[stage], phase ^ 1, nullptr, wait_code(1, 0, stage, phase ^ 1, k))) {
+          ok = false;
+          break;
+        }
+        mbar_arrive_expect_tx(&full[stage], bytes);
+        uint8_t* a = smem + stage * L::kStageBytes;
+        uint8_t* b = a + L::kA;
+        if (s.a_mn) {
+          for (int c = 0; c < a_chunks; ++c) tma_load_2d(a + c * 8192, &tmap_a, &full[stage], m0 + c * 64, k * 64);
+        } else {
+          tma_load_2d(a, &tmap_a, &full[stage], k * 64, m0);
+        }
+        if (s.b_mn) {
+#pragma unroll
+          for (int c = 0; c < BN / 64; ++c) tma_load_2d(b + c * 8192, &tmap_b, &full[stage], n0 + c * 64, k * 64);
+        } else {
+          tma_load_2d(b, &tmap_b, &full[stage], k * 64, n0);
+        }
+        if (++stage == S) { stage = 0; phase ^= 1; }
+      }
+    }
+    __syncwarp();
+  } else if (warp == 5) {
+    const uint32_t idesc = idesc_f16(s.bf16, s.a_mn, s.b_mn, 128, BN);
+    const uint32_t a_step = operand_k_step(s.a_mn), b_step = operand_k_step(s.b_mn);
+    int stage = 0;
+    uint32_t phase = 0;
+    for (int i = 0, k = k_first; i < sums && ok; ++i) {
+      const int buf = PROMOTE ? i & 1 : 0;
+      if (PROMOTE && !mbar_wait_cta_warp(&tempty[buf], ((i >> 1) & 1) ^ 1, nullptr, wait_code(2, 0, buf, i, k))) {
+        ok = false;
+        break;
+      }
+      tc_fence_after();
+      const int end = PROMOTE ? min(k_last, k + kPromoteSteps) : k_last;
+      for (bool first = true; k < end; ++k) {
+        if (!mbar_wait_cta_warp(&full[stage], phase, nullptr, wait_code(3, 0, stage, phase, k))) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        const uint32_t base = smem_u32(smem + stage * L::kStageBytes);
+        const uint64_t ad = operand_desc(base, s.a_mn), bd = operand_desc(base + L::kA, s.b_mn);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          tc_mma_f16_warp(tmem + buf * BN, ad + j * a_step, bd + j * b_step, idesc, first ? 0u : 1u);
+          first = false;
+        }
+        tc_commit_warp(&empty[stage]);
+        if (++stage == S) { stage = 0; phase ^= 1; }
+      }
+      if (ok) tc_commit_warp(&tfull[buf]);
+    }
+  } else {
+    const uint32_t lanes = tmem + (static_cast<uint32_t>(warp * 32) << 16);
+    const int64_t m = m0 + warp * 32 + lane;
+    float* part = reinterpret_cast<float*>(smem);  // [BN][128] partial sums of this split
+    if constexpr (PROMOTE) {
+#pragma unroll
+      for (int j = 0; j < BN; ++j) acc[j] = 0.0f;
+      for (int i = 0; i < sums && ok; ++i) {
+        const int buf = i & 1;
+        if (!mbar_wait_cta_warp(&tfull[buf], (i >> 1) & 1, nullptr, wait_code(4, 0, buf, i >> 1, i))) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+#pragma unroll
+        for (int c = 0; c < BN / 32; ++c) {
+          uint32_t r[32];
+          tmem_ld32(lanes + buf * BN + c * 32, r);
+          tmem_ld_wait();
+#pragma unroll
+          for (int j = 0; j < 32; ++j) acc[c * 32 + j] += __uint_as_float(r[j]);
+        }
+        tc_fence_before();
+        mbar_arrive(&tempty[buf]);
+      }
+    } else {
+      if (sums && !mbar_wait_cta_warp(&tfull[0], 0, nullptr, wait_code(4, 0, 0, 0, 0))) ok = false;
+      tc_fence_after();
+    }
+    if (ok) {
+#pragma unroll
+      for (int c = 0; c < BN / 32; ++c) {
+        float v[32];
+        if constexpr (PROMOTE) {
+#pragma unroll
+          for (int j = 0; j < 32; ++j) v[j] = acc[c * 32 + j];
+        } else {
+          uint32_t r[32];
+          tmem_ld32(lanes + c * 32, r);
+          tmem_ld_wait();
+#pragma unroll
+          for (int j = 0; j < 32; ++j) v[j] = sums ? __uint_as_float(r[j]) : 0.0f;  // K = 0: nothing was summed
+        }
+        if (splits > 1) {
+          // every product of this CTA has completed, so the stages are free
+#pragma unroll
+          for (int j = 0; j < 32; ++j) part[(c * 32 + j) * 128 + warp * 32 + lane] = v[j];
+        } else if (m < s.M) {
+#pragma unroll
+          for (int g = 0; g < 4; ++g) {
+            float w[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) w[j] = v[g * 8 + j];
+            const int64_t n = n0 + c * 32 + g * 8;
+            if (n < s.N) finish8<T, O>(e, m, n, s.N, w);
+          }
+        }
+      }
+    }
+  }
+
+  if (splits > 1) {
+    // every CTA of the cluster takes part, also one whose wait gave up (its sums are then wrong,
+    // and the device record says so)
+    cluster_sync();
+    const float* part = reinterpret_cast<const float*>(smem);
+    for (int item = threadIdx.x; item < 128 * (BN / 8); item += kTileThreads) {
+      const int group = item / 128, row = item % 128;
+      if (group % splits != split) continue;
+      const int64_t m = m0 + row, n = n0 + group * 8;
+      if (m >= s.M || n >= s.N) continue;
+      float v[8] = {};
+      for (int r = 0; r < splits; ++r) {
+        const uint32_t at = cluster_addr(part + group * 8 * 128 + row, r);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          float f;
+          asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(f) : "r"(at + j * 512));
+          v[j] += f;
+        }
+      }
+      finish8<T, O>(e, m, n, s.N, v);
+    }
+    cluster_sync();  // no CTA leaves while another reads its shared memory
+  }
+  tc_fence_before();
+  if (__syncthreads_or(!ok)) {
+    // after a wait that gave up, copies issued before it still land: give them time before exit
+    const uint64_t t0 = global_timer_ns();
+    while (global_timer_ns() - t0 < 200000ull) __nanosleep(20000);
+  }
+  if (warp == 5) {
+    tc_fence_after();
+    tmem_dealloc(tmem, L::kTmemCols);
+  }
+}
+
+}  // namespace
+}  // namespace cdg

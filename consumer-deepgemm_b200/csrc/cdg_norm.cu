@@ -20,124 +20,10 @@
 #include <cstdint>
 
 #include "cdg_b200.h"
+#include "cdg_rows.cuh"
 
 namespace cdg {
 namespace {
-
-template <typename T>
-__device__ __forceinline__ float to_f(T v);
-template <>
-__device__ __forceinline__ float to_f(float v) { return v; }
-template <>
-__device__ __forceinline__ float to_f(__nv_bfloat16 v) { return __bfloat162float(v); }
-template <>
-__device__ __forceinline__ float to_f(__half v) { return __half2float(v); }
-
-template <typename T>
-__device__ __forceinline__ T from_f(float v);
-template <>
-__device__ __forceinline__ float from_f(float v) { return v; }
-template <>
-__device__ __forceinline__ __nv_bfloat16 from_f(float v) { return __float2bfloat16_rn(v); }
-template <>
-__device__ __forceinline__ __half from_f(float v) { return __float2half_rn(v); }
-
-__device__ __forceinline__ float2 unpack2(uint32_t v, __nv_bfloat16) {
-  return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&v));
-}
-__device__ __forceinline__ float2 unpack2(uint32_t v, __half) {
-  return __half22float2(*reinterpret_cast<const __half2*>(&v));
-}
-__device__ __forceinline__ uint32_t pack2(float a, float b, __nv_bfloat16) {
-  const __nv_bfloat162 p = __floats2bfloat162_rn(a, b);
-  return *reinterpret_cast<const uint32_t*>(&p);
-}
-__device__ __forceinline__ uint32_t pack2(float a, float b, __half) {
-  const __half2 p = __floats2half2_rn(a, b);
-  return *reinterpret_cast<const uint32_t*>(&p);
-}
-
-// A warp takes 256 columns at a time, eight per lane.  Wide (rows on 16-byte boundaries, H a
-// multiple of 8): lane l holds columns 8l .. 8l+7, one 128-column scale block per half warp.
-// Narrow (anything else): lane l holds columns l, l + 32, ..., so that each load of the warp
-// stays contiguous; the first four are in the first scale block, the others in the second.
-template <bool WIDE>
-__device__ __forceinline__ int64_t column(int64_t chunk, int lane, int j) {
-  return chunk * 256 + (WIDE ? lane * 8 + j : j * 32 + lane);
-}
-
-// The lane's eight elements of a chunk as they lie in memory.
-template <typename T>
-struct Raw {
-  static constexpr int kWords = static_cast<int>(sizeof(T)) * 2;
-  uint32_t w[kWords];
-};
-
-template <typename T>
-__device__ __forceinline__ void unpack8(const Raw<T>& raw, float (&v)[8]) {
-  if constexpr (sizeof(T) == 4) {
-#pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = __uint_as_float(raw.w[j]);
-  } else {
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const float2 f = unpack2(raw.w[j], T());
-      v[2 * j] = f.x;
-      v[2 * j + 1] = f.y;
-    }
-  }
-}
-
-template <typename T, bool WIDE>
-__device__ __forceinline__ Raw<T> load8(const T* row, int64_t chunk, int lane, int64_t H) {
-  Raw<T> raw;
-#pragma unroll
-  for (int j = 0; j < Raw<T>::kWords; ++j) raw.w[j] = 0;
-  if constexpr (WIDE) {
-    const int64_t c = column<true>(chunk, lane, 0);
-    if (c < H) {
-      const uint4* p = reinterpret_cast<const uint4*>(row + c);
-#pragma unroll
-      for (int k = 0; k < Raw<T>::kWords / 4; ++k) {
-        const uint4 t = p[k];
-        raw.w[4 * k] = t.x; raw.w[4 * k + 1] = t.y; raw.w[4 * k + 2] = t.z; raw.w[4 * k + 3] = t.w;
-      }
-    }
-  } else {
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const int64_t c = column<false>(chunk, lane, j);
-      if (c < H) {
-        if constexpr (sizeof(T) == 4)
-          raw.w[j] = reinterpret_cast<const uint32_t*>(row)[c];
-        else
-          raw.w[j / 2] |= static_cast<uint32_t>(reinterpret_cast<const uint16_t*>(row)[c]) << (16 * (j & 1));
-      }
-    }
-  }
-  return raw;
-}
-
-template <typename T, bool WIDE>
-__device__ __forceinline__ void store8(T* row, int64_t chunk, int lane, int64_t H, const float (&v)[8]) {
-  if constexpr (WIDE) {
-    const int64_t c = column<true>(chunk, lane, 0);
-    if (c >= H) return;
-    uint4* p = reinterpret_cast<uint4*>(row + c);
-    if constexpr (sizeof(T) == 4) {
-      p[0] = make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
-      p[1] = make_uint4(__float_as_uint(v[4]), __float_as_uint(v[5]), __float_as_uint(v[6]), __float_as_uint(v[7]));
-    } else {
-      p[0] = make_uint4(pack2(v[0], v[1], T()), pack2(v[2], v[3], T()), pack2(v[4], v[5], T()), pack2(v[6], v[7], T()));
-    }
-  } else {
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const int64_t c = column<false>(chunk, lane, j);
-      if (c < H) row[c] = from_f<T>(v[j]);
-    }
-  }
-}
 
 // The norm's weights: of the rows' type or FP32.
 template <typename T, bool WIDE>
@@ -401,48 +287,12 @@ __global__ void __launch_bounds__(THREADS) rms_norm_backward_kernel(const NormBw
   }
 }
 
-// dw[c] = the sum of the CTAs' partial sums, in CTA order per thread and then over the eight
-// threads of a column: the same order every time.
-template <typename W>
-__global__ void __launch_bounds__(256) rms_norm_dw_kernel(const float* partial, int parts, int64_t H, W* dw) {
-  __shared__ float sums[8][33];
-  const int lane = threadIdx.x & 31, g = threadIdx.x >> 5;
-  const int64_t c = static_cast<int64_t>(blockIdx.x) * 32 + lane;
-  float v = 0.0f;
-  if (c < H)
-    for (int p = g; p < parts; p += 8) v += partial[static_cast<int64_t>(p) * H + c];
-  sums[g][lane] = v;
-  __syncthreads();
-  if (g == 0 && c < H) {
-#pragma unroll
-    for (int i = 1; i < 8; ++i) v += sums[i][lane];
-    dw[c] = from_f<W>(v);
-  }
-}
-
-int launched() { return cudaGetLastError() == cudaSuccess ? CDG_OK : CDG_ERR_CUDA; }
-
-int sm_count() {
-  int dev = 0, n = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
-    return 148;
-  return n > 0 ? n : 148;
-}
 }  // namespace
 
 // Row widths up to this one fit the registers of one CTA (32 warps of four 256-column chunks).
 constexpr int64_t kNormMaxH = 32768;
 
 namespace {
-
-int element_size(int dtype) { return dtype == CDG_DTYPE_F32 ? 4 : 2; }
-
-bool row_dtype(int dtype) { return dtype == CDG_DTYPE_BF16 || dtype == CDG_DTYPE_F16 || dtype == CDG_DTYPE_F32; }
-
-// Whether every row of a tensor starts on a 16-byte boundary (absent tensors do).
-bool wide_rows(const void* p, int64_t stride, int64_t bytes) {
-  return !p || (reinterpret_cast<uintptr_t>(p) % 16 == 0 && stride * bytes % 16 == 0);
-}
 
 template <typename T, bool WIDE>
 int launch_norm(const NormFwd& a, cudaStream_t st) {
@@ -547,11 +397,11 @@ int cdg_rms_norm_backward(const cdg_norm_backward_args* g, void* workspace, size
   if (rc != CDG_OK) return rc;
   const unsigned grid = static_cast<unsigned>((g->H + 31) / 32);
   if (g->w_dtype == CDG_DTYPE_BF16)
-    rms_norm_dw_kernel<__nv_bfloat16><<<grid, 256, 0, st>>>(a.partial, s.grid, g->H, static_cast<__nv_bfloat16*>(g->dw));
+    column_sum_kernel<__nv_bfloat16><<<grid, 256, 0, st>>>(a.partial, s.grid, g->H, static_cast<__nv_bfloat16*>(g->dw));
   else if (g->w_dtype == CDG_DTYPE_F16)
-    rms_norm_dw_kernel<__half><<<grid, 256, 0, st>>>(a.partial, s.grid, g->H, static_cast<__half*>(g->dw));
+    column_sum_kernel<__half><<<grid, 256, 0, st>>>(a.partial, s.grid, g->H, static_cast<__half*>(g->dw));
   else
-    rms_norm_dw_kernel<float><<<grid, 256, 0, st>>>(a.partial, s.grid, g->H, static_cast<float*>(g->dw));
+    column_sum_kernel<float><<<grid, 256, 0, st>>>(a.partial, s.grid, g->H, static_cast<float*>(g->dw));
   return launched();
 }
 

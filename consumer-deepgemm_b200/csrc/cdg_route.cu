@@ -24,6 +24,7 @@
 #include <cstdint>
 
 #include "cdg_b200.h"
+#include "cdg_rows.cuh"
 
 namespace cdg {
 namespace {
@@ -31,15 +32,6 @@ namespace {
 constexpr int kRouteMaxExperts = 1024;
 constexpr int kRouteMaxTopk = 32;  // lane j keeps the row's j-th choice
 constexpr unsigned kAll = 0xffffffffu;
-
-template <typename T>
-__device__ __forceinline__ float load_logit(const T* p);
-template <>
-__device__ __forceinline__ float load_logit(const float* p) { return __ldg(p); }
-template <>
-__device__ __forceinline__ float load_logit(const __nv_bfloat16* p) { return __bfloat162float(*p); }
-template <>
-__device__ __forceinline__ float load_logit(const __half* p) { return __half2float(*p); }
 
 // NaN counts as -inf (never chosen), +inf as the largest finite value, -0 as 0.
 __device__ __forceinline__ float clean_logit(float v) {
@@ -127,7 +119,7 @@ __global__ void __launch_bounds__(WARPS * 32) moe_route_kernel(const Route a) {
   auto load_row = [&](int64_t row) {
 #pragma unroll
     for (int i = 0; i < N; ++i)
-      next[i] = i * 32 + lane < a.E ? load_logit<T>(logits + row * a.stride + i * 32 + lane) : -INFINITY;
+      next[i] = i * 32 + lane < a.E ? to_f(logits[row * a.stride + i * 32 + lane]) : -INFINITY;
   };
   int64_t row = static_cast<int64_t>(blockIdx.x) * WARPS + warp;
   if (row < a.T) load_row(row);
@@ -198,7 +190,7 @@ __global__ void __launch_bounds__(WARPS * 32) moe_route_kernel(const Route a) {
         if (lane == j) id = winner;
       }
       if (id >= 0) {
-        const float l = clean_logit(load_logit<T>(logits + row * a.stride + id));
+        const float l = clean_logit(to_f(logits[row * a.stride + id]));
         w = a.sigmoid ? sigmoid_fast(l) : __expf(l - m) * inv;
         atomicAdd(&s_counts[id], 1);
       }
@@ -261,15 +253,6 @@ struct RouteBwd {
   int64_t d_stride;
 };
 
-template <typename T>
-__device__ __forceinline__ T grad_cast(float v);
-template <>
-__device__ __forceinline__ float grad_cast(float v) { return v; }
-template <>
-__device__ __forceinline__ __nv_bfloat16 grad_cast(float v) { return __float2bfloat16_rn(v); }
-template <>
-__device__ __forceinline__ __half grad_cast(float v) { return __float2half_rn(v); }
-
 // Dynamic shared memory: one row of E floats per warp, the scattered gradient of the chosen
 // scores (zero between rows).
 template <typename T, int N, int WARPS>
@@ -297,7 +280,7 @@ __global__ void __launch_bounds__(WARPS * 32) moe_route_backward_kernel(const Ro
   auto load_row = [&](int64_t row) {
 #pragma unroll
     for (int i = 0; i < N; ++i)
-      next[i] = i * 32 + lane < a.E ? load_logit<T>(logits + row * a.stride + i * 32 + lane) : -INFINITY;
+      next[i] = i * 32 + lane < a.E ? to_f(logits[row * a.stride + i * 32 + lane]) : -INFINITY;
     if (lane < a.k) {
       next_id = __ldg(a.ids + row * a.k + lane);
       if (a.gw) next_g = __ldg(a.gw + row * a.k + lane);
@@ -320,7 +303,7 @@ __global__ void __launch_bounds__(WARPS * 32) moe_route_backward_kernel(const Ro
     if (!__any_sync(kAll, id >= 0)) {  // masked token: no gradient
 #pragma unroll
       for (int i = 0; i < N; ++i)
-        if (i * 32 + lane < a.E) out[i * 32 + lane] = grad_cast<T>(0.0f);
+        if (i * 32 + lane < a.E) out[i * 32 + lane] = from_f<T>(0.0f);
       continue;
     }
     m = a.sigmoid ? 0.0f : key_value(__reduce_max_sync(kAll, order_key(m)));
@@ -340,7 +323,7 @@ __global__ void __launch_bounds__(WARPS * 32) moe_route_backward_kernel(const Ro
       if (a.renormalize) {
         float c = 0.0f;
         if (id >= 0) {
-          const float l = clean_logit(load_logit<T>(logits + row * a.stride + id));
+          const float l = clean_logit(to_f(logits[row * a.stride + id]));
           c = a.sigmoid ? sigmoid_fast(l) : __expf(l - m) * inv;
         }
         float chosen = warp_sum(c);
@@ -370,19 +353,12 @@ __global__ void __launch_bounds__(WARPS * 32) moe_route_backward_kernel(const Ro
         v = (d[i] + (load[i] - dot * inv) * inv) * s[i] * (1.0f - s[i]);
       else
         v = s[i] * (d[i] + load[i] - dot);
-      if (i * 32 + lane < a.E) out[i * 32 + lane] = grad_cast<T>(v);
+      if (i * 32 + lane < a.E) out[i * 32 + lane] = from_f<T>(v);
     }
   }
 }
 
 constexpr int kRouteWarps = 8;
-
-int route_sms() {
-  int dev = 0, n = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
-    return 148;
-  return n > 0 ? n : 148;
-}
 
 // CTAs per SM by registers: N experts per lane take about 4N registers of a thread.
 int route_ctas_per_sm(int n) { return n <= 8 ? 6 : n <= 16 ? 4 : 2; }
@@ -390,18 +366,18 @@ int route_ctas_per_sm(int n) { return n <= 8 ? 6 : n <= 16 ? 4 : 2; }
 template <typename T, int N>
 int launch_route(const Route& a, cudaStream_t st) {
   const int64_t ctas = (a.T + kRouteWarps - 1) / kRouteWarps;
-  const unsigned grid = static_cast<unsigned>(std::min<int64_t>(ctas, int64_t(route_sms()) * route_ctas_per_sm(N)));
+  const unsigned grid = static_cast<unsigned>(std::min<int64_t>(ctas, int64_t(sm_count()) * route_ctas_per_sm(N)));
   const size_t smem = a.E * 4 + (a.balance ? size_t(kRouteWarps) * a.E * 4 : 0);
   moe_route_kernel<T, N, kRouteWarps><<<grid, kRouteWarps * 32, smem, st>>>(a);
-  return cudaGetLastError() == cudaSuccess ? CDG_OK : CDG_ERR_CUDA;
+  return launched();
 }
 
 template <typename T, int N>
 int launch_route_backward(const RouteBwd& a, cudaStream_t st) {
   const int64_t ctas = (a.T + kRouteWarps - 1) / kRouteWarps;
-  const unsigned grid = static_cast<unsigned>(std::min<int64_t>(ctas, int64_t(route_sms()) * route_ctas_per_sm(N)));
+  const unsigned grid = static_cast<unsigned>(std::min<int64_t>(ctas, int64_t(sm_count()) * route_ctas_per_sm(N)));
   moe_route_backward_kernel<T, N, kRouteWarps><<<grid, kRouteWarps * 32, size_t(kRouteWarps) * a.E * 4, st>>>(a);
-  return cudaGetLastError() == cudaSuccess ? CDG_OK : CDG_ERR_CUDA;
+  return launched();
 }
 
 template <typename T>
@@ -426,8 +402,6 @@ int dispatch_route_backward(const RouteBwd& a, cudaStream_t st) {
   return launch_route_backward<T, 32>(a, st);
 }
 
-bool logit_dtype(int dtype) { return dtype == CDG_DTYPE_BF16 || dtype == CDG_DTYPE_F16 || dtype == CDG_DTYPE_F32; }
-
 }  // namespace
 }  // namespace cdg
 
@@ -440,7 +414,7 @@ size_t cdg_moe_route_workspace_bytes(int64_t E) {
 
 int cdg_moe_route(const cdg_route_args* g, void* workspace, size_t workspace_bytes, cdg_stream_t stream) {
   using namespace cdg;
-  if (!g || g->T < 0 || g->E <= 0 || g->topk <= 0 || g->topk > g->E || !logit_dtype(g->dtype))
+  if (!g || g->T < 0 || g->E <= 0 || g->topk <= 0 || g->topk > g->E || !row_dtype(g->dtype))
     return CDG_ERR_INVALID_ARGUMENT;
   if (g->scoring != CDG_SCORE_SOFTMAX && g->scoring != CDG_SCORE_SIGMOID) return CDG_ERR_INVALID_ARGUMENT;
   if (g->E > kRouteMaxExperts || g->topk > kRouteMaxTopk || g->T > kRouteMaxTokens) return CDG_ERR_UNSUPPORTED;
@@ -484,7 +458,7 @@ int cdg_moe_route(const cdg_route_args* g, void* workspace, size_t workspace_byt
 
 int cdg_moe_route_backward(const cdg_route_backward_args* g, cdg_stream_t stream) {
   using namespace cdg;
-  if (!g || g->T < 0 || g->E <= 0 || g->topk <= 0 || g->topk > g->E || !logit_dtype(g->dtype))
+  if (!g || g->T < 0 || g->E <= 0 || g->topk <= 0 || g->topk > g->E || !row_dtype(g->dtype))
     return CDG_ERR_INVALID_ARGUMENT;
   if (g->scoring != CDG_SCORE_SOFTMAX && g->scoring != CDG_SCORE_SIGMOID) return CDG_ERR_INVALID_ARGUMENT;
   if (g->E > kRouteMaxExperts || g->topk > kRouteMaxTopk || g->T > kRouteMaxTokens) return CDG_ERR_UNSUPPORTED;

@@ -836,6 +836,125 @@ torch::Tensor moe_route_backward(const torch::Tensor& logits, const torch::Tenso
   return out;
 }
 
+bool half_rows(const torch::Tensor& t) {
+  return t.scalar_type() == torch::kBFloat16 || t.scalar_type() == torch::kFloat16;
+}
+
+// (y, z or None)
+py::tuple linear(const torch::Tensor& x, const torch::Tensor& w, const c10::optional<torch::Tensor>& bias,
+                 const c10::optional<torch::Tensor>& residual, int64_t activation, bool out_f32, bool preact) {
+  const auto dev = x.device();
+  check_cuda(x, "x", dev);
+  check_cuda(w, "weight", dev);
+  TORCH_CHECK_VALUE(x.dim() == 2, "x must be [M, K], got ", x.sizes());
+  TORCH_CHECK_VALUE(half_rows(x), "x must be BF16 or FP16, got ", x.scalar_type());
+  TORCH_CHECK_VALUE(w.dim() == 2 && w.scalar_type() == x.scalar_type(), "weight must be [N, K] of x's dtype");
+  const int64_t M = x.size(0), K = x.size(1), N = w.size(0);
+  check_rows(x, "x", dev, M, K);
+  check_rows(w, "weight", dev, N, K);
+  cdg_linear_args g{};
+  if (bias.has_value()) {
+    check_vector(*bias, "bias", dev, N);
+    TORCH_CHECK_VALUE(bias->scalar_type() == x.scalar_type() || bias->scalar_type() == torch::kFloat32,
+                      "bias must have x's dtype or FP32");
+    g.bias = bias->data_ptr();
+    g.bias_dtype = dtype_code(*bias);
+  }
+  if (residual.has_value()) {
+    check_rows(*residual, "residual", dev, M, N);
+    TORCH_CHECK_VALUE(residual->scalar_type() == x.scalar_type() || residual->scalar_type() == torch::kFloat32,
+                      "residual must have x's dtype or FP32");
+    g.residual = residual->data_ptr();
+    g.residual_stride = residual->stride(0);
+    g.residual_dtype = dtype_code(*residual);
+  }
+  const c10::cuda::CUDAGuard guard(dev);
+  auto y = torch::empty({M, N}, out_f32 ? x.options().dtype(torch::kFloat32) : x.options());
+  torch::Tensor z;
+  if (preact) {
+    z = torch::empty({M, N}, x.options());
+    g.z_out = z.data_ptr();
+    g.z_stride = N;
+  }
+  g.x = x.data_ptr();
+  g.x_stride = x.stride(0);
+  g.w = w.data_ptr();
+  g.w_stride = w.stride(0);
+  g.dtype = dtype_code(x);
+  g.out_dtype = dtype_code(y);
+  g.activation = static_cast<int32_t>(activation);
+  g.M = M;
+  g.N = N;
+  g.K = K;
+  g.y = y.data_ptr();
+  g.y_stride = N;
+  const size_t ws_bytes = cdg_linear_workspace_bytes(&g);
+  torch::Tensor ws;
+  if (ws_bytes) ws = torch::empty({static_cast<int64_t>(ws_bytes)}, x.options().dtype(torch::kUInt8));
+  check_status(cdg_linear(&g, ws_bytes ? ws.data_ptr() : nullptr, ws_bytes, cur_stream(x)), "linear");
+  return py::make_tuple(y, preact ? py::cast(z) : py::none());
+}
+
+// (dx, dw, db), None where not asked for
+py::tuple linear_backward(const torch::Tensor& dy, const torch::Tensor& x, const torch::Tensor& w,
+                          const c10::optional<torch::Tensor>& z, int64_t activation, bool want_dx, bool want_dw,
+                          bool want_db) {
+  const auto dev = dy.device();
+  check_cuda(dy, "dy", dev);
+  check_cuda(x, "x", dev);
+  check_cuda(w, "weight", dev);
+  TORCH_CHECK_VALUE(x.dim() == 2 && w.dim() == 2, "x must be [M, K] and weight [N, K]");
+  TORCH_CHECK_VALUE(half_rows(x), "x must be BF16 or FP16, got ", x.scalar_type());
+  TORCH_CHECK_VALUE(w.scalar_type() == x.scalar_type() && dy.scalar_type() == x.scalar_type(),
+                    "dy and weight must have x's dtype");
+  const int64_t M = x.size(0), K = x.size(1), N = w.size(0);
+  check_rows(x, "x", dev, M, K);
+  check_rows(w, "weight", dev, N, K);
+  check_rows(dy, "dy", dev, M, N);
+  cdg_linear_backward_args g{};
+  if (activation != CDG_ACT_NONE) {
+    TORCH_CHECK_VALUE(z.has_value(), "an activation's gradient needs z, the value before it (linear(..., preact=True))");
+    check_rows(*z, "z", dev, M, N);
+    TORCH_CHECK_VALUE(z->scalar_type() == x.scalar_type(), "z must have x's dtype");
+    g.z = z->data_ptr();
+    g.z_stride = z->stride(0);
+  }
+  const c10::cuda::CUDAGuard guard(dev);
+  torch::Tensor dx, dw, db;
+  if (want_dx) {
+    dx = torch::empty({M, K}, x.options());
+    g.dx = dx.data_ptr();
+    g.dx_stride = K;
+  }
+  if (want_dw) {
+    dw = torch::empty({N, K}, x.options());
+    g.dw = dw.data_ptr();
+    g.dw_stride = K;
+  }
+  if (want_db) {
+    db = torch::empty({N}, x.options());
+    g.db = db.data_ptr();
+  }
+  g.db_dtype = dtype_code(x);
+  g.dy = dy.data_ptr();
+  g.dy_stride = dy.stride(0);
+  g.x = x.data_ptr();
+  g.x_stride = x.stride(0);
+  g.w = w.data_ptr();
+  g.w_stride = w.stride(0);
+  g.dtype = dtype_code(x);
+  g.activation = static_cast<int32_t>(activation);
+  g.M = M;
+  g.N = N;
+  g.K = K;
+  const size_t ws_bytes = cdg_linear_backward_workspace_bytes(&g);
+  torch::Tensor ws;
+  if (ws_bytes) ws = torch::empty({static_cast<int64_t>(ws_bytes)}, x.options().dtype(torch::kUInt8));
+  check_status(cdg_linear_backward(&g, ws_bytes ? ws.data_ptr() : nullptr, ws_bytes, cur_stream(x)), "linear_backward");
+  auto give = [](const torch::Tensor& t) -> py::object { return t.defined() ? py::cast(t) : py::none(); };
+  return py::make_tuple(give(dx), give(dw), give(db));
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -944,4 +1063,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("moe_route_backward", &moe_route_backward, py::arg("logits"), py::arg("ids"), py::arg("grad_weights"),
         py::arg("grad_loss"), py::arg("counts"), py::arg("tokens"), py::arg("sigmoid"), py::arg("renormalize"),
         py::arg("scale"));
+  m.def("linear", &linear, py::arg("x"), py::arg("weight"), py::arg("bias"), py::arg("residual"),
+        py::arg("activation"), py::arg("out_f32"), py::arg("preact"));
+  m.def("linear_backward", &linear_backward, py::arg("dy"), py::arg("x"), py::arg("weight"), py::arg("z"),
+        py::arg("activation"), py::arg("want_dx"), py::arg("want_dw"), py::arg("want_db"));
 }

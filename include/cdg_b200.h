@@ -599,6 +599,68 @@ typedef struct cdg_route_backward_args {
 
 int cdg_moe_route_backward(const cdg_route_backward_args* args, cdg_stream_t stream);
 
+/* Dense product with bias, activation and residual in its epilogue:
+ *   z = x w^T + bias (FP32),  y = act(z) + residual.
+ * x [M, K] and w [N, K] are both BF16 or both F16 (`dtype`), any row strides; bias [N] and
+ * residual [M, N] of `dtype` or F32, each may be NULL; y [M, N] of `dtype` or F32; z_out, when
+ * not NULL, receives z [M, N] in `dtype` (the backward call's z).  Sums are FP32; for an F32 y no
+ * running sum of the tensor cores covers more than 512 of K.  K = 0 gives act(bias) + residual.
+ * The workspace holds operands whose rows do not start on 16-byte boundaries (0 bytes when both do;
+ * then it may be NULL). */
+#define CDG_ACT_NONE 0
+#define CDG_ACT_RELU 1
+#define CDG_ACT_SILU 2      /* z / (1 + exp(-z)) */
+#define CDG_ACT_GELU 3      /* z (1 + erf(z / sqrt 2)) / 2 */
+#define CDG_ACT_GELU_TANH 4 /* z (1 + tanh(sqrt(2 / pi) (z + 0.044715 z^3))) / 2 */
+
+typedef struct cdg_linear_args {
+  const void* x;
+  int64_t x_stride;
+  const void* w;
+  int64_t w_stride;
+  const void* bias;
+  const void* residual;
+  int64_t residual_stride;
+  int32_t dtype, bias_dtype, residual_dtype, out_dtype;
+  int32_t activation; /* CDG_ACT_* */
+  int64_t M, N, K;
+  void* y;
+  int64_t y_stride;
+  void* z_out;
+  int64_t z_stride;
+} cdg_linear_args;
+
+size_t cdg_linear_workspace_bytes(const cdg_linear_args* args);
+int cdg_linear(const cdg_linear_args* args, void* workspace, size_t workspace_bytes, cdg_stream_t stream);
+
+/* Gradients of cdg_linear from dy, the gradient of y (also that of the residual):
+ *   dz = dy * act'(z),  dx = dz w,  dw = dz^T x,  db = sum over rows of dz.
+ * dy, x, w, z, dx, dw are of `dtype`; db of `dtype` or F32.  dx, dw and db may each be NULL.  z (the
+ * forward call's z_out) is read only with an activation; dz, an operand of both products, is held
+ * in `dtype`, db sums its FP32 values in a fixed order. */
+typedef struct cdg_linear_backward_args {
+  const void* dy;
+  int64_t dy_stride;
+  const void* x;
+  int64_t x_stride;
+  const void* w;
+  int64_t w_stride;
+  const void* z;
+  int64_t z_stride;
+  int32_t dtype, db_dtype;
+  int32_t activation;
+  int64_t M, N, K;
+  void* dx;
+  int64_t dx_stride;
+  void* dw;
+  int64_t dw_stride;
+  void* db;
+} cdg_linear_backward_args;
+
+size_t cdg_linear_backward_workspace_bytes(const cdg_linear_backward_args* args);
+int cdg_linear_backward(const cdg_linear_backward_args* args, void* workspace, size_t workspace_bytes,
+                        cdg_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

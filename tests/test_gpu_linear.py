@@ -1,0 +1,266 @@
+"""GPU checks of the dense product with its epilogue, and of its gradients.
+
+Against plain formulas in 64 bits on the same inputs.  Tolerances, with d the unit roundoff of the
+output's type (2^-8 BF16, 2^-11 FP16) and S = sum_k |x||w| of an element:
+  * The tensor cores add 16 products at a time to a 32-bit sum and may drop what lies below its
+    last bit: K / 16 additions of 17 terms, each within 2^-23 of S, so a sum is within
+    (K + 64) 2^-23 S however it was split.  Activations have slopes within 1.2 and are computed
+    within 2^-20 of their value and argument.
+  * An element is thus within d |y| + 1.2 (K + 64) 2^-23 S + 2^-20 (|act| + |z|), and the whole
+    result, whose errors are independent, within 0.6 d of its norm (a rounding's mean square is
+    d^2 / 3) plus 2^-18 for the sums.
+  * FP32 results: no running sum covers more than 512 of K, so the norm of the error is within
+    2^-19 of that of S-weighted results; checked as 2^-19 |y| in the norm and per element as above
+    without d.
+  * Gradients: dz is rounded to the operands' type, so an element of dx is within
+    d |dx| + (d + (N + 64) 2^-23) sum |dz||w|, and the norm of the error within 0.6 sqrt(2) d.
+"""
+
+import math
+
+import pytest
+import torch
+
+import cabi
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+UNIT = {torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11, torch.float32: 0.0}
+ACTS = [None, "relu", "silu", "gelu", "gelu_tanh"]
+
+
+def _cdg():
+    import consumer_deep_gemm
+
+    return consumer_deep_gemm
+
+
+def _act64(z, act):
+    if act == "relu":
+        return z.relu()  # slope 0 at 0
+    if act == "silu":
+        return z * torch.sigmoid(z)
+    if act == "gelu":
+        return z * torch.special.ndtr(z)
+    if act == "gelu_tanh":
+        return 0.5 * z * (1 + torch.tanh(math.sqrt(2 / math.pi) * (z + 0.044715 * z ** 3)))
+    return z
+
+
+def _operands(M, N, K, dtype, seed=0):
+    g = torch.Generator(device=DEV).manual_seed(seed)
+    x = torch.randn(M, K, generator=g, device=DEV).to(dtype)
+    w = (torch.randn(N, K, generator=g, device=DEV) / max(1, K) ** 0.5).to(dtype)
+    return x, w
+
+
+def _check(got, x, w, bias, residual, act, out_dtype):
+    K = x.shape[1]
+    z = x.double() @ w.double().t()
+    S = x.double().abs() @ w.double().abs().t()
+    if bias is not None:
+        z = z + bias.double()
+        S = S + bias.double().abs()
+    a = _act64(z, act)
+    y = a if residual is None else a + residual.double()
+    assert got.dtype == out_dtype and got.shape == y.shape
+    if y.numel() == 0:
+        return
+    err = (got.double() - y).abs()
+    d = UNIT[out_dtype]
+    slack = d * y.abs() + 1.2 * (K + 64) * 2.0 ** -23 * S + 2.0 ** -20 * (a.abs() + z.abs() + y.abs())
+    if out_dtype == torch.float16:
+        slack = slack + 2.0 ** -25
+    bad = err > slack
+    assert not bool(bad.any()), f"{int(bad.sum())} of {bad.numel()} out of tolerance, first {bad.nonzero()[0].tolist()}"
+    if y.numel() >= 64:
+        norm = 2.0 ** -19 if out_dtype == torch.float32 else 0.6 * d + 2.0 ** -18
+        assert float(err.norm()) <= norm * float((y.abs() + z.abs()).norm())
+    assert cabi.device_status() == (0, 0)
+
+
+SHAPES = [(1, 4096, 4096), (1, 1, 1), (1, 130, 33), (2, 256, 64), (3, 1000, 520), (8, 4096, 1024), (17, 77, 200),
+          (64, 512, 2048), (100, 64, 64), (128, 128, 128), (129, 257, 65), (300, 200, 72), (1000, 384, 1000),
+          (513, 1030, 333), (2048, 256, 4096), (256, 2048, 511), (5, 16, 8192), (700, 3, 100), (4096, 512, 128),
+          (2049, 1100, 1088), (1536, 2560, 320), (33, 8, 16)]
+
+
+@pytest.mark.parametrize("M,N,K", SHAPES)
+@pytest.mark.parametrize("dtype,out_dtype", [(torch.bfloat16, torch.bfloat16), (torch.float16, torch.float16),
+                                             (torch.bfloat16, torch.float32), (torch.float16, torch.float32)])
+def test_linear_against_64_bits(M, N, K, dtype, out_dtype):
+    x, w = _operands(M, N, K, dtype)
+    _check(_cdg().linear(x, w, out_dtype=out_dtype), x, w, None, None, None, out_dtype)
+    bias = torch.randn(N, device=DEV).to(dtype)
+    residual = torch.randn(M, N, device=DEV).to(dtype)
+    got = _cdg().linear(x, w, bias, residual, activation="silu", out_dtype=out_dtype)
+    _check(got, x, w, bias, residual, "silu", out_dtype)
+    assert torch.equal(got, _cdg().linear(x, w, bias, residual, activation="silu", out_dtype=out_dtype))
+
+
+@pytest.mark.parametrize("act", ACTS)
+@pytest.mark.parametrize("M,N,K", [(1, 300, 128), (200, 96, 100), (1024, 1024, 256), (4, 640, 4096)])
+def test_linear_epilogues(M, N, K, act):
+    x, w = _operands(M, N, K, torch.bfloat16, seed=1)
+    w = w * 3
+    for bias, residual in ((None, None), (torch.randn(N, device=DEV), None),
+                           (torch.randn(N, device=DEV).bfloat16(), torch.randn(M, N, device=DEV)),
+                           (None, torch.randn(M, N, device=DEV).bfloat16())):
+        for out in (torch.bfloat16, torch.float32):
+            _check(_cdg().linear(x, w, bias, residual, activation=act, out_dtype=out), x, w, bias, residual, act, out)
+
+
+def test_linear_preactivation_output():
+    x, w = _operands(130, 200, 96, torch.float16, seed=2)
+    bias = torch.randn(200, device=DEV).half()
+    y, z = _cdg().linear(x, w, bias, activation="gelu", preact=True)
+    _check(z, x, w, bias, None, None, torch.float16)
+    _check(y, x, w, bias, None, "gelu", torch.float16)
+
+
+@pytest.mark.parametrize("off,width", [(0, 128), (8, 264), (1, 130), (3, 200)])
+def test_linear_strides_broadcast_and_stream(off, width):
+    big = torch.randn(300, 512, device=DEV).bfloat16()
+    x = big[:150, off:off + width]
+    w = big[100:, off:off + width][::2]
+    residual = big.t()[:150].contiguous()[:, 7:107]
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        got = _cdg().linear(x, w, None, residual)
+    s.synchronize()
+    _check(got, x, w, None, residual, None, torch.bfloat16)
+    # one row of x, and one row of the residual, for every row
+    xb, rb = x[:1].expand(150, width), residual[:1].expand(150, 100)
+    _check(_cdg().linear(xb, w, None, rb), xb, w, None, rb, None, torch.bfloat16)
+
+
+def test_linear_empty():
+    x, w = _operands(5, 7, 0, torch.bfloat16)
+    bias = torch.randn(7, device=DEV)
+    r = torch.randn(5, 7, device=DEV).bfloat16()
+    _check(_cdg().linear(x, w, bias, r, activation="silu"), x, w, bias, r, "silu", torch.bfloat16)
+    _check(_cdg().linear(x, w, out_dtype=torch.float32), x, w, None, None, None, torch.float32)
+    x, w = _operands(0, 7, 16, torch.bfloat16)
+    assert _cdg().linear(x, w).shape == (0, 7)
+    x, w = _operands(4, 0, 16, torch.bfloat16)
+    assert _cdg().linear(x, w).shape == (4, 0)
+
+
+def test_linear_infinities_stay_in_their_rows():
+    x, w = _operands(200, 160, 320, torch.bfloat16, seed=3)
+    clean = _cdg().linear(x, w)
+    x2 = x.clone()
+    x2[17, 5] = math.inf
+    x2[140, 300] = math.nan
+    got = _cdg().linear(x2, w)
+    rows = torch.ones(200, dtype=torch.bool, device=DEV)
+    rows[17] = rows[140] = False
+    assert torch.equal(got[rows], clean[rows])
+    assert not bool(torch.isfinite(got[17]).any()) and bool(torch.isnan(got[140]).all())
+
+
+def _backward64(dy, x, w, z, act):
+    dz = dy.double()
+    if act:
+        zz = z.double().requires_grad_(True)
+        dz, = torch.autograd.grad(_act64(zz, act), zz, dz)
+    return dz
+
+
+def _check_gradient(got, want, terms, depth, d, count):
+    assert got.shape == want.shape
+    if want.numel() == 0:
+        return
+    slack = d * want.abs() + (d * (1 + 2.0 ** -8) + (depth + 64) * 2.0 ** -23) * terms + 2.0 ** -24
+    bad = (got.double() - want).abs() > slack
+    assert not bool(bad.any()), f"{int(bad.sum())} of {bad.numel()} out of tolerance"
+    if want.numel() >= 256:
+        err = (got.double() - want).norm()
+        assert float(err) <= (0.6 * math.sqrt(2) * d + 2.0 ** -18) * float(want.norm()) * 1.1 + 2.0 ** -24 * count
+
+
+@pytest.mark.parametrize("M,N,K", [(1, 64, 64), (1, 1, 1), (128, 256, 192), (130, 70, 100), (1000, 513, 257),
+                                   (2048, 256, 1024), (77, 1030, 40), (512, 2048, 512), (4099, 24, 136), (3000, 1024, 1536)])
+@pytest.mark.parametrize("dtype,act", [(torch.bfloat16, None), (torch.bfloat16, "silu"), (torch.float16, "gelu"),
+                                       (torch.bfloat16, "gelu_tanh"), (torch.float16, "relu")])
+def test_linear_backward_against_64_bits(M, N, K, dtype, act):
+    x, w = _operands(M, N, K, dtype, seed=4)
+    dy = torch.randn(M, N, device=DEV).to(dtype)
+    z = torch.randn(M, N, device=DEV).to(dtype) if act else None
+    dx, dw, db = _cdg().linear_backward(dy, x, w, z, activation=act, bias_grad=True)
+    dz = _backward64(dy, x, w, z, act)
+    d = UNIT[dtype]
+    count = dz.numel() ** 0.5
+    _check_gradient(dx, dz @ w.double(), dz.abs() @ w.double().abs(), N, d, count)
+    _check_gradient(dw, dz.t() @ x.double(), dz.abs().t() @ x.double().abs(), M, d, count)
+    # db: FP32 sums of values within 2^-20
+    slack = d * dz.sum(0).abs() + (M / 8 + 1100) * 2.0 ** -24 * dz.abs().sum(0) + 2.0 ** -20 * dz.abs().sum(0) + 2.0 ** -24
+    assert bool(((db.double() - dz.sum(0)).abs() <= slack).all())
+    again = _cdg().linear_backward(dy, x, w, z, activation=act, bias_grad=True)
+    assert all(torch.equal(a, b) for a, b in zip(again, (dx, dw, db)))
+    only = _cdg().linear_backward(dy, x, w, z, activation=act, weight_grad=False)
+    assert torch.equal(only[0], dx) and only[1] is None and only[2] is None
+    assert cabi.device_status() == (0, 0)
+
+
+def test_linear_backward_strides():
+    big = torch.randn(260, 700, device=DEV).half()
+    for off in (0, 8, 5):
+        dy, x, w = big[:200, off:off + 136], big[:200, 200 + off:280 + off], big[:136, 300 + off:380 + off]
+        z = big[60:, 400 + off:536 + off]
+        got = _cdg().linear_backward(dy, x, w, z, activation="silu", bias_grad=True)
+        want = _cdg().linear_backward(dy.contiguous(), x.contiguous(), w.contiguous(), z.contiguous(), activation="silu",
+                                      bias_grad=True)
+        for a, b in zip(got, want):
+            assert float((a.double() - b.double()).norm()) <= 2.0 ** -10 * float(b.double().norm())
+
+
+def test_linear_backward_against_differences():
+    """Central differences of sum(dy * y) in 64 bits; FP16 gradients within 2^-9 of the largest."""
+    x, w = _operands(6, 5, 9, torch.float16, seed=7)
+    dy = torch.randn(6, 5, device=DEV).half()
+    bias = torch.randn(5, device=DEV).half()
+    for act in ACTS[2:]:
+        y, z = _cdg().linear(x, w, bias, activation=act, preact=True)
+        dx, dw, db = _cdg().linear_backward(dy, x, w, z, activation=act, bias_grad=True)
+
+        def f(a, b, c):
+            return float((_act64(a @ b.t() + c, act) * dy.double()).sum())
+
+        x64, w64, b64 = x.double(), w.double(), bias.double()
+        for which, got in ((0, dx), (1, dw), (2, db)):
+            for at in ((0,), (got.numel() - 1,), (got.numel() // 2,)):
+                args = [x64, w64, b64]
+                e = torch.zeros_like(args[which]).view(-1)
+                e[at[0]] = 1e-5
+                e = e.view_as(args[which])
+                up = f(*(a + e if i == which else a for i, a in enumerate(args)))
+                down = f(*(a - e if i == which else a for i, a in enumerate(args)))
+                tol = 2.0 ** -9 * float(got.abs().max()) * 4
+                assert abs((up - down) / 2e-5 - float(got.view(-1)[at[0]])) < tol
+
+
+def test_linear_backward_empty():
+    x, w = _operands(0, 8, 16, torch.bfloat16)
+    dy = torch.empty(0, 8, device=DEV, dtype=torch.bfloat16)
+    dx, dw, db = _cdg().linear_backward(dy, x, w, bias_grad=True)
+    assert dx.shape == (0, 16) and float(dw.float().abs().sum()) == 0 and float(db.float().abs().sum()) == 0
+
+
+def test_linear_refusals():
+    cdg = _cdg()
+    x, w = _operands(4, 8, 16, torch.bfloat16)
+    dy = torch.zeros(4, 8, device=DEV, dtype=torch.bfloat16)
+    bad = [lambda: cdg.linear(x, w.half()), lambda: cdg.linear(x.float(), w.float()), lambda: cdg.linear(x, w[:, :8]),
+           lambda: cdg.linear(x, w, torch.zeros(7, device=DEV)), lambda: cdg.linear(x, w, torch.zeros(8, device=DEV).half()),
+           lambda: cdg.linear(x, w, None, torch.zeros(4, 7, device=DEV)), lambda: cdg.linear(x, w, activation="tanh"),
+           lambda: cdg.linear(x, w, out_dtype=torch.float16), lambda: cdg.linear(x[0], w),
+           lambda: cdg.linear(x.t(), torch.zeros(8, 4, device=DEV, dtype=torch.bfloat16)),
+           lambda: cdg.linear_backward(dy, x, w, activation="silu"), lambda: cdg.linear_backward(dy[:3], x, w),
+           lambda: cdg.linear_backward(dy.half(), x, w), lambda: cdg.linear_backward(dy, x, w, dy[:, :4], activation="relu")]
+    for call in bad:
+        with pytest.raises(ValueError):
+            call()
+    with pytest.raises(RuntimeError):
+        cdg.linear(x.cpu(), w)
