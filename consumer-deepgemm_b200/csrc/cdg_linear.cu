@@ -101,9 +101,15 @@ bool allow_smem() {
                               TileSmem<BN, PROMOTE>::kBytes) == cudaSuccess;
 }
 
+template <typename T, typename O, int BN>
+bool allow_pair_smem() {
+  return cudaFuncSetAttribute(cdg_linear_pair_kernel<T, O, BN>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                              PairTileSmem<BN>::kBytes) == cudaSuccess;
+}
+
 template <typename T>
 bool allow_smem_of() {
-  return allow_smem<T, T, 64, false>() && allow_smem<T, T, 128, false>() && allow_smem<T, float, 64, true>() &&
+  return allow_pair_smem<T, T, 256>() && allow_pair_smem<T, float, 128>() && allow_smem<T, T, 64, false>() && allow_smem<T, T, 128, false>() && allow_smem<T, float, 64, true>() &&
          allow_smem<T, float, 128, true>();
 }
 
@@ -156,16 +162,20 @@ int repack(Matrix& m, uint8_t*& ws, cudaStream_t st) {
   return launched();
 }
 
-int make_map(CUtensorMap* map, const Matrix& m, bool bf16, uint32_t box_rows) {
+// Boxes of 128 bytes x box_rows in the 128-byte swizzle.
+int make_map(CUtensorMap* map, const Matrix& m, int dtype, uint32_t box_rows) {
   EncodeTiledFn enc = encode_tiled();
   if (!enc) return CDG_ERR_CUDA;
+  const int64_t e = element_size(dtype);
   cuuint64_t dims[2] = {static_cast<cuuint64_t>(m.cols), static_cast<cuuint64_t>(m.rows)};
   // one row may have any stride; the map wants a multiple of 16 bytes all the same
-  cuuint64_t strides[1] = {static_cast<cuuint64_t>(m.rows > 1 ? m.stride : padded(m.cols)) * 2};
-  cuuint32_t box[2] = {64, box_rows};
+  cuuint64_t strides[1] = {static_cast<cuuint64_t>(m.rows > 1 ? m.stride : padded(m.cols)) * e};
+  cuuint32_t box[2] = {static_cast<cuuint32_t>(128 / e), box_rows};
   cuuint32_t estr[2] = {1, 1};
-  return enc(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2,
-             const_cast<void*>(m.p), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+  const CUtensorMapDataType type = dtype == CDG_DTYPE_BF16  ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
+                                   : dtype == CDG_DTYPE_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
+                                                            : CU_TENSOR_MAP_DATA_TYPE_FLOAT32;
+  return enc(map, type, 2, const_cast<void*>(m.p), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
              CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS
              ? CDG_OK
@@ -191,13 +201,35 @@ int launch_tiles(const CUtensorMap& ta, const CUtensorMap& tb, const LinearShape
              : CDG_ERR_CUDA;
 }
 
+template <typename T, typename O, int BN>
+int launch_pairs(const Matrix& A, const Matrix& B, const LinearShape& s, Epilogue e, int64_t M, int64_t N,
+                 cudaStream_t st) {
+  constexpr int kType = std::is_same<T, __nv_bfloat16>::value ? CDG_DTYPE_BF16 : CDG_DTYPE_F16;
+  constexpr int kOut = sizeof(O) == 4 ? CDG_DTYPE_F32 : kType;
+  CUtensorMap ta{}, tb{}, ty{}, tr{};
+  int rc = make_map(&ta, A, kType, s.a_mn ? 64 : 128);
+  if (rc == CDG_OK) rc = make_map(&tb, B, kType, s.b_mn ? 64 : BN / 2);
+  // a box of y or of the residual is one warp's 32 rows x 128 bytes
+  const Matrix y{e.y, e.y_stride, M, N}, r{e.residual, e.residual_stride, M, N};
+  const bool apart = M == 1 || (y.stride >= N && (!e.residual || r.stride >= N));
+  e.staged = e.wide && !e.z && apart && (!e.residual || (e.residual_f32 != 0) == (sizeof(O) == 4));
+  if (rc == CDG_OK && e.staged) rc = make_map(&ty, y, kOut, 32);
+  if (rc == CDG_OK && e.staged && e.residual) rc = make_map(&tr, r, kOut, 32);
+  if (rc != CDG_OK) return rc;
+  const unsigned grid =
+      static_cast<unsigned>(2 * std::min<int64_t>(int64_t(s.m_tiles) * s.n_tiles, std::max(1, sm_count() / 2)));
+  cdg_linear_pair_kernel<T, O, BN>
+      <<<grid, PairTileSmem<BN>::kThreads, PairTileSmem<BN>::kBytes, st>>>(ta, tb, ty, tr, s, e);
+  return launched();
+}
+
 // D [M, N] = epilogue(sum over K of A and B); a_mn: A lies as [K, M], else [M, K]; b_mn: B lies as
 // [K, N], else [N, K].  Rows of both on 16-byte boundaries.
 template <typename T, typename O>
 int product(const Matrix& A, bool a_mn, const Matrix& B, bool b_mn, int64_t M, int64_t N, int64_t K,
             const Epilogue& e, cudaStream_t st) {
   constexpr bool kPromote = sizeof(O) == 4;
-  constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
+  constexpr int kType = std::is_same<T, __nv_bfloat16>::value ? CDG_DTYPE_BF16 : CDG_DTYPE_F16;
   if (M == 0 || N == 0) return CDG_OK;
   LinearShape s{};
   s.M = M;
@@ -205,10 +237,17 @@ int product(const Matrix& A, bool a_mn, const Matrix& B, bool b_mn, int64_t M, i
   s.k_steps = static_cast<int>((K + 63) / 64);
   s.a_mn = a_mn;
   s.b_mn = b_mn;
-  s.bf16 = kBf16;
+  s.bf16 = kType == CDG_DTYPE_BF16;
   s.a_rows = static_cast<int>(std::min<int64_t>(128, (M + 7) / 8 * 8));
-  const int64_t m_tiles = (M + 127) / 128;
   const int sms = sm_count();
+  constexpr int kPairN = kPromote ? 128 : 256;
+  const int64_t pair_tiles = ((M + 255) / 256) * ((N + kPairN - 1) / kPairN);
+  if (K > 0 && pair_tiles >= sms / 2 && pair_tiles < (int64_t(1) << 30)) {
+    s.m_tiles = static_cast<int>((M + 255) / 256);
+    s.n_tiles = static_cast<int>((N + kPairN - 1) / kPairN);
+    return launch_pairs<T, O, kPairN>(A, B, s, e, M, N, st);
+  }
+  const int64_t m_tiles = (M + 127) / 128;
   const int bn = m_tiles * ((N + 127) / 128) >= sms ? 128 : 64;
   const int64_t n_tiles = (N + bn - 1) / bn;
   if (m_tiles * n_tiles * 8 > 0x7fffffff) return CDG_ERR_UNSUPPORTED;
@@ -219,8 +258,8 @@ int product(const Matrix& A, bool a_mn, const Matrix& B, bool b_mn, int64_t M, i
   while (splits < 8 && m_tiles * n_tiles * splits * 2 <= 2 * sms && s.k_steps / (splits * 2) >= 4) splits *= 2;
   CUtensorMap ta{}, tb{};
   if (K > 0) {
-    int rc = make_map(&ta, A, kBf16, a_mn ? 64 : s.a_rows);
-    if (rc == CDG_OK) rc = make_map(&tb, B, kBf16, b_mn ? 64 : bn);
+    int rc = make_map(&ta, A, kType, a_mn ? 64 : s.a_rows);
+    if (rc == CDG_OK) rc = make_map(&tb, B, kType, b_mn ? 64 : bn);
     if (rc != CDG_OK) return rc;
   }
   return bn == 128 ? launch_tiles<T, O, 128, kPromote>(ta, tb, s, e, splits, st)
@@ -256,6 +295,7 @@ int forward(const cdg_linear_args* g, uint8_t* ws, cudaStream_t st) {
   e.y_stride = g->y_stride;
   e.z = g->z_out;
   e.z_stride = g->z_stride;
+  e.wide_bias = e.bias && !e.bias_f32 && reinterpret_cast<uintptr_t>(e.bias) % 16 == 0;
   e.wide = wide_columns(e.y, e.y_stride, element_size(g->out_dtype)) && wide_columns(e.z, e.z_stride, 2) &&
            wide_columns(e.residual, e.residual_stride, e.residual_f32 ? 4 : 2);
   return g->out_dtype == CDG_DTYPE_F32 ? product<T, float>(x, false, w, false, g->M, g->N, g->K, e, st)

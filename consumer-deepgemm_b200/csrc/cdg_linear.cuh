@@ -121,7 +121,9 @@ struct Epilogue {
   void* z;  // the value before the activation, in the operands' type; NULL = not stored
   int64_t residual_stride, y_stride, z_stride;
   int bias_f32, residual_f32, act;
-  int wide;  // y, z and residual rows on 16-byte boundaries
+  int wide;       // y, z and residual rows on 16-byte boundaries
+  int wide_bias;  // bias of the operands' type, on a 16-byte boundary
+  int staged;     // pair kernel: y and residual through shared memory and TMA
 };
 
 template <typename T>
@@ -418,6 +420,380 @@ __global__ void __launch_bounds__(kTileThreads)
   if (warp == 5) {
     tc_fence_after();
     tmem_dealloc(tmem, L::kTmemCols);
+  }
+}
+
+// ---------------------------------------------------------------- CTA pairs, persistent, for many tiles
+// A pair of CTAs takes tiles of 256 x BN in turn: CTA r of it holds rows 128r .. 128r + 127 of A and
+// of the result and half of B's rows.  The tensor cores fill one of two accumulators in TMEM while
+// eight epilogue warps per CTA empty the other (warp w: the 32 lanes of quadrant w % 4, half of the
+// columns).  Staged (y, and the residual where there is one, of the output's type and on 16-byte
+// rows, z not stored): each epilogue warp has the residual brought into its own two shared-memory
+// tiles of 32 rows x 128 bytes by TMA, ahead of the accumulator, adds it in place and has the result
+// stored from there, so that global memory sees whole tiles; clipping at M and N is TMA's.
+// Otherwise its lanes load and store their rows themselves.
+// Warps: 0 TMA producer, 1 MMA issuer (even CTA) and TMEM owner, 4-11 epilogue.
+template <int BN>
+struct PairTileSmem {
+  static constexpr int kA = 128 * 128;
+  static constexpr int kB = BN / 2 * 128;
+  static constexpr int kStageBytes = kA + kB;
+  static constexpr int kStages = BN == 256 ? 5 : 6;
+  static constexpr int kEpiWarps = 8;
+  static constexpr int kStaging = kStages * kStageBytes;      // [warp][2] tiles of 4096 bytes
+  static constexpr int kBars = kStaging + kEpiWarps * 2 * 4096;
+  // full, empty [kStages]; tfull, tempty [2]; done; residual [warp][2]; TMEM address
+  static constexpr int kBytes = kBars + (2 * kStages + 5 + kEpiWarps * 2) * 8 + 16 + 1024;
+  static constexpr int kThreads = 128 + 32 * kEpiWarps;
+  static_assert(kBytes <= 232448, "shared memory per CTA");
+};
+
+__device__ __forceinline__ void tc_mma_f16_pair_warp(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
+                                                     uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p, e;\n\t"
+      "elect.sync _|e, 0xffffffff;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "@e tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+      ::"r"(d_tmem), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
+// 2-D tiled store of one box from shared memory (bulk group of the issuing thread).
+__device__ __forceinline__ void tma_store_2d(const void* tmap, const void* src, int32_t x, int32_t y) {
+  asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%2, %3}], [%1];"
+               ::"l"(reinterpret_cast<uint64_t>(tmap)), "r"(smem_u32(src)), "r"(x), "r"(y)
+               : "memory");
+}
+__device__ __forceinline__ void bulk_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
+// The stores issued by this thread have read their shared memory / have completed.
+__device__ __forceinline__ void bulk_wait_read() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
+__device__ __forceinline__ void bulk_wait_all() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
+
+// Tile t of a grid of m_tiles x n_tiles: bands of kBand row tiles, column by column, so that the
+// tiles in flight share their operands in L2.
+constexpr int kBand = 8;
+__device__ __forceinline__ void tile_at(int t, int m_tiles, int n_tiles, int& mt, int& nt) {
+  const int band = t / (kBand * n_tiles), first = band * kBand;
+  const int height = min(kBand, m_tiles - first), in = t - band * kBand * n_tiles;
+  mt = first + in % height;
+  nt = in / height;
+}
+
+// Values of the lane's row for CH consecutive columns from n on, from the accumulator (v), through
+// the epilogue, in place of the residual in the staged tile (row `lane`, 128 bytes, 16-byte pieces
+// XORed with the row's low three bits: the 128-byte swizzle).
+template <typename T, typename O, int CH>
+__device__ __forceinline__ void finish_staged(const Epilogue& e, int64_t n, int64_t N, float (&v)[CH], uint8_t* tile,
+                                              int lane) {
+  constexpr int kPer = 16 / static_cast<int>(sizeof(O));  // columns per 16-byte piece
+  if (e.bias) {
+    if (e.wide_bias && n + CH <= N) {
+#pragma unroll
+      for (int g = 0; g < CH / 8; ++g) {
+        const uint4 r = __ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(e.bias) + n) + g);
+        const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float2 f = unpack2(w[j], T());
+          v[g * 8 + 2 * j] += f.x;
+          v[g * 8 + 2 * j + 1] += f.y;
+        }
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < CH; ++j)
+        if (n + j < N) v[j] += load_any<T>(e.bias, n + j, e.bias_f32);
+    }
+  }
+  switch (e.act) {  // one test per chunk, not per value
+    case CDG_ACT_RELU:
+#pragma unroll
+      for (int j = 0; j < CH; ++j) v[j] = activate(v[j], CDG_ACT_RELU);
+      break;
+    case CDG_ACT_SILU:
+#pragma unroll
+      for (int j = 0; j < CH; ++j) v[j] = activate(v[j], CDG_ACT_SILU);
+      break;
+    case CDG_ACT_GELU:
+#pragma unroll
+      for (int j = 0; j < CH; ++j) v[j] = activate(v[j], CDG_ACT_GELU);
+      break;
+    case CDG_ACT_GELU_TANH:
+#pragma unroll
+      for (int j = 0; j < CH; ++j) v[j] = activate(v[j], CDG_ACT_GELU_TANH);
+      break;
+    default: break;
+  }
+#pragma unroll
+  for (int c = 0; c < CH / kPer; ++c) {
+    uint4* at = reinterpret_cast<uint4*>(tile + lane * 128 + ((c ^ (lane & 7)) << 4));
+    if (e.residual) {
+      const uint4 r = *at;
+      const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if constexpr (sizeof(O) == 4) {
+          v[c * kPer + j] += __uint_as_float(w[j]);
+        } else {
+          const float2 f = unpack2(w[j], O());
+          v[c * kPer + 2 * j] += f.x;
+          v[c * kPer + 2 * j + 1] += f.y;
+        }
+      }
+    }
+    if constexpr (sizeof(O) == 4) {
+      *at = make_uint4(__float_as_uint(v[c * 4]), __float_as_uint(v[c * 4 + 1]), __float_as_uint(v[c * 4 + 2]),
+                       __float_as_uint(v[c * 4 + 3]));
+    } else {
+      *at = make_uint4(pack2(v[c * 8], v[c * 8 + 1], O()), pack2(v[c * 8 + 2], v[c * 8 + 3], O()),
+                       pack2(v[c * 8 + 4], v[c * 8 + 5], O()), pack2(v[c * 8 + 6], v[c * 8 + 7], O()));
+    }
+  }
+}
+
+template <typename T, typename O, int BN>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairTileSmem<BN>::kThreads, 1)
+    cdg_linear_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_b,
+                           const __grid_constant__ CUtensorMap tmap_y, const __grid_constant__ CUtensorMap tmap_r,
+                           const LinearShape s, const Epilogue e) {
+  using L = PairTileSmem<BN>;
+  constexpr bool PROMOTE = sizeof(O) == 4;
+  constexpr int S = L::kStages;
+  constexpr int CH = 128 / static_cast<int>(sizeof(O));  // columns of a staged tile
+  constexpr int kChunks = BN / 2 / CH;                   // staged tiles of a warp per output tile
+  static_assert(kChunks == 2, "two staged tiles per warp");
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + L::kBars);
+  uint64_t* empty = full + S;
+  uint64_t* tfull = empty + S;
+  uint64_t* tempty = tfull + 2;
+  uint64_t* done = tempty + 2;
+  uint64_t* rfull = done + 1;
+  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(rfull + L::kEpiWarps * 2);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = cluster_ctarank();
+  const int pair = static_cast<int>(blockIdx.x >> 1), pairs = static_cast<int>(gridDim.x >> 1);
+  const int tiles = s.m_tiles * s.n_tiles;
+
+  if (warp == 0 && lane == 0) {
+    prefetch_tmap(&tmap_a);
+    prefetch_tmap(&tmap_b);
+    for (int i = 0; i < S; ++i) {
+      mbar_init(&full[i], 1);
+      mbar_init(&empty[i], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&tfull[i], 1);
+      mbar_init(&tempty[i], 2 * 32 * L::kEpiWarps);
+    }
+    mbar_init(done, 1);
+    for (int i = 0; i < 2 * L::kEpiWarps; ++i) mbar_init(&rfull[i], 1);
+    fence_mbarrier_init();
+  }
+  if (warp == 1) {
+    tmem_alloc_pair(tmem_holder, 2 * BN);
+    tmem_relinquish_pair();
+  }
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync();  // both CTAs' barriers ready before any copy or commit reaches them
+  tc_fence_after();
+  const uint32_t tmem = *tmem_holder;
+  bool ok = true;
+
+  if (warp == 0) {
+    if (lane == 0) {
+      int stage = 0;
+      uint32_t phase = 0;
+      const uint32_t full0 = cluster_addr(&full[0], 0);
+      for (int t = pair; t < tiles && ok; t += pairs) {
+        int mt, nt;
+        tile_at(t, s.m_tiles, s.n_tiles, mt, nt);
+        const int m0 = mt * 256 + static_cast<int>(rank) * 128, n0 = nt * BN + static_cast<int>(rank) * (BN / 2);
+        for (int k = 0; k < s.k_steps; ++k) {
+          if (!mbar_wait_cluster(&empty[stage], phase ^ 1, nullptr, wait_code(1, static_cast<int>(rank), stage, phase ^ 1, k))) {
+            ok = false;
+            break;
+          }
+          const uint32_t fb = full0 + stage * 8;
+          if (rank == 0) mbar_arrive_expect_tx(&full[stage], 2u * L::kStageBytes);
+          uint8_t* a = smem + stage * L::kStageBytes;
+          uint8_t* b = a + L::kA;
+          if (s.a_mn) {
+            tma_load_2d_pair(a, &tmap_a, fb, m0, k * 64);
+            tma_load_2d_pair(a + 8192, &tmap_a, fb, m0 + 64, k * 64);
+          } else {
+            tma_load_2d_pair(a, &tmap_a, fb, k * 64, m0);
+          }
+          if (s.b_mn) {
+#pragma unroll
+            for (int c = 0; c < BN / 128; ++c) tma_load_2d_pair(b + c * 8192, &tmap_b, fb, n0 + c * 64, k * 64);
+          } else {
+            tma_load_2d_pair(b, &tmap_b, fb, k * 64, n0);
+          }
+          if (++stage == S) { stage = 0; phase ^= 1; }
+        }
+      }
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    if (rank == 0) {
+      const uint32_t idesc = idesc_f16(s.bf16, s.a_mn, s.b_mn, 256, BN);
+      const uint32_t a_step = operand_k_step(s.a_mn), b_step = operand_k_step(s.b_mn);
+      int stage = 0, sum = 0;
+      uint32_t phase = 0;
+      for (int t = pair; t < tiles && ok; t += pairs) {
+        for (int k = 0; k < s.k_steps && ok; ++sum) {
+          const int buf = sum & 1;
+          if (!mbar_wait_cluster_warp(&tempty[buf], ((sum >> 1) & 1) ^ 1, nullptr, wait_code(2, 0, buf, sum >> 1, k))) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          const int end = PROMOTE ? min(s.k_steps, k + kPromoteSteps) : s.k_steps;
+          for (uint32_t more = 0; k < end; ++k) {
+            if (!mbar_wait_cta_warp(&full[stage], phase, nullptr, wait_code(3, 0, stage, phase, k))) {
+              ok = false;
+              break;
+            }
+            tc_fence_after();
+            const uint32_t base = smem_u32(smem + stage * L::kStageBytes);
+            const uint64_t ad = operand_desc(base, s.a_mn), bd = operand_desc(base + L::kA, s.b_mn);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              tc_mma_f16_pair_warp(tmem + buf * BN, ad + j * a_step, bd + j * b_step, idesc, more);
+              more = 1;
+            }
+            tc_commit_pair_warp(&empty[stage], 0x3);
+            if (++stage == S) { stage = 0; phase ^= 1; }
+          }
+          if (ok) tc_commit_pair_warp(&tfull[buf], 0x3);
+        }
+      }
+      tc_commit_pair_warp(done, 0x1);  // every product completes before teardown
+      mbar_wait_cluster_warp(done, 0, nullptr, wait_code(5, 0, 0, 0, 0));
+    }
+  } else if (warp >= 4) {
+    const int w = warp - 4, half = w >> 2, q = warp & 3;
+    const uint32_t tempty0 = cluster_addr(&tempty[0], 0);
+    uint8_t* stagings = smem + L::kStaging + w * 2 * 4096;
+    const uint32_t lanes = tmem + (static_cast<uint32_t>(q * 32) << 16) + half * (BN / 2);
+    int sum = 0;
+    uint32_t turn[kChunks] = {};  // phase of each staged tile's residual barrier
+    for (int t = pair; t < tiles && ok; t += pairs) {
+      int mt, nt;
+      tile_at(t, s.m_tiles, s.n_tiles, mt, nt);
+      const int row0 = mt * 256 + static_cast<int>(rank) * 128 + q * 32, col0 = nt * BN + half * (BN / 2);
+      const bool any = row0 < s.M;  // a warp past the last row only keeps the barriers moving
+      if (e.staged && any) {
+        if (lane == 0) {
+          bulk_wait_read();  // the last tile's stores have read the staged tiles
+          if (e.residual) {
+#pragma unroll
+            for (int c = 0; c < kChunks; ++c) {
+              if (col0 + c * CH < s.N) {
+                mbar_arrive_expect_tx(&rfull[w * 2 + c], 4096);
+                tma_load_2d(stagings + c * 4096, &tmap_r, &rfull[w * 2 + c], col0 + c * CH, row0);
+              }
+            }
+          }
+        }
+        __syncwarp();
+      }
+      float acc[PROMOTE ? BN / 2 : 1];
+      if constexpr (PROMOTE) {
+#pragma unroll
+        for (int j = 0; j < BN / 2; ++j) acc[j] = 0.0f;
+        for (int k = 0; k < s.k_steps; k += kPromoteSteps, ++sum) {
+          const int buf = sum & 1;
+          if (!mbar_wait_cluster_warp(&tfull[buf], (sum >> 1) & 1, nullptr, wait_code(4, static_cast<int>(rank), buf, sum >> 1, k))) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+#pragma unroll
+          for (int c = 0; c < BN / 64; ++c) {
+            uint32_t r[32];
+            tmem_ld32(lanes + buf * BN + c * 32, r);
+            tmem_ld_wait();
+#pragma unroll
+            for (int j = 0; j < 32; ++j) acc[c * 32 + j] += __uint_as_float(r[j]);
+          }
+          tc_fence_before();
+          if (rank == 0) mbar_arrive(&tempty[buf]); else mbar_arrive_cluster(tempty0 + buf * 8);
+        }
+        if (!ok) break;
+      } else {
+        if (!mbar_wait_cluster_warp(&tfull[sum & 1], (sum >> 1) & 1, nullptr, wait_code(4, static_cast<int>(rank), sum & 1, sum >> 1, 0))) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+      }
+#pragma unroll
+      for (int c = 0; c < kChunks; ++c) {
+        const int n = col0 + c * CH;
+        float v[CH];
+        if constexpr (PROMOTE) {
+#pragma unroll
+          for (int j = 0; j < CH; ++j) v[j] = acc[c * CH + j];
+        } else {
+          uint32_t r0[32], r1[32];
+          tmem_ld32(lanes + (sum & 1) * BN + c * CH, r0);
+          tmem_ld32(lanes + (sum & 1) * BN + c * CH + 32, r1);
+          tmem_ld_wait();
+#pragma unroll
+          for (int j = 0; j < 32; ++j) {
+            v[j] = __uint_as_float(r0[j]);
+            v[(32 + j) % CH] = __uint_as_float(r1[j]);
+          }
+          if (c == kChunks - 1) {
+            tc_fence_before();
+            if (rank == 0) mbar_arrive(&tempty[sum & 1]); else mbar_arrive_cluster(tempty0 + (sum & 1) * 8);
+          }
+        }
+        if (!any || n >= s.N) continue;
+        if (e.staged) {
+          if (e.residual) {
+            if (!mbar_wait_cta_warp(&rfull[w * 2 + c], turn[c], nullptr, wait_code(4, 8 + w, c, turn[c], 0))) ok = false;
+            turn[c] ^= 1;
+          }
+          finish_staged<T, O, CH>(e, n, s.N, v, stagings + c * 4096, lane);
+          fence_proxy_async_shared();
+          __syncwarp();
+          if (lane == 0) {
+            tma_store_2d(&tmap_y, stagings + c * 4096, n, row0);
+            bulk_commit();
+          }
+        } else if (row0 + lane < s.M) {
+#pragma unroll
+          for (int g = 0; g < CH / 8; ++g) {
+            float u[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) u[j] = v[g * 8 + j];
+            if (n + g * 8 < s.N) finish8<T, O>(e, row0 + lane, n + g * 8, s.N, u);
+          }
+        }
+      }
+      if constexpr (!PROMOTE) ++sum;
+    }
+    if (e.staged && lane == 0) bulk_wait_all();
+    __syncwarp();
+  }
+
+  tc_fence_before();
+  const int any_fail = __syncthreads_or(!ok);
+  cluster_sync();  // no CTA releases TMEM or exits while its pair still uses it
+  if (any_fail) {
+    // after a wait that gave up, copies issued before it still land: give them time before exit
+    const uint64_t t0 = global_timer_ns();
+    while (global_timer_ns() - t0 < 200000ull) __nanosleep(20000);
+  }
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc_pair(tmem, 2 * BN);
   }
 }
 

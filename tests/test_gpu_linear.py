@@ -110,6 +110,23 @@ def test_linear_epilogues(M, N, K, act):
             _check(_cdg().linear(x, w, bias, residual, activation=act, out_dtype=out), x, w, bias, residual, act, out)
 
 
+@pytest.mark.parametrize("M,N,K", [(4611, 2568, 130), (8200, 2600, 64), (2560, 2305, 520), (19000, 256, 72)])
+@pytest.mark.parametrize("dtype,out_dtype", [(torch.bfloat16, torch.bfloat16), (torch.float16, torch.float32)])
+def test_linear_many_tiles(M, N, K, dtype, out_dtype):
+    """Enough 256 x 256 tiles for every SM pair to take several, with ragged edges."""
+    x, w = _operands(M, N, K, dtype, seed=5)
+    bias = torch.randn(N, device=DEV)
+    for b, r, act in ((None, None, None), (bias.to(dtype), torch.randn(M, N, device=DEV).to(out_dtype), "gelu_tanh"),
+                      (bias, torch.randn(M, N, device=DEV), "relu"),
+                      (None, torch.randn(M, N, device=DEV).to(dtype), None)):
+        got = _cdg().linear(x, w, b, r, activation=act, out_dtype=out_dtype)
+        _check(got, x, w, b, r, act, out_dtype)
+        assert torch.equal(got, _cdg().linear(x, w, b, r, activation=act, out_dtype=out_dtype))
+    y, z = _cdg().linear(x, w, bias, activation="silu", out_dtype=out_dtype, preact=True)
+    _check(z, x, w, bias, None, None, dtype)
+    _check(y, x, w, bias, None, "silu", out_dtype)
+
+
 def test_linear_preactivation_output():
     x, w = _operands(130, 200, 96, torch.float16, seed=2)
     bias = torch.randn(200, device=DEV).half()
@@ -181,7 +198,8 @@ def _check_gradient(got, want, terms, depth, d, count):
 
 
 @pytest.mark.parametrize("M,N,K", [(1, 64, 64), (1, 1, 1), (128, 256, 192), (130, 70, 100), (1000, 513, 257),
-                                   (2048, 256, 1024), (77, 1030, 40), (512, 2048, 512), (4099, 24, 136), (3000, 1024, 1536)])
+                                   (2048, 256, 1024), (77, 1030, 40), (512, 2048, 512), (4099, 24, 136), (3000, 1024, 1536), (2312, 2570, 2500),
+                                   (5000, 2056, 1032)])
 @pytest.mark.parametrize("dtype,act", [(torch.bfloat16, None), (torch.bfloat16, "silu"), (torch.float16, "gelu"),
                                        (torch.bfloat16, "gelu_tanh"), (torch.float16, "relu")])
 def test_linear_backward_against_64_bits(M, N, K, dtype, act):
