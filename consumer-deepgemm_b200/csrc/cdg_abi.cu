@@ -654,12 +654,13 @@ int cdg_read_device_status(const void* workspace, cdg_stream_t stream) {
 namespace cdg {
 int ep_sticky_status(int clear, int32_t* out);  // cdg_moe.cu: the exchange kernels' record
 int linear_sticky_status(int clear, int32_t* out);  // cdg_linear.cu: the dense product's record
+int norm_sticky_status(int clear, int32_t* out);    // cdg_norm.cu: the norm's
 }  // namespace cdg
 
 extern "C" {
 
 int cdg_device_status(int32_t clear, int32_t* where) {
-  int32_t gemm[2] = {0, 0}, ep[2] = {0, 0}, lin[2] = {0, 0};
+  int32_t gemm[2] = {0, 0}, ep[2] = {0, 0}, lin[2] = {0, 0}, norm[2] = {0, 0};
   if (cudaDeviceSynchronize() != cudaSuccess) return CDG_ERR_CUDA;
   if (cudaMemcpyFromSymbol(gemm, cdg::g_sticky_status, sizeof(gemm)) != cudaSuccess) return CDG_ERR_CUDA;
   if (clear) {
@@ -668,9 +669,10 @@ int cdg_device_status(int32_t clear, int32_t* where) {
   }
   int st = cdg::ep_sticky_status(clear, ep);
   if (st == CDG_OK) st = cdg::linear_sticky_status(clear, lin);
+  if (st == CDG_OK) st = cdg::norm_sticky_status(clear, norm);
   if (st != CDG_OK) return st;
-  if (where) *where = gemm[1] ? gemm[1] : ep[1] ? ep[1] : lin[1];
-  const int bits = gemm[0] | ep[0] | lin[0];
+  if (where) *where = gemm[1] ? gemm[1] : ep[1] ? ep[1] : lin[1] ? lin[1] : norm[1];
+  const int bits = gemm[0] | ep[0] | lin[0] | norm[0];
   return (bits & cdg::kStatusTimeout) ? CDG_ERR_DEVICE_TIMEOUT : bits ? CDG_ERR_DEVICE_INDEX : CDG_OK;
 }
 

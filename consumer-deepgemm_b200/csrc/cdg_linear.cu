@@ -93,8 +93,6 @@ __global__ void __launch_bounds__(256) linear_dz_kernel(const T* dy, int64_t dy_
 }
 
 // ------------------------------------------------------------------ host
-constexpr int kMaxDevices = 64;
-
 template <typename T, typename O, int BN, bool PROMOTE>
 bool allow_smem() {
   return cudaFuncSetAttribute(cdg_linear_tile_kernel<T, O, BN, PROMOTE>, cudaFuncAttributeMaxDynamicSharedMemorySize,
@@ -347,9 +345,9 @@ int backward(const cdg_linear_backward_args* g, uint8_t* ws, cudaStream_t st) {
     if (g->db) {
       const unsigned blocks = static_cast<unsigned>((g->N + 31) / 32);
       if (g->db_dtype == CDG_DTYPE_F32)
-        column_sum_kernel<float><<<blocks, 256, 0, st>>>(partial, groups, g->N, static_cast<float*>(g->db));
+        column_sum_kernel<float><<<blocks, 1024, 0, st>>>(partial, groups, g->N, static_cast<float*>(g->db));
       else
-        column_sum_kernel<T><<<blocks, 256, 0, st>>>(partial, groups, g->N, static_cast<T*>(g->db));
+        column_sum_kernel<T><<<blocks, 1024, 0, st>>>(partial, groups, g->N, static_cast<T*>(g->db));
       rc = launched();
       if (rc != CDG_OK) return rc;
     }
@@ -405,14 +403,7 @@ int check_backward(const cdg_linear_backward_args* g) {
 }  // namespace
 
 // This unit's record of waits that gave up (cdg_device_status reads it with the others').
-int linear_sticky_status(int clear, int32_t* out) {
-  if (cudaMemcpyFromSymbol(out, g_sticky_status, 2 * sizeof(int32_t)) != cudaSuccess) return CDG_ERR_CUDA;
-  if (clear && (out[0] || out[1])) {
-    const int32_t z[2] = {0, 0};
-    if (cudaMemcpyToSymbol(g_sticky_status, z, sizeof(z)) != cudaSuccess) return CDG_ERR_CUDA;
-  }
-  return CDG_OK;
-}
+int linear_sticky_status(int clear, int32_t* out) { return read_sticky(g_sticky_status, clear, out); }
 
 }  // namespace cdg
 

@@ -18,8 +18,10 @@
 
 #include <algorithm>
 #include <cstdint>
+#include <mutex>
 
 #include "cdg_b200.h"
+#include "cdg_ptx.cuh"
 #include "cdg_rows.cuh"
 
 namespace cdg {
@@ -183,6 +185,8 @@ __global__ void __launch_bounds__(THREADS) add_rms_norm_kernel(const NormFwd a, 
   }
 }
 
+constexpr int kRingMax = 8;  // rows in flight per CTA of the ring kernel
+
 struct NormBwd {
   const void *dy, *h, *w, *dh;
   void* dx;
@@ -287,6 +291,100 @@ __global__ void __launch_bounds__(THREADS) rms_norm_backward_kernel(const NormBw
   }
 }
 
+// The same with the rows brought into shared memory by bulk copies, for rows on 16-byte boundaries
+// of up to 8192 columns: thread t holds columns 8t .. 8t + 7 of every row of its CTA, and a ring of
+// `slots` rows (h, dy and dh side by side) keeps the loads of the next rows in flight whatever the
+// registers hold.  At 16,384 x 4096 BF16 the register form moved 3.9 TB/s at its best shape.
+template <typename T>
+__global__ void __launch_bounds__(1024) rms_norm_backward_ring_kernel(const NormBwd a, const int slots) {
+  extern __shared__ __align__(128) uint8_t ring[];
+  __shared__ float2 slot_sum[2][32];
+  __shared__ __align__(8) uint64_t full[kRingMax];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
+  const uint32_t row_bytes = static_cast<uint32_t>(a.H * sizeof(T));
+  const int arrays = a.dh ? 3 : 2;
+  const T* h = static_cast<const T*>(a.h);
+  const T* dy = static_cast<const T*>(a.dy);
+  const T* dh = static_cast<const T*>(a.dh);
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < slots; ++i) mbar_init(&full[i], 1);
+    fence_mbarrier_init();
+  }
+  __syncthreads();
+  auto load_row = [&](int64_t row, int s) {  // by thread 0
+    uint8_t* at = ring + static_cast<size_t>(s) * arrays * row_bytes;
+    mbar_arrive_expect_tx(&full[s], arrays * row_bytes);
+    bulk_load(at, h + row * a.h_stride, row_bytes, &full[s]);
+    bulk_load(at + row_bytes, dy + row * a.dy_stride, row_bytes, &full[s]);
+    if (dh) bulk_load(at + 2 * row_bytes, dh + row * a.dh_stride, row_bytes, &full[s]);
+  };
+  const int64_t step = gridDim.x;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < slots; ++i)
+      if (blockIdx.x + i * step < a.T) load_row(blockIdx.x + i * step, i);
+  }
+  float w[8], acc[8] = {};
+  load_weight8<T, true>(a.w, a.w_f32, warp, lane, a.H, w);
+  const int64_t c = column<true>(warp, lane, 0);
+  const float inv = 1.0f / static_cast<float>(a.H);
+  int s = 0, turn = 0;
+  uint32_t phase = 0;
+  bool ok = true;
+  for (int64_t row = blockIdx.x; row < a.T; row += step, turn ^= 1) {
+    ok = mbar_wait_cta(&full[s], phase, nullptr, wait_code(1, 1, s, phase, static_cast<int>(row)));
+    const uint8_t* at = ring + static_cast<size_t>(s) * arrays * row_bytes + c * sizeof(T);
+    float hv[8] = {}, g[8] = {}, d[8] = {};
+    if (c < a.H) {
+      unpack8<T>(*reinterpret_cast<const Raw<T>*>(at), hv);
+      unpack8<T>(*reinterpret_cast<const Raw<T>*>(at + row_bytes), g);
+      if (dh) unpack8<T>(*reinterpret_cast<const Raw<T>*>(at + 2 * row_bytes), d);
+    }
+    float sq = 0.0f, uh = 0.0f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      sq = fmaf(hv[j], hv[j], sq);
+      uh = fmaf(g[j] * w[j], hv[j], uh);
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      sq += __shfl_xor_sync(0xffffffffu, sq, o);
+      uh += __shfl_xor_sync(0xffffffffu, uh, o);
+    }
+    if (lane == 0) slot_sum[turn][warp] = make_float2(sq, uh);
+    // also: every thread has taken its columns out of the slot; a wait that gave up ends the CTA
+    if (__syncthreads_or(!ok)) {
+      // copies issued before it still land: give them time before exit
+      const uint64_t t0 = global_timer_ns();
+      while (global_timer_ns() - t0 < 200000ull) __nanosleep(20000);
+      return;
+    }
+    if (threadIdx.x == 0 && row + slots * step < a.T) load_row(row + slots * step, s);
+    const float2 t = lane < warps ? slot_sum[turn][lane] : make_float2(0.0f, 0.0f);
+    sq = t.x;
+    uh = t.y;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      sq += __shfl_xor_sync(0xffffffffu, sq, o);
+      uh += __shfl_xor_sync(0xffffffffu, uh, o);
+    }
+    const float rstd = 1.0f / sqrtf(sq * inv + a.eps);
+    const float k = uh * inv * rstd * rstd;
+    float out[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      acc[j] = fmaf(g[j], hv[j] * rstd, acc[j]);
+      out[j] = fmaf(rstd, fmaf(-hv[j], k, g[j] * w[j]), d[j]);
+    }
+    store8<T, true>(static_cast<T*>(a.dx) + row * a.dx_stride, warp, lane, a.H, out);
+    if (++s == slots) { s = 0; phase ^= 1; }
+  }
+  if (c < a.H) {
+    float4* partial = reinterpret_cast<float4*>(a.partial + static_cast<int64_t>(blockIdx.x) * a.H + c);
+    partial[0] = make_float4(acc[0], acc[1], acc[2], acc[3]);
+    partial[1] = make_float4(acc[4], acc[5], acc[6], acc[7]);
+  }
+}
+
 }  // namespace
 
 // Row widths up to this one fit the registers of one CTA (32 warps of four 256-column chunks).
@@ -297,48 +395,73 @@ namespace {
 template <typename T, bool WIDE>
 int launch_norm(const NormFwd& a, cudaStream_t st) {
   const int chunks = static_cast<int>((a.H + 255) / 256);
-  // Rows of few tokens are spread over as many warps as they have chunks (latency); otherwise a
-  // warp holds four chunks, so that one barrier and one reduction serve more loads.
-  // Rows of more than 8192 columns take up to 32 warps, whose registers then hold four chunks
-  // with some spilling.
-  const int iter = chunks <= 32 && a.T <= 2 * sm_count() ? 1 : chunks >= 4 ? 4 : chunks >= 2 ? 2 : 1;
+  // Few rows are spread over as many warps as they have chunks (latency).  Otherwise a warp holds
+  // two chunks: 32,768 x 4096 BF16 with residual and codes takes 203 us so, 259 us with one (more
+  // warps wait at each row's barrier) and 236 us with four (100 registers a thread leave too few
+  // warps to cover the loads); 65,536 x 1024 takes 96 us, 118 us and 119 us.  Only rows of more
+  // than 16,384 columns need four, with some spilling.
+  const int iter = chunks <= 32 && a.T <= 2 * sm_count() ? 1 : chunks > 64 ? 4 : chunks >= 2 ? 2 : 1;
   const int warps = (chunks + iter - 1) / iter;
   const int rows = warps == 1 ? 4 : 1;  // rows per CTA
   const unsigned grid = static_cast<unsigned>((a.T + rows - 1) / rows);
-  auto kernel = iter == 1    ? add_rms_norm_kernel<T, WIDE, 1, 1024>
-                : iter == 2  ? add_rms_norm_kernel<T, WIDE, 2, 128>
-                : warps <= 8 ? add_rms_norm_kernel<T, WIDE, 4, 256>
-                             : add_rms_norm_kernel<T, WIDE, 4, 1024>;
+  auto kernel = iter == 1   ? add_rms_norm_kernel<T, WIDE, 1, 1024>
+                : iter == 2 ? add_rms_norm_kernel<T, WIDE, 2, 1024>
+                            : add_rms_norm_kernel<T, WIDE, 4, 1024>;
   kernel<<<grid, warps * rows * 32, 0, st>>>(a, warps);
   return launched();
 }
 
-// CTAs of the backward kernel: every SM filled, each CTA taking several rows where there are
+// CTAs of the backward kernels: every SM filled, each CTA taking several rows where there are
 // that many, because each writes one row of partial weight gradients.
 struct BwdShape {
-  int iter, warps, grid;
+  int warps, grid;
 };
 
-BwdShape backward_shape(int64_t T, int64_t H) {
+constexpr int64_t kRingMaxH = 8192;  // 1024 threads of eight columns
+
+int backward_warps(int64_t H) {
   const int chunks = static_cast<int>((H + 255) / 256);
+  return H <= kRingMaxH ? chunks : (chunks + 3) / 4;
+}
+
+BwdShape backward_shape(int64_t T, int64_t H) {
   BwdShape s;
-  s.iter = chunks <= 4 ? 1 : chunks <= 32 ? 2 : 4;
-  s.warps = (chunks + s.iter - 1) / s.iter;
-  const int per_sm = std::max(1, std::min(16, 16 / s.warps));
+  s.warps = backward_warps(H);
+  const int per_sm = std::max(1, std::min(16, 32 / s.warps));
   s.grid = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(T, int64_t(sm_count()) * per_sm)));
   return s;
 }
 
-template <typename T, bool WIDE>
-int launch_norm_backward(const NormBwd& a, const BwdShape& s, cudaStream_t st) {
-  auto kernel = s.iter == 1   ? rms_norm_backward_kernel<T, WIDE, 1, 128>
-                : s.iter == 2 ? rms_norm_backward_kernel<T, WIDE, 2, 512>
-                              : rms_norm_backward_kernel<T, WIDE, 4, 1024>;
-  kernel<<<s.grid, s.warps * 32, 0, st>>>(a);
+template <typename T>
+int launch_norm_backward(const NormBwd& a, const BwdShape& s, bool wide, cudaStream_t st) {
+  if (wide && a.H <= kRingMaxH) {
+    const int64_t row = a.H * static_cast<int64_t>(sizeof(T)) * (a.dh ? 3 : 2);
+    const int per_sm = std::max(1, std::min(16, 32 / s.warps));
+    const int slots = static_cast<int>(std::max<int64_t>(2, std::min<int64_t>(kRingMax, 200 * 1024 / per_sm / row)));
+    static std::once_flag flags[kMaxDevices];
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) return CDG_ERR_CUDA;
+    std::call_once(flags[dev], [] {
+      (void)cudaFuncSetAttribute(rms_norm_backward_ring_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                 200 * 1024);
+    });
+    rms_norm_backward_ring_kernel<T><<<s.grid, s.warps * 32, slots * row, st>>>(a, slots);
+    return launched();
+  }
+  if (a.H <= kRingMaxH)
+    rms_norm_backward_kernel<T, false, 1, 1024><<<s.grid, s.warps * 32, 0, st>>>(a);
+  else if (wide)
+    rms_norm_backward_kernel<T, true, 4, 1024><<<s.grid, s.warps * 32, 0, st>>>(a);
+  else
+    rms_norm_backward_kernel<T, false, 4, 1024><<<s.grid, s.warps * 32, 0, st>>>(a);
   return launched();
 }
 
 }  // namespace
+
+// This unit's record of waits that gave up (cdg_device_status reads it with the others').
+int norm_sticky_status(int clear, int32_t* out) { return read_sticky(g_sticky_status, clear, out); }
+
 }  // namespace cdg
 
 extern "C" {
@@ -389,19 +512,19 @@ int cdg_rms_norm_backward(const cdg_norm_backward_args* g, void* workspace, size
   const BwdShape s = backward_shape(g->T, g->H);
   int rc;
   if (g->dtype == CDG_DTYPE_BF16)
-    rc = wide ? launch_norm_backward<__nv_bfloat16, true>(a, s, st) : launch_norm_backward<__nv_bfloat16, false>(a, s, st);
+    rc = launch_norm_backward<__nv_bfloat16>(a, s, wide, st);
   else if (g->dtype == CDG_DTYPE_F16)
-    rc = wide ? launch_norm_backward<__half, true>(a, s, st) : launch_norm_backward<__half, false>(a, s, st);
+    rc = launch_norm_backward<__half>(a, s, wide, st);
   else
-    rc = wide ? launch_norm_backward<float, true>(a, s, st) : launch_norm_backward<float, false>(a, s, st);
+    rc = launch_norm_backward<float>(a, s, wide, st);
   if (rc != CDG_OK) return rc;
   const unsigned grid = static_cast<unsigned>((g->H + 31) / 32);
   if (g->w_dtype == CDG_DTYPE_BF16)
-    column_sum_kernel<__nv_bfloat16><<<grid, 256, 0, st>>>(a.partial, s.grid, g->H, static_cast<__nv_bfloat16*>(g->dw));
+    column_sum_kernel<__nv_bfloat16><<<grid, 1024, 0, st>>>(a.partial, s.grid, g->H, static_cast<__nv_bfloat16*>(g->dw));
   else if (g->w_dtype == CDG_DTYPE_F16)
-    column_sum_kernel<__half><<<grid, 256, 0, st>>>(a.partial, s.grid, g->H, static_cast<__half*>(g->dw));
+    column_sum_kernel<__half><<<grid, 1024, 0, st>>>(a.partial, s.grid, g->H, static_cast<__half*>(g->dw));
   else
-    column_sum_kernel<float><<<grid, 256, 0, st>>>(a.partial, s.grid, g->H, static_cast<float*>(g->dw));
+    column_sum_kernel<float><<<grid, 1024, 0, st>>>(a.partial, s.grid, g->H, static_cast<float*>(g->dw));
   return launched();
 }
 

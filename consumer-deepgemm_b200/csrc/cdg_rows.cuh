@@ -57,7 +57,7 @@ __device__ __forceinline__ int64_t column(int64_t chunk, int lane, int j) {
 
 // The lane's eight elements of a chunk as they lie in memory.
 template <typename T>
-struct Raw {
+struct alignas(16) Raw {
   static constexpr int kWords = static_cast<int>(sizeof(T)) * 2;
   uint32_t w[kWords];
 };
@@ -128,23 +128,26 @@ __device__ __forceinline__ void store8(T* row, int64_t chunk, int lane, int64_t 
   }
 }
 
-// out[c] = the sum of `parts` rows of partial column sums, in their order per thread and then over
-// the eight threads of a column: the same order every time.
+// out[c] = the sum of `parts` rows of partial column sums, every 32nd row per thread and then over
+// the 32 threads of a column: the same order every time.  1024 threads.
 template <typename W>
-__global__ void __launch_bounds__(256) column_sum_kernel(const float* partial, int parts, int64_t H, W* out) {
-  __shared__ float sums[8][33];
+__global__ void __launch_bounds__(1024) column_sum_kernel(const float* partial, int parts, int64_t H, W* out) {
+  __shared__ float sums[32][33];
   const int lane = threadIdx.x & 31, g = threadIdx.x >> 5;
   const int64_t c = static_cast<int64_t>(blockIdx.x) * 32 + lane;
   float v = 0.0f;
-  if (c < H)
-    for (int p = g; p < parts; p += 8) v += partial[static_cast<int64_t>(p) * H + c];
+  if (c < H) {
+#pragma unroll 4
+    for (int p = g; p < parts; p += 32) v += partial[static_cast<int64_t>(p) * H + c];
+  }
   sums[g][lane] = v;
   __syncthreads();
-  if (g == 0 && c < H) {
+  // warp g sums column g of the block
+  v = sums[lane][g];
 #pragma unroll
-    for (int i = 1; i < 8; ++i) v += sums[i][lane];
-    out[c] = from_f<W>(v);
-  }
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  const int64_t out_c = static_cast<int64_t>(blockIdx.x) * 32 + g;
+  if (lane == 0 && out_c < H) out[out_c] = from_f<W>(v);
 }
 
 // ------------------------------------------------------------------ host
@@ -156,6 +159,18 @@ inline int sm_count() {
   if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
     return 148;
   return n > 0 ? n : 148;
+}
+
+constexpr int kMaxDevices = 64;
+
+// Reads a unit's device-side error record (two words) into `out`, and clears it if asked.
+inline int read_sticky(const int (&record)[2], int clear, int32_t* out) {
+  if (cudaMemcpyFromSymbol(out, record, 2 * sizeof(int32_t)) != cudaSuccess) return CDG_ERR_CUDA;
+  if (clear && (out[0] || out[1])) {
+    const int32_t z[2] = {0, 0};
+    if (cudaMemcpyToSymbol(record, z, sizeof(z)) != cudaSuccess) return CDG_ERR_CUDA;
+  }
+  return CDG_OK;
 }
 
 inline int element_size(int dtype) { return dtype == CDG_DTYPE_F32 ? 4 : 2; }
