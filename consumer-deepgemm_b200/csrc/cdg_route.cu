@@ -13,8 +13,7 @@
 //   sigmoid: dl_i = (scatter(g)_i + (a_i - sum_j a_j p_j) / S) s_i (1 - s_i),  S = sum s
 //
 // A warp takes a row, lane l the experts l, l + 32, ...; a row is read once and its next row's
-// loads are in flight meanwhile.  Bound by instructions rather than memory: k rounds of a
-// warp-wide maximum per row.
+// loads are in flight meanwhile.  Bound by instructions rather than memory: the choice.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -34,15 +33,14 @@ constexpr int kRouteMaxTopk = 32;  // lane j keeps the row's j-th choice
 constexpr unsigned kAll = 0xffffffffu;
 
 // NaN counts as -inf (never chosen), +inf as the largest finite value, -0 as 0.
-__device__ __forceinline__ float clean_logit(float v) {
-  return v == v ? fminf(v, FLT_MAX) + 0.0f : -INFINITY;
-}
+__device__ __forceinline__ float clean_logit(float v) { return fminf(fmaxf(v, -INFINITY), FLT_MAX) + 0.0f; }
 
-// Keys whose unsigned order is the values' order; 0 stands for "cannot be chosen" (-inf).
+// Keys whose unsigned order is the values' order.  Keys below kFirstKey, that of -FLT_MAX, cannot
+// be chosen (-inf, and 0 for what was taken).
+constexpr uint32_t kFirstKey = 0x00800000u;
 __device__ __forceinline__ uint32_t order_key(float v) {
   const uint32_t b = __float_as_uint(v);
-  const uint32_t key = b ^ (b & 0x80000000u ? 0xFFFFFFFFu : 0x80000000u);
-  return v == -INFINITY ? 0u : key;
+  return b ^ (static_cast<uint32_t>(static_cast<int32_t>(b) >> 31) | 0x80000000u);
 }
 __device__ __forceinline__ float key_value(uint32_t key) {
   return __uint_as_float(key ^ (key & 0x80000000u ? 0x80000000u : 0xFFFFFFFFu));
@@ -57,6 +55,72 @@ __device__ __forceinline__ float warp_sum(float v) {
 // Fast exponential and division (errors of a few units in the last place): the gate's weights
 // and gradients stay within 1e-6 of the exact ones.
 __device__ __forceinline__ float sigmoid_fast(float v) { return __fdividef(1.0f, 1.0f + __expf(-v)); }
+
+// The k experts of the largest keys of a row, of equal keys the lowest first: lane j gets the j-th
+// (x its key, y the expert), or y = -1 where no key that can be chosen is left.  key[i] is that of
+// expert i * 32 + lane, mine the lane's largest.
+//
+// The k-th largest of the 32 lanes' maxima is a lower bound of the k-th largest key, and few keys
+// reach it (with 256 experts and k = 8 about ten), so: k rounds over the maxima alone give the
+// bound; the keys that reach it are listed in the order of their experts; each lane takes one of
+// the list and counts how many of the others go before it.  A list of more than 32 (many equal
+// keys, or k near 32) is chosen from round by round.  At 32,768 x 256, k = 8 the choice round by
+// round alone took the kernel 43 us.
+template <int N>
+__device__ __forceinline__ int2 choose(uint32_t (&key)[N], uint32_t mine, int k, int lane, uint2* list) {
+  uint32_t bound = 0;
+  uint32_t top = mine;
+  for (int j = 0; j < k; ++j) {
+    bound = __reduce_max_sync(kAll, top);
+    if (bound < kFirstKey) break;
+    if (lane == __ffs(__ballot_sync(kAll, top == bound)) - 1) top = 0;
+  }
+  bound = max(bound, kFirstKey);
+  int count = 0;
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const unsigned at = __ballot_sync(kAll, key[i] >= bound);
+    if (at == 0) continue;
+    const int place = count + __popc(at & ((1u << lane) - 1u));
+    if (key[i] >= bound && place < 32) list[place] = make_uint2(key[i], i * 32 + lane);
+    count += __popc(at);
+  }
+  int2 got = make_int2(0, -1);
+  if (count <= 32) {
+    __syncwarp();
+    const uint2 own = lane < count ? list[lane] : make_uint2(0, 0);
+    int before = 0;
+    for (int j = 0; j < count; ++j)  // of equal keys the one listed first, the lower expert, goes first
+      before += __shfl_sync(kAll, own.x, j) >= own.x + (j < lane ? 0u : 1u) ? 1 : 0;
+    __syncwarp();
+    if (lane < count && before < k) list[before] = own;
+    __syncwarp();
+    if (lane < min(count, k)) got = make_int2(static_cast<int>(list[lane].x), static_cast<int>(list[lane].y));
+    __syncwarp();
+    return got;
+  }
+  for (int j = 0; j < k; ++j) {
+    const uint32_t best = __reduce_max_sync(kAll, mine);
+    if (best < kFirstKey) break;
+    int e = 0x7fffffff;
+    if (mine == best) {
+#pragma unroll
+      for (int i = N - 1; i >= 0; --i)
+        if (key[i] == best) e = i * 32 + lane;
+    }
+    const int winner = static_cast<int>(__reduce_min_sync(kAll, static_cast<unsigned>(e)));
+    if (e == winner) {
+      mine = 0;
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        if (i * 32 + lane == winner) key[i] = 0;
+        mine = max(mine, key[i]);
+      }
+    }
+    if (lane == j) got = make_int2(static_cast<int>(best), winner);
+  }
+  return got;
+}
 
 struct Route {
   const void* logits;
@@ -81,27 +145,26 @@ struct Route {
 constexpr float kFixed = 1099511627776.0f;
 constexpr int64_t kRouteMaxTokens = int64_t(1) << 23;
 
-__device__ float balance_loss(const Route& a, int32_t tokens, const volatile unsigned long long* psum,
-                              const volatile int32_t* counts, double* scratch) {
-  double v = 0.0;
-  for (int e = threadIdx.x; e < a.E; e += blockDim.x)
-    v += static_cast<double>(counts[e]) * (static_cast<double>(psum[e]) / static_cast<double>(kFixed));
-  scratch[threadIdx.x] = v;
+// Sum of one value per thread, in a fixed order; thread 0 gets it.
+template <int WARPS>
+__device__ double cta_sum64(double v, double* scratch) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(kAll, v, o);
+  if ((threadIdx.x & 31) == 0) scratch[threadIdx.x >> 5] = v;
   __syncthreads();
-  for (int o = blockDim.x / 2; o > 0; o >>= 1) {
-    if (threadIdx.x < static_cast<unsigned>(o)) scratch[threadIdx.x] += scratch[threadIdx.x + o];
-    __syncthreads();
-  }
-  const double n = tokens > 0 ? tokens : 1;
-  return static_cast<float>(scratch[0] * a.E / a.k / n / n);
+  v = 0.0;
+  if (threadIdx.x == 0)
+    for (int i = 0; i < WARPS; ++i) v += scratch[i];
+  return v;
 }
 
 // N experts per lane.  Dynamic shared memory: E counts, then one row of E sums of p per warp.
 template <typename T, int N, int WARPS>
 __global__ void __launch_bounds__(WARPS * 32) moe_route_kernel(const Route a) {
   extern __shared__ int32_t route_smem[];
-  __shared__ double scratch[WARPS * 32];
+  __shared__ double scratch[WARPS];
   __shared__ int32_t s_tokens, s_last;
+  __shared__ uint2 s_list[WARPS][32];
   int32_t* s_counts = route_smem;
   float* s_psum = reinterpret_cast<float*>(route_smem + a.E);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -137,7 +200,7 @@ __global__ void __launch_bounds__(WARPS * 32) moe_route_kernel(const Route a) {
     top = __reduce_max_sync(kAll, top);
     int32_t id = -1;
     float w = 0.0f;
-    if (top != 0 && (!a.mask || a.mask[row])) {  // warp-uniform
+    if (top >= kFirstKey && (!a.mask || a.mask[row])) {  // warp-uniform
       const float m = a.sigmoid ? 0.0f : key_value(top);
       float inv = 1.0f;   // 1 / sum of exponentials (softmax)
       float part = 0.0f;  // 1 / sum of scores
@@ -154,45 +217,27 @@ __global__ void __launch_bounds__(WARPS * 32) moe_route_kernel(const Route a) {
         if (a.bias) {
 #pragma unroll
           for (int i = 0; i < N; ++i)
-            if (key[i] != 0) key[i] = order_key(clean_logit(v[i] * inv + __ldg(a.bias + i * 32 + lane)));
+            if (key[i] >= kFirstKey) key[i] = order_key(clean_logit(v[i] * inv + __ldg(a.bias + i * 32 + lane)));
         }
       }
-      // k rounds: the largest key, of equal ones the lowest expert
       uint32_t mine = 0;
 #pragma unroll
       for (int i = 0; i < N; ++i) mine = max(mine, key[i]);
-      const bool valid = __any_sync(kAll, mine != 0);  // a bias of -inf may have left nothing
+      const bool valid = __any_sync(kAll, mine >= kFirstKey);  // a bias of -inf may have left nothing
       if (valid) {
         ++tokens;
         if (a.balance) {
 #pragma unroll
           for (int i = 0; i < N; ++i) psum[i] = fmaf(v[i], part, psum[i]);
         }
-      }
-      for (int j = 0; j < a.k; ++j) {
-        const uint32_t best = __reduce_max_sync(kAll, mine);
-        if (best == 0) break;
-        int e = 0x7fffffff;
-        if (mine == best) {
-#pragma unroll
-          for (int i = N - 1; i >= 0; --i)
-            if (key[i] == best) e = i * 32 + lane;
+        const int2 got = choose<N>(key, mine, a.k, lane, s_list[warp]);
+        id = got.y;
+        if (id >= 0) {
+          // the key is that of the logit itself, unless a bias went into it
+          const float l = a.bias ? clean_logit(to_f(logits[row * a.stride + id])) : key_value(got.x);
+          w = a.sigmoid ? sigmoid_fast(l) : __expf(l - m) * inv;
+          atomicAdd(&s_counts[id], 1);
         }
-        const int winner = static_cast<int>(__reduce_min_sync(kAll, static_cast<unsigned>(e)));
-        if (e == winner) {
-          mine = 0;
-#pragma unroll
-          for (int i = 0; i < N; ++i) {
-            if (i * 32 + lane == winner) key[i] = 0;
-            mine = max(mine, key[i]);
-          }
-        }
-        if (lane == j) id = winner;
-      }
-      if (id >= 0) {
-        const float l = clean_logit(to_f(logits[row * a.stride + id]));
-        w = a.sigmoid ? sigmoid_fast(l) : __expf(l - m) * inv;
-        atomicAdd(&s_counts[id], 1);
       }
       if (a.renormalize) {
         const float total = warp_sum(w);
@@ -213,6 +258,24 @@ __global__ void __launch_bounds__(WARPS * 32) moe_route_kernel(const Route a) {
       if (i * 32 + lane < a.E) s_psum[warp * a.E + i * 32 + lane] = psum[i];
   }
   __syncthreads();
+  if (gridDim.x == 1) {  // one CTA saw every row
+    double sum = 0.0;
+    for (int e = threadIdx.x; e < a.E; e += blockDim.x) {
+      a.counts[e] = s_counts[e];
+      if (a.balance) {
+        double p = 0.0;
+        for (int i = 0; i < WARPS; ++i) p += s_psum[i * a.E + e];
+        sum += p * s_counts[e];
+      }
+    }
+    const double n = s_tokens > 0 ? s_tokens : 1;
+    if (a.balance) sum = cta_sum64<WARPS>(sum, scratch);
+    if (threadIdx.x == 0) {
+      *a.tokens = s_tokens;
+      if (a.balance) *a.loss = static_cast<float>(sum * a.E / a.k / n / n);
+    }
+    return;
+  }
   for (int e = threadIdx.x; e < a.E; e += blockDim.x) {
     if (s_counts[e]) atomicAdd(&a.acc_counts[e], s_counts[e]);
     if (a.balance) {
@@ -228,13 +291,18 @@ __global__ void __launch_bounds__(WARPS * 32) moe_route_kernel(const Route a) {
   __syncthreads();
   if (!s_last) return;
   __threadfence();
-  const volatile int32_t* counts = a.acc_counts;
-  for (int e = threadIdx.x; e < a.E; e += blockDim.x) a.counts[e] = counts[e];
-  const int32_t n = *static_cast<const volatile int32_t*>(a.acc_tokens);
-  if (threadIdx.x == 0) *a.tokens = n;
-  if (a.balance) {
-    const float loss = balance_loss(a, n, a.psum, counts, scratch);
-    if (threadIdx.x == 0) *a.loss = loss;
+  double sum = 0.0;
+  for (int e = threadIdx.x; e < a.E; e += blockDim.x) {
+    const int32_t count = __ldcg(a.acc_counts + e);
+    a.counts[e] = count;
+    if (a.balance) sum += static_cast<double>(count) * (static_cast<double>(__ldcg(a.psum + e)) / static_cast<double>(kFixed));
+  }
+  const int32_t tokens_all = __ldcg(a.acc_tokens);
+  if (a.balance) sum = cta_sum64<WARPS>(sum, scratch);
+  if (threadIdx.x == 0) {
+    const double n = tokens_all > 0 ? tokens_all : 1;
+    *a.tokens = tokens_all;
+    if (a.balance) *a.loss = static_cast<float>(sum * a.E / a.k / n / n);
   }
 }
 
@@ -359,14 +427,38 @@ __global__ void __launch_bounds__(WARPS * 32) moe_route_backward_kernel(const Ro
 }
 
 constexpr int kRouteWarps = 8;
+// Few tokens over few experts run in one CTA of 32 warps, which needs neither zeroed sums (a
+// memset before the kernel) nor a last CTA.
+constexpr int64_t kOneCtaTokens = 64;
+constexpr int kOneCtaExperts = 256;
+bool one_cta(int64_t T, int64_t E) { return T <= kOneCtaTokens && E <= kOneCtaExperts; }
 
-// CTAs per SM by registers: N experts per lane take about 4N registers of a thread.
-int route_ctas_per_sm(int n) { return n <= 8 ? 6 : n <= 16 ? 4 : 2; }
+// CTAs of a kernel that an SM holds at once (looked up once per device).
+template <typename K>
+int resident_ctas(K kernel, int threads, size_t smem, int* known) {
+  if (*known == 0) {
+    int n = 0;
+    if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kernel, threads, smem) != cudaSuccess || n < 1) n = 1;
+    *known = n;
+  }
+  return *known;
+}
 
 template <typename T, int N>
 int launch_route(const Route& a, cudaStream_t st) {
+  if constexpr (N * 32 <= kOneCtaExperts) {
+    if (one_cta(a.T, a.E)) {
+      const size_t smem = a.E * 4 + (a.balance ? size_t(32) * a.E * 4 : 0);
+      moe_route_kernel<T, N, 32><<<1, 1024, smem, st>>>(a);
+      return launched();
+    }
+  }
+  // the largest dynamic shared memory of this N, so that one look-up serves every call
+  static int known = 0;
+  const int per_sm = resident_ctas(moe_route_kernel<T, N, kRouteWarps>, kRouteWarps * 32,
+                                   size_t(N) * 32 * 4 * (kRouteWarps + 1), &known);
   const int64_t ctas = (a.T + kRouteWarps - 1) / kRouteWarps;
-  const unsigned grid = static_cast<unsigned>(std::min<int64_t>(ctas, int64_t(sm_count()) * route_ctas_per_sm(N)));
+  const unsigned grid = static_cast<unsigned>(std::min<int64_t>(ctas, int64_t(sm_count()) * per_sm));
   const size_t smem = a.E * 4 + (a.balance ? size_t(kRouteWarps) * a.E * 4 : 0);
   moe_route_kernel<T, N, kRouteWarps><<<grid, kRouteWarps * 32, smem, st>>>(a);
   return launched();
@@ -374,8 +466,11 @@ int launch_route(const Route& a, cudaStream_t st) {
 
 template <typename T, int N>
 int launch_route_backward(const RouteBwd& a, cudaStream_t st) {
+  static int known = 0;
+  const int per_sm = resident_ctas(moe_route_backward_kernel<T, N, kRouteWarps>, kRouteWarps * 32,
+                                   size_t(N) * 32 * 4 * kRouteWarps, &known);
   const int64_t ctas = (a.T + kRouteWarps - 1) / kRouteWarps;
-  const unsigned grid = static_cast<unsigned>(std::min<int64_t>(ctas, int64_t(sm_count()) * route_ctas_per_sm(N)));
+  const unsigned grid = static_cast<unsigned>(std::min<int64_t>(ctas, int64_t(sm_count()) * per_sm));
   moe_route_backward_kernel<T, N, kRouteWarps><<<grid, kRouteWarps * 32, size_t(kRouteWarps) * a.E * 4, st>>>(a);
   return launched();
 }
@@ -429,7 +524,9 @@ int cdg_moe_route(const cdg_route_args* g, void* workspace, size_t workspace_byt
       return CDG_ERR_CUDA;
     return CDG_OK;
   }
-  if (cudaMemsetAsync(workspace, 0, cdg_moe_route_workspace_bytes(g->E), st) != cudaSuccess) return CDG_ERR_CUDA;
+  if (!one_cta(g->T, g->E) &&
+      cudaMemsetAsync(workspace, 0, cdg_moe_route_workspace_bytes(g->E), st) != cudaSuccess)
+    return CDG_ERR_CUDA;
   Route a{};
   a.logits = g->logits;
   a.stride = g->stride;
