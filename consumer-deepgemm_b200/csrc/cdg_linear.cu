@@ -93,9 +93,10 @@ __global__ void __launch_bounds__(256) linear_dz_kernel(const T* dy, int64_t dy_
 }
 
 // ------------------------------------------------------------------ host
-template <typename T, typename O, int BN, bool PROMOTE>
+template <typename T, typename O, int BN, bool SWAP>
 bool allow_smem() {
-  return cudaFuncSetAttribute(cdg_linear_tile_kernel<T, O, BN, PROMOTE>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+  constexpr bool PROMOTE = sizeof(O) == 4;
+  return cudaFuncSetAttribute(cdg_linear_tile_kernel<T, O, BN, PROMOTE, SWAP>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                               TileSmem<BN, PROMOTE>::kBytes) == cudaSuccess;
 }
 
@@ -105,10 +106,15 @@ bool allow_pair_smem() {
                               PairTileSmem<BN>::kBytes) == cudaSuccess;
 }
 
+template <typename T, typename O>
+bool allow_smem_for() {
+  return allow_pair_smem<T, O, 256>() && allow_smem<T, O, 64, false>() && allow_smem<T, O, 128, false>() &&
+         allow_smem<T, O, 16, true>() && allow_smem<T, O, 32, true>() && allow_smem<T, O, 64, true>();
+}
+
 template <typename T>
 bool allow_smem_of() {
-  return allow_pair_smem<T, T, 256>() && allow_pair_smem<T, float, 128>() && allow_smem<T, T, 64, false>() && allow_smem<T, T, 128, false>() && allow_smem<T, float, 64, true>() &&
-         allow_smem<T, float, 128, true>();
+  return allow_smem_for<T, T>() && allow_smem_for<T, float>();
 }
 
 // Compute capability and kernel attributes, once per device.
@@ -180,9 +186,10 @@ int make_map(CUtensorMap* map, const Matrix& m, int dtype, uint32_t box_rows) {
              : CDG_ERR_CUDA;
 }
 
-template <typename T, typename O, int BN, bool PROMOTE>
+template <typename T, typename O, int BN, bool SWAP>
 int launch_tiles(const CUtensorMap& ta, const CUtensorMap& tb, const LinearShape& s, const Epilogue& e, int splits,
                  cudaStream_t st) {
+  constexpr bool PROMOTE = sizeof(O) == 4;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(static_cast<unsigned>(s.m_tiles) * s.n_tiles * splits);
   cfg.blockDim = dim3(kTileThreads);
@@ -194,7 +201,7 @@ int launch_tiles(const CUtensorMap& ta, const CUtensorMap& tb, const LinearShape
   at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
   cfg.attrs = at;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, cdg_linear_tile_kernel<T, O, BN, PROMOTE>, ta, tb, s, e, splits) == cudaSuccess
+  return cudaLaunchKernelEx(&cfg, cdg_linear_tile_kernel<T, O, BN, PROMOTE, SWAP>, ta, tb, s, e, splits) == cudaSuccess
              ? CDG_OK
              : CDG_ERR_CUDA;
 }
@@ -210,7 +217,8 @@ int launch_pairs(const Matrix& A, const Matrix& B, const LinearShape& s, Epilogu
   // a box of y or of the residual is one warp's 32 rows x 128 bytes
   const Matrix y{e.y, e.y_stride, M, N}, r{e.residual, e.residual_stride, M, N};
   const bool apart = M == 1 || (y.stride >= N && (!e.residual || r.stride >= N));
-  e.staged = e.wide && !e.z && apart && (!e.residual || (e.residual_f32 != 0) == (sizeof(O) == 4));
+  // (FP32 results have four chunks a warp and tile, and no staged residual)
+  e.staged = e.wide && !e.z && apart && (!e.residual || (sizeof(O) == 2 && !e.residual_f32));
   if (rc == CDG_OK && e.staged) rc = make_map(&ty, y, kOut, 32);
   if (rc == CDG_OK && e.staged && e.residual) rc = make_map(&tr, r, kOut, 32);
   if (rc != CDG_OK) return rc;
@@ -221,12 +229,60 @@ int launch_pairs(const Matrix& A, const Matrix& B, const LinearShape& s, Epilogu
   return launched();
 }
 
+// How a product is cut.  The costs are cycles of an SM, fitted to measured times (in microseconds,
+// one B200 at 1.9 GHz):
+//   pairs  a wave of 256 x 256 tiles takes about 530 cycles per K step (the tensor cores' 512) and
+//          1500 more; 5000 to start and to drain.
+//   tiles  of 128 x 128 take about 620 cycles per K step alone on an SM and 1170 two at a time, of
+//          128 x 64 about 400 and 770.
+struct Plan {
+  enum Kind { kPairs, kTiles, kSwapped } kind;
+  int bn, splits;
+};
+
+Plan make_plan(int64_t M, int64_t N, int64_t k_steps, int sms) {
+  Plan p{Plan::kTiles, 64, 1};
+  // K is split while there are CTAs to spare (two per SM) and each part keeps four K steps
+  auto split = [&](int64_t tiles) {
+    int s = 1;
+    while (s < 8 && tiles * s * 2 <= 2 * sms && k_steps / (s * 2) >= 4) s *= 2;
+    return s;
+  };
+  if (M <= 64) {
+    p.kind = Plan::kSwapped;
+    p.bn = M <= 16 ? 16 : M <= 32 ? 32 : 64;
+    p.splits = split((N + 127) / 128);
+    return p;
+  }
+  auto tile_cost = [&](int bn, int s) {
+    const int64_t ctas = (M + 127) / 128 * ((N + bn - 1) / bn) * s;
+    const double alone = bn == 128 ? 620 : 400, two = bn == 128 ? 1170 : 770;
+    const double steps = static_cast<double>((k_steps + s - 1) / s);
+    if (ctas <= sms) return steps * alone + 6000 + (s > 1 ? 2000 : 0);
+    return static_cast<double>((ctas + 2 * sms - 1) / (2 * sms)) * (steps * two + 3000) + 3000 + (s > 1 ? 2000 : 0);
+  };
+  double best = 1e300;
+  for (int bn : {64, 128}) {
+    const int s = split((M + 127) / 128 * ((N + bn - 1) / bn));
+    const double c = tile_cost(bn, s);
+    if (c < best) {
+      best = c;
+      p.bn = bn;
+      p.splits = s;
+    }
+  }
+  const int64_t pairs = std::max(1, sms / 2), pair_tiles = (M + 255) / 256 * ((N + 255) / 256);
+  if (k_steps > 0 &&
+      static_cast<double>((pair_tiles + pairs - 1) / pairs) * (static_cast<double>(k_steps) * 530 + 1500) + 5000 < best)
+    p.kind = Plan::kPairs;
+  return p;
+}
+
 // D [M, N] = epilogue(sum over K of A and B); a_mn: A lies as [K, M], else [M, K]; b_mn: B lies as
 // [K, N], else [N, K].  Rows of both on 16-byte boundaries.
 template <typename T, typename O>
 int product(const Matrix& A, bool a_mn, const Matrix& B, bool b_mn, int64_t M, int64_t N, int64_t K,
             const Epilogue& e, cudaStream_t st) {
-  constexpr bool kPromote = sizeof(O) == 4;
   constexpr int kType = std::is_same<T, __nv_bfloat16>::value ? CDG_DTYPE_BF16 : CDG_DTYPE_F16;
   if (M == 0 || N == 0) return CDG_OK;
   LinearShape s{};
@@ -237,31 +293,40 @@ int product(const Matrix& A, bool a_mn, const Matrix& B, bool b_mn, int64_t M, i
   s.b_mn = b_mn;
   s.bf16 = kType == CDG_DTYPE_BF16;
   s.a_rows = static_cast<int>(std::min<int64_t>(128, (M + 7) / 8 * 8));
-  const int sms = sm_count();
-  constexpr int kPairN = kPromote ? 128 : 256;
-  const int64_t pair_tiles = ((M + 255) / 256) * ((N + kPairN - 1) / kPairN);
-  if (K > 0 && pair_tiles >= sms / 2 && pair_tiles < (int64_t(1) << 30)) {
-    s.m_tiles = static_cast<int>((M + 255) / 256);
-    s.n_tiles = static_cast<int>((N + kPairN - 1) / kPairN);
-    return launch_pairs<T, O, kPairN>(A, B, s, e, M, N, st);
+  Plan p = make_plan(M, N, s.k_steps, sm_count());
+  if (p.kind == Plan::kSwapped && a_mn) {  // x's place is loaded in boxes of 16 to 64 rows, K-major
+    p.kind = Plan::kTiles;
+    p.bn = 64;
   }
-  const int64_t m_tiles = (M + 127) / 128;
-  const int bn = m_tiles * ((N + 127) / 128) >= sms ? 128 : 64;
-  const int64_t n_tiles = (N + bn - 1) / bn;
+  const int64_t tm = p.kind == Plan::kPairs ? 256 : 128, tn = p.kind == Plan::kPairs ? 256 : p.bn;
+  const int64_t rows = p.kind == Plan::kSwapped ? N : M, cols = p.kind == Plan::kSwapped ? M : N;
+  const int64_t m_tiles = (rows + tm - 1) / tm, n_tiles = (cols + tn - 1) / tn;
   if (m_tiles * n_tiles * 8 > 0x7fffffff) return CDG_ERR_UNSUPPORTED;
   s.m_tiles = static_cast<int>(m_tiles);
   s.n_tiles = static_cast<int>(n_tiles);
-  // K is split while the tiles leave SMs without work and each part keeps four K steps
-  int splits = 1;
-  while (splits < 8 && m_tiles * n_tiles * splits * 2 <= 2 * sms && s.k_steps / (splits * 2) >= 4) splits *= 2;
+  if (p.kind == Plan::kPairs) return launch_pairs<T, O, 256>(A, B, s, e, M, N, st);
   CUtensorMap ta{}, tb{};
+  if (p.kind == Plan::kSwapped) {
+    std::swap(s.M, s.N);
+    s.a_mn = b_mn;
+    s.b_mn = 0;
+    s.a_rows = static_cast<int>(std::min<int64_t>(128, (s.M + 7) / 8 * 8));
+    if (K > 0) {
+      int rc = make_map(&ta, B, kType, b_mn ? 64 : s.a_rows);
+      if (rc == CDG_OK) rc = make_map(&tb, A, kType, p.bn);
+      if (rc != CDG_OK) return rc;
+    }
+    return p.bn == 16   ? launch_tiles<T, O, 16, true>(ta, tb, s, e, p.splits, st)
+           : p.bn == 32 ? launch_tiles<T, O, 32, true>(ta, tb, s, e, p.splits, st)
+                        : launch_tiles<T, O, 64, true>(ta, tb, s, e, p.splits, st);
+  }
   if (K > 0) {
     int rc = make_map(&ta, A, kType, a_mn ? 64 : s.a_rows);
-    if (rc == CDG_OK) rc = make_map(&tb, B, kType, b_mn ? 64 : bn);
+    if (rc == CDG_OK) rc = make_map(&tb, B, kType, b_mn ? 64 : p.bn);
     if (rc != CDG_OK) return rc;
   }
-  return bn == 128 ? launch_tiles<T, O, 128, kPromote>(ta, tb, s, e, splits, st)
-                   : launch_tiles<T, O, 64, kPromote>(ta, tb, s, e, splits, st);
+  return p.bn == 128 ? launch_tiles<T, O, 128, false>(ta, tb, s, e, p.splits, st)
+                     : launch_tiles<T, O, 64, false>(ta, tb, s, e, p.splits, st);
 }
 
 bool operand_dtype(int dtype) { return dtype == CDG_DTYPE_BF16 || dtype == CDG_DTYPE_F16; }

@@ -51,6 +51,9 @@ __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&r)[32]) {
       : "r"(taddr));
 }
 
+__device__ __forceinline__ void tmem_ld(uint32_t taddr, uint32_t (&r)[32]) { tmem_ld32(taddr, r); }
+__device__ __forceinline__ void tmem_ld(uint32_t taddr, uint32_t (&r)[16]) { tmem_ld16(taddr, r); }
+
 // Operand tiles of one K step (64 columns of K) in shared memory, 128-byte swizzle:
 //   K-major:  [rows][64 k], 8-row groups 1024 bytes apart;
 //   MN-major: chunks of 64 rows, each [64 k][64 rows] (8192 bytes); the 8-k groups of a chunk
@@ -187,6 +190,43 @@ __device__ __forceinline__ void finish8(const Epilogue& e, int64_t m, int64_t n,
   }
 }
 
+// One element.
+template <typename T, typename O>
+__device__ __forceinline__ void finish1(const Epilogue& e, int64_t m, int64_t n, float v) {
+  if (e.bias) v += load_any<T>(e.bias, n, e.bias_f32);
+  if (e.z) static_cast<T*>(e.z)[m * e.z_stride + n] = from_f<T>(v);
+  v = activate(v, e.act);
+  if (e.residual) v += load_any<T>(e.residual, m * e.residual_stride + n, e.residual_f32);
+  static_cast<O*>(e.y)[m * e.y_stride + n] = from_f<O>(v);
+}
+
+// 32 rows x 32 columns of a warp, lane = row, turned in shared memory (32 x 33 floats of the warp's
+// own) so that the lanes load and store along the rows: four lanes with eight columns each per
+// row, or, where rows do not start on 16-byte boundaries, one column per lane.
+template <typename T, typename O>
+__device__ __forceinline__ void finish_turned(const Epilogue& e, int64_t m0, int64_t M, int64_t n0, int64_t N,
+                                              const float (&v)[32], float* turn, int lane) {
+  __syncwarp();
+#pragma unroll
+  for (int j = 0; j < 32; ++j) turn[lane * 33 + j] = v[j];
+  __syncwarp();
+  if (e.wide) {
+    const int64_t n = n0 + (lane & 3) * 8;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int row = i * 8 + (lane >> 2);
+      float w[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) w[j] = turn[row * 33 + (lane & 3) * 8 + j];
+      if (m0 + row < M && n < N) finish8<T, O>(e, m0 + row, n, N, w);
+    }
+  } else {
+    const int rows = static_cast<int>(M - m0 < 32 ? M - m0 : 32);
+    if (n0 + lane < N)
+      for (int row = 0; row < rows; ++row) finish1<T, O>(e, m0 + row, n0 + lane, turn[row * 33 + lane]);
+  }
+}
+
 struct LinearShape {
   int64_t M, N;
   int k_steps;         // of 64 columns of K
@@ -203,13 +243,16 @@ struct LinearShape {
 // PROMOTE (32-bit outputs): the tensor core's running sum loses about one part in 2^20 over a
 // few thousand terms (its additions truncate), which 16-bit outputs do not see; here a sum
 // covers 512 of K at most, and FP32 registers add those up.
+// SWAP (few rows of x): A is the weight and B is x, so that 128 rows of the weight meet 16, 32 or 64
+// rows of x without tiles that are mostly padding; the epilogue's roles of rows and columns change
+// places with them (M and N here are those of the swapped product).
 // Warps: 0-3 epilogue (one per TMEM lane quadrant), 4 TMA producer, 5 MMA issuer and TMEM owner.
 template <int BN, bool PROMOTE>
 struct TileSmem {
   static constexpr int kA = 128 * 128;
   static constexpr int kB = BN * 128;
   static constexpr int kStageBytes = kA + kB;
-  static constexpr int kStages = BN >= 128 ? 3 : 4;
+  static constexpr int kStages = BN >= 128 ? 3 : BN == 64 ? 4 : BN == 32 ? 5 : 6;
   static constexpr int kBars = kStages * kStageBytes;  // full, empty [kStages]; tfull, tempty [2]; TMEM address
   static constexpr int kBytes = kBars + (2 * kStages + 4) * 8 + 16 + 1024;
   static constexpr int kAccs = PROMOTE ? 2 : 1;
@@ -221,12 +264,13 @@ struct TileSmem {
 constexpr int kTileThreads = 192;
 constexpr int kPromoteSteps = 8;  // K steps of 64 per running sum
 
-template <typename T, typename O, int BN, bool PROMOTE>
+template <typename T, typename O, int BN, bool PROMOTE, bool SWAP>
 __global__ void __launch_bounds__(kTileThreads)
     cdg_linear_tile_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_b,
                            const LinearShape s, const Epilogue e, const int splits) {
   using L = TileSmem<BN, PROMOTE>;
   constexpr int S = L::kStages;
+  constexpr int CC = BN < 32 ? BN : 32;  // columns taken out of TMEM at a time
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + L::kBars);
@@ -287,7 +331,8 @@ __global__ void __launch_bounds__(kTileThreads)
         }
         if (s.b_mn) {
 #pragma unroll
-          for (int c = 0; c < BN / 64; ++c) tma_load_2d(b + c * 8192, &tmap_b, &full[stage], n0 + c * 64, k * 64);
+          for (int c = 0; c < (BN + 63) / 64; ++c)
+            tma_load_2d(b + c * 8192, &tmap_b, &full[stage], n0 + c * 64, k * 64);  // BN of 64 or 128 alone
         } else {
           tma_load_2d(b, &tmap_b, &full[stage], k * 64, n0);
         }
@@ -341,12 +386,12 @@ __global__ void __launch_bounds__(kTileThreads)
         }
         tc_fence_after();
 #pragma unroll
-        for (int c = 0; c < BN / 32; ++c) {
-          uint32_t r[32];
-          tmem_ld32(lanes + buf * BN + c * 32, r);
+        for (int c = 0; c < BN / CC; ++c) {
+          uint32_t r[CC];
+          tmem_ld(lanes + buf * BN + c * CC, r);
           tmem_ld_wait();
 #pragma unroll
-          for (int j = 0; j < 32; ++j) acc[c * 32 + j] += __uint_as_float(r[j]);
+          for (int j = 0; j < CC; ++j) acc[c * CC + j] += __uint_as_float(r[j]);
         }
         tc_fence_before();
         mbar_arrive(&tempty[buf]);
@@ -357,31 +402,30 @@ __global__ void __launch_bounds__(kTileThreads)
     }
     if (ok) {
 #pragma unroll
-      for (int c = 0; c < BN / 32; ++c) {
-        float v[32];
+      for (int c = 0; c < BN / CC; ++c) {
+        float v[CC];
         if constexpr (PROMOTE) {
 #pragma unroll
-          for (int j = 0; j < 32; ++j) v[j] = acc[c * 32 + j];
+          for (int j = 0; j < CC; ++j) v[j] = acc[c * CC + j];
         } else {
-          uint32_t r[32];
-          tmem_ld32(lanes + c * 32, r);
+          uint32_t r[CC];
+          tmem_ld(lanes + c * CC, r);
           tmem_ld_wait();
 #pragma unroll
-          for (int j = 0; j < 32; ++j) v[j] = sums ? __uint_as_float(r[j]) : 0.0f;  // K = 0: nothing was summed
+          for (int j = 0; j < CC; ++j) v[j] = sums ? __uint_as_float(r[j]) : 0.0f;  // K = 0: nothing was summed
         }
+        // every product of this CTA has completed, so the stages are free
         if (splits > 1) {
-          // every product of this CTA has completed, so the stages are free
 #pragma unroll
-          for (int j = 0; j < 32; ++j) part[(c * 32 + j) * 128 + warp * 32 + lane] = v[j];
-        } else if (m < s.M) {
+          for (int j = 0; j < CC; ++j) part[(c * CC + j) * 128 + warp * 32 + lane] = v[j];
+        } else if constexpr (SWAP) {
+          if (m < s.M) {
 #pragma unroll
-          for (int g = 0; g < 4; ++g) {
-            float w[8];
-#pragma unroll
-            for (int j = 0; j < 8; ++j) w[j] = v[g * 8 + j];
-            const int64_t n = n0 + c * 32 + g * 8;
-            if (n < s.N) finish8<T, O>(e, m, n, s.N, w);
+            for (int j = 0; j < CC; ++j)
+              if (n0 + c * CC + j < s.N) finish1<T, O>(e, n0 + c * CC + j, m, v[j]);
           }
+        } else if (m0 + warp * 32 < s.M && n0 + c * CC < s.N) {
+          finish_turned<T, O>(e, m0 + warp * 32, s.M, n0 + c * CC, s.N, v, part + warp * 32 * 33, lane);
         }
       }
     }
@@ -392,22 +436,39 @@ __global__ void __launch_bounds__(kTileThreads)
     // and the device record says so)
     cluster_sync();
     const float* part = reinterpret_cast<const float*>(smem);
-    for (int item = threadIdx.x; item < 128 * (BN / 8); item += kTileThreads) {
-      const int group = item / 128, row = item % 128;
-      if (group % splits != split) continue;
-      const int64_t m = m0 + row, n = n0 + group * 8;
-      if (m >= s.M || n >= s.N) continue;
-      float v[8] = {};
-      for (int r = 0; r < splits; ++r) {
-        const uint32_t at = cluster_addr(part + group * 8 * 128 + row, r);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
+    if constexpr (SWAP) {
+      // this CTA finishes 128 / splits rows (of the weight), all columns; rows run along y's rows
+      const int share = 128 / splits;
+      for (int item = threadIdx.x; item < share * BN; item += kTileThreads) {
+        const int col = item / share, row = split * share + item % share;
+        const int64_t m = m0 + row, n = n0 + col;
+        if (m >= s.M || n >= s.N) continue;
+        float v = 0.0f;
+        for (int r = 0; r < splits; ++r) {
           float f;
-          asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(f) : "r"(at + j * 512));
-          v[j] += f;
+          asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(f) : "r"(cluster_addr(part + col * 128 + row, r)));
+          v += f;
         }
+        finish1<T, O>(e, n, m, v);
       }
-      finish8<T, O>(e, m, n, s.N, v);
+    } else {
+      for (int item = threadIdx.x; item < 128 * (BN / 8); item += kTileThreads) {
+        const int group = item / 128, row = item % 128;
+        if (group % splits != split) continue;
+        const int64_t m = m0 + row, n = n0 + group * 8;
+        if (m >= s.M || n >= s.N) continue;
+        float v[8] = {};
+        for (int r = 0; r < splits; ++r) {
+          const uint32_t at = cluster_addr(part + group * 8 * 128 + row, r);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            float f;
+            asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(f) : "r"(at + j * 512));
+            v[j] += f;
+          }
+        }
+        finish8<T, O>(e, m, n, s.N, v);
+      }
     }
     cluster_sync();  // no CTA leaves while another reads its shared memory
   }
@@ -424,7 +485,7 @@ __global__ void __launch_bounds__(kTileThreads)
 }
 
 // ---------------------------------------------------------------- CTA pairs, persistent, for many tiles
-// A pair of CTAs takes tiles of 256 x BN in turn: CTA r of it holds rows 128r .. 128r + 127 of A and
+// A pair of CTAs takes tiles of 256 x BN (256) in turn: CTA r of it holds rows 128r .. 128r + 127 of A and
 // of the result and half of B's rows.  The tensor cores fill one of two accumulators in TMEM while
 // eight epilogue warps per CTA empty the other (warp w: the 32 lanes of quadrant w % 4, half of the
 // columns).  Staged (y, and the residual where there is one, of the output's type and on 16-byte
@@ -438,7 +499,7 @@ struct PairTileSmem {
   static constexpr int kA = 128 * 128;
   static constexpr int kB = BN / 2 * 128;
   static constexpr int kStageBytes = kA + kB;
-  static constexpr int kStages = BN == 256 ? 5 : 6;
+  static constexpr int kStages = 5;
   static constexpr int kEpiWarps = 8;
   static constexpr int kStaging = kStages * kStageBytes;      // [warp][2] tiles of 4096 bytes
   static constexpr int kBars = kStaging + kEpiWarps * 2 * 4096;
@@ -468,6 +529,7 @@ __device__ __forceinline__ void tma_store_2d(const void* tmap, const void* src, 
 __device__ __forceinline__ void bulk_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
 // The stores issued by this thread have read their shared memory / have completed.
 __device__ __forceinline__ void bulk_wait_read() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
+__device__ __forceinline__ void bulk_wait_read_but_one() { asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory"); }
 __device__ __forceinline__ void bulk_wait_all() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
 
 // Tile t of a grid of m_tiles x n_tiles: bands of kBand row tiles, column by column, so that the
@@ -561,8 +623,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairTileSmem<BN>::kT
   constexpr bool PROMOTE = sizeof(O) == 4;
   constexpr int S = L::kStages;
   constexpr int CH = 128 / static_cast<int>(sizeof(O));  // columns of a staged tile
-  constexpr int kChunks = BN / 2 / CH;                   // staged tiles of a warp per output tile
-  static_assert(kChunks == 2, "two staged tiles per warp");
+  constexpr int kChunks = BN / 2 / CH;                   // staged tiles of a warp per output tile (2 or 4)
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + L::kBars);
@@ -681,7 +742,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairTileSmem<BN>::kT
     uint8_t* stagings = smem + L::kStaging + w * 2 * 4096;
     const uint32_t lanes = tmem + (static_cast<uint32_t>(q * 32) << 16) + half * (BN / 2);
     int sum = 0;
-    uint32_t turn[kChunks] = {};  // phase of each staged tile's residual barrier
+    uint32_t turn[2] = {};  // phase of each staged tile's residual barrier
     for (int t = pair; t < tiles && ok; t += pairs) {
       int mt, nt;
       tile_at(t, s.m_tiles, s.n_tiles, mt, nt);
@@ -690,9 +751,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairTileSmem<BN>::kT
       if (e.staged && any) {
         if (lane == 0) {
           bulk_wait_read();  // the last tile's stores have read the staged tiles
-          if (e.residual) {
+          if (e.residual) {  // with 16-bit results alone, where a warp has two chunks
 #pragma unroll
-            for (int c = 0; c < kChunks; ++c) {
+            for (int c = 0; c < 2; ++c) {
               if (col0 + c * CH < s.N) {
                 mbar_arrive_expect_tx(&rfull[w * 2 + c], 4096);
                 tma_load_2d(stagings + c * 4096, &tmap_r, &rfull[w * 2 + c], col0 + c * CH, row0);
@@ -714,12 +775,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairTileSmem<BN>::kT
           }
           tc_fence_after();
 #pragma unroll
-          for (int c = 0; c < BN / 64; ++c) {
-            uint32_t r[32];
-            tmem_ld32(lanes + buf * BN + c * 32, r);
+          for (int c = 0; c < BN / 32; ++c) {  // 16 at a time: the sums take most of the registers
+            uint32_t r[16];
+            tmem_ld16(lanes + buf * BN + c * 16, r);
             tmem_ld_wait();
 #pragma unroll
-            for (int j = 0; j < 32; ++j) acc[c * 32 + j] += __uint_as_float(r[j]);
+            for (int j = 0; j < 16; ++j) acc[c * 16 + j] += __uint_as_float(r[j]);
           }
           tc_fence_before();
           if (rank == 0) mbar_arrive(&tempty[buf]); else mbar_arrive_cluster(tempty0 + buf * 8);
@@ -756,24 +817,31 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairTileSmem<BN>::kT
         }
         if (!any || n >= s.N) continue;
         if (e.staged) {
+          uint8_t* tile = stagings + (c & 1) * 4096;
           if (e.residual) {
-            if (!mbar_wait_cta_warp(&rfull[w * 2 + c], turn[c], nullptr, wait_code(4, 8 + w, c, turn[c], 0))) ok = false;
-            turn[c] ^= 1;
+            if (!mbar_wait_cta_warp(&rfull[w * 2 + (c & 1)], turn[c & 1], nullptr, wait_code(4, 8 + w, c, turn[c & 1], 0)))
+              ok = false;
+            turn[c & 1] ^= 1;
           }
-          finish_staged<T, O, CH>(e, n, s.N, v, stagings + c * 4096, lane);
+          if (c >= 2) {  // the store of two chunks ago has read the tile
+            if (lane == 0) bulk_wait_read_but_one();
+            __syncwarp();
+          }
+          finish_staged<T, O, CH>(e, n, s.N, v, tile, lane);
           fence_proxy_async_shared();
           __syncwarp();
           if (lane == 0) {
-            tma_store_2d(&tmap_y, stagings + c * 4096, n, row0);
+            tma_store_2d(&tmap_y, tile, n, row0);
             bulk_commit();
           }
-        } else if (row0 + lane < s.M) {
+        } else {
 #pragma unroll
-          for (int g = 0; g < CH / 8; ++g) {
-            float u[8];
+          for (int g = 0; g < CH / 32; ++g) {
+            float u[32];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) u[j] = v[g * 8 + j];
-            if (n + g * 8 < s.N) finish8<T, O>(e, row0 + lane, n + g * 8, s.N, u);
+            for (int j = 0; j < 32; ++j) u[j] = v[g * 32 + j];
+            if (n + g * 32 < s.N)
+              finish_turned<T, O>(e, row0, s.M, n + g * 32, s.N, u, reinterpret_cast<float*>(stagings), lane);
           }
         }
       }
