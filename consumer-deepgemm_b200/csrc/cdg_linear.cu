@@ -37,21 +37,39 @@ EncodeTiledFn encode_tiled() {
   return fn;
 }
 
-// Copies rows of 16-bit values to rows of `out_stride` columns, zeros past `cols`.
-__global__ void __launch_bounds__(256) repack_rows_kernel(const uint16_t* in, int64_t in_stride, int64_t rows,
-                                                          int64_t cols, uint16_t* out, int64_t out_stride) {
-  const int64_t words = out_stride / 8, total = rows * words;
-  for (int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; i < total;
-       i += static_cast<int64_t>(gridDim.x) * blockDim.x) {
-    const int64_t r = i / words, c = (i - r * words) * 8;
-    const uint16_t* p = in + r * in_stride + c;
-    uint32_t w[4];
+// Copies rows of 16-bit values to rows of `out_stride` columns, zeros past `cols`; one or two
+// matrices (blockIdx.y).
+struct Repack {
+  const uint16_t* in;
+  int64_t in_stride, rows, cols;
+  uint16_t* out;
+  int64_t out_stride;
+};
+
+__global__ void __launch_bounds__(256) repack_rows_kernel(const Repack first, const Repack second) {
+  const Repack p = blockIdx.y == 0 ? first : second;
+  const int lane = threadIdx.x & 31;
+  // whole words where every row starts on a 4-byte boundary
+  const bool even = p.in_stride % 2 == 0 && reinterpret_cast<uintptr_t>(p.in) % 4 == 0;
+  for (int64_t r = (static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x) >> 5; r < p.rows;
+       r += (static_cast<int64_t>(gridDim.x) * blockDim.x) >> 5) {
+    const uint16_t* from = p.in + r * p.in_stride;
+    uint16_t* to = p.out + r * p.out_stride;
+#pragma unroll 4
+    for (int64_t c = lane * 8; c < p.out_stride; c += 256) {
+      uint32_t w[4];
+      if (even && c + 8 <= p.cols) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const uint32_t lo = c + 2 * j < cols ? p[2 * j] : 0, hi = c + 2 * j + 1 < cols ? p[2 * j + 1] : 0;
-      w[j] = lo | (hi << 16);
+        for (int j = 0; j < 4; ++j) w[j] = __ldg(reinterpret_cast<const uint32_t*>(from + c) + j);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const uint32_t lo = c + 2 * j < p.cols ? from[c + 2 * j] : 0, hi = c + 2 * j + 1 < p.cols ? from[c + 2 * j + 1] : 0;
+          w[j] = lo | (hi << 16);
+        }
+      }
+      *reinterpret_cast<uint4*>(to + c) = make_uint4(w[0], w[1], w[2], w[3]);
     }
-    *reinterpret_cast<uint4*>(out + r * out_stride + c) = make_uint4(w[0], w[1], w[2], w[3]);
   }
 }
 
@@ -96,8 +114,9 @@ __global__ void __launch_bounds__(256) linear_dz_kernel(const T* dy, int64_t dy_
 template <typename T, typename O, int BN, bool SWAP>
 bool allow_smem() {
   constexpr bool PROMOTE = sizeof(O) == 4;
+  using L = TileSmem<BN, PROMOTE>;
   return cudaFuncSetAttribute(cdg_linear_tile_kernel<T, O, BN, PROMOTE, SWAP>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                              TileSmem<BN, PROMOTE>::kBytes) == cudaSuccess;
+                              std::max(L::kBytes, L::bytes(L::kStagesAlone))) == cudaSuccess;
 }
 
 template <typename T, typename O, int BN>
@@ -109,7 +128,7 @@ bool allow_pair_smem() {
 template <typename T, typename O>
 bool allow_smem_for() {
   return allow_pair_smem<T, O, 256>() && allow_smem<T, O, 64, false>() && allow_smem<T, O, 128, false>() &&
-         allow_smem<T, O, 16, true>() && allow_smem<T, O, 32, true>() && allow_smem<T, O, 64, true>();
+         allow_smem<T, O, 16, true>() && allow_smem<T, O, 32, true>();
 }
 
 template <typename T>
@@ -153,16 +172,24 @@ size_t repack_bytes(const Matrix& m) {
   return tma_rows(m) ? 0 : (static_cast<size_t>(m.rows) * padded(m.cols) * 2 + 255) / 256 * 256;
 }
 
-int repack(Matrix& m, uint8_t*& ws, cudaStream_t st) {
-  if (tma_rows(m)) return CDG_OK;
-  const size_t bytes = repack_bytes(m);
-  const int64_t stride = padded(m.cols), total = m.rows * stride / 8;
-  const unsigned grid = static_cast<unsigned>(std::min<int64_t>((total + 255) / 256, int64_t(sm_count()) * 16));
-  repack_rows_kernel<<<grid, 256, 0, st>>>(static_cast<const uint16_t*>(m.p), m.stride, m.rows, m.cols,
-                                           reinterpret_cast<uint16_t*>(ws), stride);
-  m.p = ws;
-  m.stride = stride;
-  ws += bytes;
+// Replaces the operands that TMA cannot load (b may be NULL) by copies in the workspace.
+int repack(Matrix* a, Matrix* b, uint8_t*& ws, cudaStream_t st) {
+  Repack todo[2];
+  int n = 0;
+  int64_t most = 0;
+  for (Matrix* m : {a, b}) {
+    if (!m || tma_rows(*m)) continue;
+    const int64_t stride = padded(m->cols);
+    todo[n++] = Repack{static_cast<const uint16_t*>(m->p), m->stride, m->rows, m->cols, reinterpret_cast<uint16_t*>(ws), stride};
+    most = std::max(most, m->rows);
+    const size_t bytes = repack_bytes(*m);
+    m->p = ws;
+    m->stride = stride;
+    ws += bytes;
+  }
+  if (n == 0 || most == 0) return CDG_OK;
+  const dim3 grid(static_cast<unsigned>(std::min<int64_t>((most + 7) / 8, int64_t(sm_count()) * 16)), n);
+  repack_rows_kernel<<<grid, 256, 0, st>>>(todo[0], n == 2 ? todo[1] : todo[0]);
   return launched();
 }
 
@@ -187,13 +214,16 @@ int make_map(CUtensorMap* map, const Matrix& m, int dtype, uint32_t box_rows) {
 }
 
 template <typename T, typename O, int BN, bool SWAP>
-int launch_tiles(const CUtensorMap& ta, const CUtensorMap& tb, const LinearShape& s, const Epilogue& e, int splits,
+int launch_tiles(const CUtensorMap& ta, const CUtensorMap& tb, LinearShape s, const Epilogue& e, int splits,
                  cudaStream_t st) {
   constexpr bool PROMOTE = sizeof(O) == 4;
+  using L = TileSmem<BN, PROMOTE>;
+  const int64_t ctas = int64_t(s.m_tiles) * s.n_tiles * splits;
+  s.stages = ctas <= sm_count() ? L::kStagesAlone : L::kStages;
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(static_cast<unsigned>(s.m_tiles) * s.n_tiles * splits);
+  cfg.gridDim = dim3(static_cast<unsigned>(ctas));
   cfg.blockDim = dim3(kTileThreads);
-  cfg.dynamicSmemBytes = TileSmem<BN, PROMOTE>::kBytes;
+  cfg.dynamicSmemBytes = L::bytes(s.stages);
   cfg.stream = st;
   cudaLaunchAttribute at[1];
   at[0].id = cudaLaunchAttributeClusterDimension;
@@ -229,53 +259,48 @@ int launch_pairs(const Matrix& A, const Matrix& B, const LinearShape& s, Epilogu
   return launched();
 }
 
-// How a product is cut.  The costs are cycles of an SM, fitted to measured times (in microseconds,
-// one B200 at 1.9 GHz):
-//   pairs  a wave of 256 x 256 tiles takes about 530 cycles per K step (the tensor cores' 512) and
-//          1500 more; 5000 to start and to drain.
-//   tiles  of 128 x 128 take about 620 cycles per K step alone on an SM and 1170 two at a time, of
-//          128 x 64 about 400 and 770.
+// How a product is cut: pairs (256 x 256 tiles), tiles (128 x 64 or 128 x 128, K split or not), or
+// swapped tiles (up to 32 rows of x).  The costs are microseconds, fitted to the GPU times of 11
+// shapes under every cut, from 64 x 4096 x 4096 to 16,384 x 64 x 1024 (one B200, launch apart).  What
+// they decide, for instance: 64 x 4096 x 4096 pairs 25.8, 128 x 64 in 4 parts 13.8 us; 1024 x 2048 x
+// 2048 pairs 17.1, 128 x 64 16.7, 128 x 128 in 2 parts 18.0 us; 300 x 8192 x 512 pairs 10.4, 128 x 128
+// 12.5 us; 3000 x 3000 x 256 pairs 12.5, 128 x 128 22.3 us.
 struct Plan {
   enum Kind { kPairs, kTiles, kSwapped } kind;
   int bn, splits;
 };
 
 Plan make_plan(int64_t M, int64_t N, int64_t k_steps, int sms) {
-  Plan p{Plan::kTiles, 64, 1};
-  // K is split while there are CTAs to spare (two per SM) and each part keeps four K steps
-  auto split = [&](int64_t tiles) {
-    int s = 1;
-    while (s < 8 && tiles * s * 2 <= 2 * sms && k_steps / (s * 2) >= 4) s *= 2;
-    return s;
-  };
-  if (M <= 64) {
-    p.kind = Plan::kSwapped;
-    p.bn = M <= 16 ? 16 : M <= 32 ? 32 : 64;
-    p.splits = split((N + 127) / 128);
+  if (M <= 32) {
+    Plan p{Plan::kSwapped, M <= 16 ? 16 : 32, 1};
+    const int64_t tiles = (N + 127) / 128;
+    // two CTAs per SM and at least four K steps each
+    while (p.splits < 8 && tiles * p.splits * 2 <= 2 * sms && k_steps / (p.splits * 2) >= 4) p.splits *= 2;
     return p;
   }
-  auto tile_cost = [&](int bn, int s) {
-    const int64_t ctas = (M + 127) / 128 * ((N + bn - 1) / bn) * s;
-    const double alone = bn == 128 ? 620 : 400, two = bn == 128 ? 1170 : 770;
-    const double steps = static_cast<double>((k_steps + s - 1) / s);
-    if (ctas <= sms) return steps * alone + 6000 + (s > 1 ? 2000 : 0);
-    return static_cast<double>((ctas + 2 * sms - 1) / (2 * sms)) * (steps * two + 3000) + 3000 + (s > 1 ? 2000 : 0);
-  };
-  double best = 1e300;
+  Plan best{Plan::kTiles, 128, 1};
+  double least = 1e300;
   for (int bn : {64, 128}) {
-    const int s = split((M + 127) / 128 * ((N + bn - 1) / bn));
-    const double c = tile_cost(bn, s);
-    if (c < best) {
-      best = c;
-      p.bn = bn;
-      p.splits = s;
+    for (int s = 1; s <= 8; s *= 2) {
+      const int64_t ctas = (M + 127) / 128 * ((N + bn - 1) / bn) * s;
+      if (s > 1 && (ctas > 2 * sms || k_steps / s < 4)) break;
+      const double steps = static_cast<double>((k_steps + s - 1) / s);
+      double cost;
+      if (ctas <= sms)  // a CTA has its SM alone
+        cost = bn == 64 ? 5.5 + 0.22 * steps : 4.9 + 0.29 * steps + (s > 1 ? 0.5 * s : 0.0);
+      else
+        cost = static_cast<double>((ctas + 2 * sms - 1) / (2 * sms)) *
+               (bn == 64 ? 7.5 + 0.2 * steps + (s > 1 ? 1.5 : 0.0) : 7.0 + 0.4 * steps + (s > 1 ? 1.0 + 0.6 * s : 0.0));
+      if (cost < least) {
+        least = cost;
+        best = Plan{Plan::kTiles, bn, s};
+      }
     }
   }
   const int64_t pairs = std::max(1, sms / 2), pair_tiles = (M + 255) / 256 * ((N + 255) / 256);
-  if (k_steps > 0 &&
-      static_cast<double>((pair_tiles + pairs - 1) / pairs) * (static_cast<double>(k_steps) * 530 + 1500) + 5000 < best)
-    p.kind = Plan::kPairs;
-  return p;
+  const double waves = static_cast<double>((pair_tiles + pairs - 1) / pairs);
+  if (k_steps > 0 && waves * (0.28 * static_cast<double>(k_steps) + 0.8) + 4.8 < least) best.kind = Plan::kPairs;
+  return best;
 }
 
 // D [M, N] = epilogue(sum over K of A and B); a_mn: A lies as [K, M], else [M, K]; b_mn: B lies as
@@ -316,9 +341,8 @@ int product(const Matrix& A, bool a_mn, const Matrix& B, bool b_mn, int64_t M, i
       if (rc == CDG_OK) rc = make_map(&tb, A, kType, p.bn);
       if (rc != CDG_OK) return rc;
     }
-    return p.bn == 16   ? launch_tiles<T, O, 16, true>(ta, tb, s, e, p.splits, st)
-           : p.bn == 32 ? launch_tiles<T, O, 32, true>(ta, tb, s, e, p.splits, st)
-                        : launch_tiles<T, O, 64, true>(ta, tb, s, e, p.splits, st);
+    return p.bn == 16 ? launch_tiles<T, O, 16, true>(ta, tb, s, e, p.splits, st)
+                      : launch_tiles<T, O, 32, true>(ta, tb, s, e, p.splits, st);
   }
   if (K > 0) {
     int rc = make_map(&ta, A, kType, a_mn ? 64 : s.a_rows);
@@ -343,8 +367,7 @@ int forward(const cdg_linear_args* g, uint8_t* ws, cudaStream_t st) {
   Matrix x{g->x, g->x_stride, g->M, g->K}, w{g->w, g->w_stride, g->N, g->K};
   int rc = CDG_OK;
   if (g->K > 0) {
-    rc = repack(x, ws, st);
-    if (rc == CDG_OK) rc = repack(w, ws, st);
+    rc = repack(&x, &w, ws, st);
     if (rc != CDG_OK) return rc;
   }
   Epilogue e{};
@@ -424,7 +447,7 @@ int backward(const cdg_linear_backward_args* g, uint8_t* ws, cudaStream_t st) {
     if (cudaMemsetAsync(g->db, 0, g->N * element_size(g->db_dtype), st) != cudaSuccess) return CDG_ERR_CUDA;
   }
   if (g->dx) {
-    int rc = g->N > 0 && g->M > 0 ? repack(w, ws, st) : CDG_OK;
+    int rc = g->N > 0 && g->M > 0 ? repack(&w, nullptr, ws, st) : CDG_OK;
     Epilogue e{};
     e.y = g->dx;
     e.y_stride = g->dx_stride;
@@ -433,7 +456,7 @@ int backward(const cdg_linear_backward_args* g, uint8_t* ws, cudaStream_t st) {
     if (rc != CDG_OK) return rc;
   }
   if (g->dw) {
-    int rc = g->M > 0 ? repack(x, ws, st) : CDG_OK;
+    int rc = g->M > 0 ? repack(&x, nullptr, ws, st) : CDG_OK;
     Epilogue e{};
     e.y = g->dw;
     e.y_stride = g->dw_stride;

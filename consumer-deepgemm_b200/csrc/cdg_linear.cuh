@@ -38,22 +38,6 @@ __device__ __forceinline__ void tc_commit_warp(uint64_t* bar) {
       : "memory");
 }
 
-// Load 32 consecutive 32-bit TMEM columns of this warp's 32 lanes.
-__device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&r)[32]) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
-      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
-      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
-        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
-        "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
-        "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
-      : "r"(taddr));
-}
-
-__device__ __forceinline__ void tmem_ld(uint32_t taddr, uint32_t (&r)[32]) { tmem_ld32(taddr, r); }
-__device__ __forceinline__ void tmem_ld(uint32_t taddr, uint32_t (&r)[16]) { tmem_ld16(taddr, r); }
-
 // Operand tiles of one K step (64 columns of K) in shared memory, 128-byte swizzle:
 //   K-major:  [rows][64 k], 8-row groups 1024 bytes apart;
 //   MN-major: chunks of 64 rows, each [64 k][64 rows] (8192 bytes); the 8-k groups of a chunk
@@ -84,11 +68,28 @@ __host__ __device__ __forceinline__ uint32_t idesc_f16(bool bf16, bool a_mn, boo
 // place) is far below the 16-bit outputs' rounding and stays within 1e-6 for 32-bit outputs.
 __device__ __forceinline__ float fast_sigmoid(float v) { return __fdividef(1.0f, 1.0f + __expf(-v)); }
 
+// Phi(-|z|), the normal distribution's tail, = erfc(|z| / sqrt 2) / 2 by Abramowitz and Stegun,
+// Handbook of Mathematical Functions, formula 7.1.26 (erfc(x) = t (a1 + t (a2 + ...)) exp(-x^2),
+// t = 1 / (1 + p x), error below 1.5e-7).  The tail itself, not 1 + erf, so that nothing cancels; a
+// third of erff's instructions, which an epilogue that no product hides is bound by.
+__device__ __forceinline__ float normal_tail(float z) {
+  const float a = fabsf(z);
+  const float t = __fdividef(1.0f, fmaf(0.3275911f * 0.70710678f, a, 1.0f));
+  float p = fmaf(t, 1.061405429f, -1.453152027f);
+  p = fmaf(t, p, 1.421413741f);
+  p = fmaf(t, p, -0.284496736f);
+  p = fmaf(t, p, 0.254829592f);
+  return 0.5f * t * p * __expf(-0.5f * a * a);
+}
+
 __device__ __forceinline__ float activate(float z, int act) {
   switch (act) {
     case CDG_ACT_RELU: return z > 0.0f || z != z ? z : 0.0f;
     case CDG_ACT_SILU: return __fdividef(z, 1.0f + __expf(-z));
-    case CDG_ACT_GELU: return 0.5f * z * (1.0f + erff(z * 0.70710678118654752f));
+    case CDG_ACT_GELU: {
+      const float tail = normal_tail(z);
+      return z * (z < 0.0f ? tail : 1.0f - tail);
+    }
     case CDG_ACT_GELU_TANH: {
       // 0.5 (1 + tanh u) = sigmoid(2u), u = sqrt(2 / pi) (z + 0.044715 z^3)
       const float u2 = 1.5957691216057308f * (z + 0.044715f * z * z * z);
@@ -106,14 +107,40 @@ __device__ __forceinline__ float activate_slope(float z, int act) {
       const float s = fast_sigmoid(z);
       return s * (1.0f + z * (1.0f - s));
     }
-    case CDG_ACT_GELU:
-      return 0.5f * (1.0f + erff(z * 0.70710678118654752f)) + z * __expf(-0.5f * z * z) * 0.39894228040143268f;
+    case CDG_ACT_GELU: {
+      const float tail = normal_tail(z);
+      return (z < 0.0f ? tail : 1.0f - tail) + z * __expf(-0.5f * z * z) * 0.39894228040143268f;
+    }
     case CDG_ACT_GELU_TANH: {
       // with s = sigmoid(2u): z s' + s, s' = s (1 - s) d(2u)/dz
       const float s = fast_sigmoid(1.5957691216057308f * (z + 0.044715f * z * z * z));
       return s + z * s * (1.0f - s) * 1.5957691216057308f * (1.0f + 0.134145f * z * z);
     }
     default: return 1.0f;
+  }
+}
+
+// The activation of C values, with one test for all of them.
+template <int C>
+__device__ __forceinline__ void activate_all(float (&v)[C], int act) {
+  switch (act) {
+    case CDG_ACT_RELU:
+#pragma unroll
+      for (int j = 0; j < C; ++j) v[j] = activate(v[j], CDG_ACT_RELU);
+      break;
+    case CDG_ACT_SILU:
+#pragma unroll
+      for (int j = 0; j < C; ++j) v[j] = activate(v[j], CDG_ACT_SILU);
+      break;
+    case CDG_ACT_GELU:
+#pragma unroll
+      for (int j = 0; j < C; ++j) v[j] = activate(v[j], CDG_ACT_GELU);
+      break;
+    case CDG_ACT_GELU_TANH:
+#pragma unroll
+      for (int j = 0; j < C; ++j) v[j] = activate(v[j], CDG_ACT_GELU_TANH);
+      break;
+    default: break;
   }
 }
 
@@ -134,30 +161,11 @@ __device__ __forceinline__ float load_any(const void* p, int64_t i, int f32) {
   return f32 ? static_cast<const float*>(p)[i] : to_f(static_cast<const T*>(p)[i]);
 }
 
-// Eight consecutive columns [n, n + 8) of row m, clipped at N.
+// Adds the residual to eight consecutive columns [n, n + 8) of row m, clipped at N, and stores them.
 template <typename T, typename O>
-__device__ __forceinline__ void finish8(const Epilogue& e, int64_t m, int64_t n, int64_t N, float (&v)[8]) {
+__device__ __forceinline__ void add_residual_and_store8(const Epilogue& e, int64_t m, int64_t n, int64_t N,
+                                                        float (&v)[8]) {
   const bool full = e.wide && n + 8 <= N;
-  if (e.bias) {
-#pragma unroll
-    for (int j = 0; j < 8; ++j)
-      if (n + j < N) v[j] += load_any<T>(e.bias, n + j, e.bias_f32);
-  }
-  if (e.z) {
-    T* z = static_cast<T*>(e.z) + m * e.z_stride + n;
-    if (full) {
-      *reinterpret_cast<uint4*>(z) = make_uint4(pack2(v[0], v[1], T()), pack2(v[2], v[3], T()),
-                                                pack2(v[4], v[5], T()), pack2(v[6], v[7], T()));
-    } else {
-#pragma unroll
-      for (int j = 0; j < 8; ++j)
-        if (n + j < N) z[j] = from_f<T>(v[j]);
-    }
-  }
-  if (e.act != CDG_ACT_NONE) {
-#pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = activate(v[j], e.act);
-  }
   if (e.residual) {
     if (full && !e.residual_f32) {
       const uint4 r = __ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(e.residual) + m * e.residual_stride + n));
@@ -190,6 +198,29 @@ __device__ __forceinline__ void finish8(const Epilogue& e, int64_t m, int64_t n,
   }
 }
 
+// The whole epilogue of eight consecutive columns [n, n + 8) of row m, clipped at N.
+template <typename T, typename O>
+__device__ __forceinline__ void finish8(const Epilogue& e, int64_t m, int64_t n, int64_t N, float (&v)[8]) {
+  const bool full = e.wide && n + 8 <= N;
+  if (e.bias) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (n + j < N) v[j] += load_any<T>(e.bias, n + j, e.bias_f32);
+  }
+  if (e.z) {
+    T* z = static_cast<T*>(e.z) + m * e.z_stride + n;
+    if (full) {
+      *reinterpret_cast<uint4*>(z) = make_uint4(pack2(v[0], v[1], T()), pack2(v[2], v[3], T()),
+                                                pack2(v[4], v[5], T()), pack2(v[6], v[7], T()));
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (n + j < N) z[j] = from_f<T>(v[j]);
+    }
+  }
+  activate_all<8>(v, e.act);
+  add_residual_and_store8<T, O>(e, m, n, N, v);
+}
 // One element.
 template <typename T, typename O>
 __device__ __forceinline__ void finish1(const Epilogue& e, int64_t m, int64_t n, float v) {
@@ -200,30 +231,80 @@ __device__ __forceinline__ void finish1(const Epilogue& e, int64_t m, int64_t n,
   static_cast<O*>(e.y)[m * e.y_stride + n] = from_f<O>(v);
 }
 
-// 32 rows x 32 columns of a warp, lane = row, turned in shared memory (32 x 33 floats of the warp's
-// own) so that the lanes load and store along the rows: four lanes with eight columns each per
-// row, or, where rows do not start on 16-byte boundaries, one column per lane.
+// v[j] += bias[n + j] (the same for every lane).
+template <typename T, int CH>
+__device__ __forceinline__ void add_bias(const Epilogue& e, int64_t n, int64_t N, float (&v)[CH]) {
+  if (e.bias) {
+    if (e.wide_bias && n + CH <= N) {
+#pragma unroll
+      for (int g = 0; g < CH / 8; ++g) {
+        const uint4 r = __ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(e.bias) + n) + g);
+        const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float2 f = unpack2(w[j], T());
+          v[g * 8 + 2 * j] += f.x;
+          v[g * 8 + 2 * j + 1] += f.y;
+        }
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < CH; ++j)
+        if (n + j < N) v[j] += load_any<T>(e.bias, n + j, e.bias_f32);
+    }
+  }
+}
+
+// Epilogues take 16 columns at a time in loops that are not unrolled: with 64 unrolled columns and
+// five activations the code outgrew the instruction cache, and a tile that no other product hides
+// spent most of its epilogue fetching instructions.
+constexpr int kTurnFloats = 32 * 17;
+
+// 32 rows x 16 columns of a warp, lane = row, turned in shared memory (kTurnFloats of the warp's own)
+// so that the lanes store along the rows.
+__device__ __forceinline__ void turn16(const float (&v)[16], float* turn, int lane) {
+  __syncwarp();
+#pragma unroll
+  for (int j = 0; j < 16; ++j) turn[lane * 17 + j] = v[j];
+  __syncwarp();
+}
+
+// The epilogue of 32 rows x 16 columns from the accumulator, lane = row.  Bias and activation come
+// before the turn, where a lane has 16 independent values; then two lanes with eight columns each
+// take a row, or, where rows do not start on 16-byte boundaries, 16 lanes with one column each.
 template <typename T, typename O>
 __device__ __forceinline__ void finish_turned(const Epilogue& e, int64_t m0, int64_t M, int64_t n0, int64_t N,
-                                              const float (&v)[32], float* turn, int lane) {
-  __syncwarp();
-#pragma unroll
-  for (int j = 0; j < 32; ++j) turn[lane * 33 + j] = v[j];
-  __syncwarp();
+                                              float (&v)[16], float* turn, int lane) {
+  add_bias<T, 16>(e, n0, N, v);
+  const int64_t n = n0 + (lane & 15);
+  const int rows = n < N ? static_cast<int>(M - m0 < 32 ? M - m0 : 32) : 0;
+  if (e.z) {
+    turn16(v, turn, lane);
+    T* z = static_cast<T*>(e.z) + m0 * e.z_stride + n;
+#pragma unroll 4
+    for (int row = lane >> 4; row < rows; row += 2) z[row * e.z_stride] = from_f<T>(turn[row * 17 + (lane & 15)]);
+  }
+  activate_all<16>(v, e.act);
+  turn16(v, turn, lane);
   if (e.wide) {
-    const int64_t n = n0 + (lane & 3) * 8;
+    const int64_t n8 = n0 + (lane & 1) * 8;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int row = i * 8 + (lane >> 2);
+    for (int i = 0; i < 2; ++i) {
+      const int row = i * 16 + (lane >> 1);
       float w[8];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) w[j] = turn[row * 33 + (lane & 3) * 8 + j];
-      if (m0 + row < M && n < N) finish8<T, O>(e, m0 + row, n, N, w);
+      for (int j = 0; j < 8; ++j) w[j] = turn[row * 17 + (lane & 1) * 8 + j];
+      if (m0 + row < M && n8 < N) add_residual_and_store8<T, O>(e, m0 + row, n8, N, w);
     }
-  } else {
-    const int rows = static_cast<int>(M - m0 < 32 ? M - m0 : 32);
-    if (n0 + lane < N)
-      for (int row = 0; row < rows; ++row) finish1<T, O>(e, m0 + row, n0 + lane, turn[row * 33 + lane]);
+    return;
+  }
+  O* y = static_cast<O*>(e.y) + m0 * e.y_stride + n;
+  const int64_t r0 = m0 * e.residual_stride + n;
+#pragma unroll 4
+  for (int row = lane >> 4; row < rows; row += 2) {
+    float f = turn[row * 17 + (lane & 15)];
+    if (e.residual) f += load_any<T>(e.residual, r0 + row * e.residual_stride, e.residual_f32);
+    y[row * e.y_stride] = from_f<O>(f);
   }
 }
 
@@ -233,6 +314,7 @@ struct LinearShape {
   int m_tiles, n_tiles;
   int a_rows;          // rows of A's box: 128, or M rounded up to 8 where M is smaller (K-major)
   int a_mn, b_mn, bf16;
+  int stages;          // of the tile kernel
 };
 
 // ---------------------------------------------------------------- one tile per CTA, K split over a cluster
@@ -243,7 +325,7 @@ struct LinearShape {
 // PROMOTE (32-bit outputs): the tensor core's running sum loses about one part in 2^20 over a
 // few thousand terms (its additions truncate), which 16-bit outputs do not see; here a sum
 // covers 512 of K at most, and FP32 registers add those up.
-// SWAP (few rows of x): A is the weight and B is x, so that 128 rows of the weight meet 16, 32 or 64
+// SWAP (few rows of x): A is the weight and B is x, so that 128 rows of the weight meet 16 or 32
 // rows of x without tiles that are mostly padding; the epilogue's roles of rows and columns change
 // places with them (M and N here are those of the swapped product).
 // Warps: 0-3 epilogue (one per TMEM lane quadrant), 4 TMA producer, 5 MMA issuer and TMEM owner.
@@ -252,13 +334,18 @@ struct TileSmem {
   static constexpr int kA = 128 * 128;
   static constexpr int kB = BN * 128;
   static constexpr int kStageBytes = kA + kB;
+  // stages where two CTAs share an SM, and where a CTA has one alone: more loads in flight then
+  // make up for the second CTA's (1110 cycles per K step of 128 x 128 with three stages)
   static constexpr int kStages = BN >= 128 ? 3 : BN == 64 ? 4 : BN == 32 ? 5 : 6;
-  static constexpr int kBars = kStages * kStageBytes;  // full, empty [kStages]; tfull, tempty [2]; TMEM address
-  static constexpr int kBytes = kBars + (2 * kStages + 4) * 8 + 16 + 1024;
+  static constexpr int kStagesAlone = BN >= 128 ? 6 : 8;
+  // after the stages: full, empty [stages]; tfull, tempty [2]; TMEM address
+  static constexpr int bytes(int stages) { return stages * kStageBytes + (2 * stages + 4) * 8 + 16 + 1024; }
+  static constexpr int kBytes = bytes(kStages);
   static constexpr int kAccs = PROMOTE ? 2 : 1;
   static constexpr int kTmemCols = kAccs * BN < 32 ? 32 : kAccs * BN;
   static_assert(128 * BN * 4 <= kStages * kStageBytes, "the split's partial sums reuse the stages");
   static_assert(2 * kBytes <= 228 * 1024, "two CTAs per SM");
+  static_assert(bytes(kStagesAlone) <= 232448, "shared memory per CTA");
 };
 
 constexpr int kTileThreads = 192;
@@ -269,11 +356,11 @@ __global__ void __launch_bounds__(kTileThreads)
     cdg_linear_tile_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_b,
                            const LinearShape s, const Epilogue e, const int splits) {
   using L = TileSmem<BN, PROMOTE>;
-  constexpr int S = L::kStages;
-  constexpr int CC = BN < 32 ? BN : 32;  // columns taken out of TMEM at a time
+  const int S = s.stages;
+  constexpr int CC = 16;  // columns taken out of TMEM at a time
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint64_t* full = reinterpret_cast<uint64_t*>(smem + L::kBars);
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + S * L::kStageBytes);
   uint64_t* empty = full + S;
   uint64_t* tfull = empty + S;
   uint64_t* tempty = tfull + 2;
@@ -388,7 +475,7 @@ __global__ void __launch_bounds__(kTileThreads)
 #pragma unroll
         for (int c = 0; c < BN / CC; ++c) {
           uint32_t r[CC];
-          tmem_ld(lanes + buf * BN + c * CC, r);
+          tmem_ld16(lanes + buf * BN + c * CC, r);
           tmem_ld_wait();
 #pragma unroll
           for (int j = 0; j < CC; ++j) acc[c * CC + j] += __uint_as_float(r[j]);
@@ -400,32 +487,39 @@ __global__ void __launch_bounds__(kTileThreads)
       if (sums && !mbar_wait_cta_warp(&tfull[0], 0, nullptr, wait_code(4, 0, 0, 0, 0))) ok = false;
       tc_fence_after();
     }
+    // every product of this CTA has completed, so the stages are free
+    auto finish = [&](int at, float (&v)[CC]) {
+      if (splits > 1) {
+#pragma unroll
+        for (int j = 0; j < CC; ++j) part[(at + j) * 128 + warp * 32 + lane] = v[j];
+      } else if constexpr (SWAP) {
+        if (m < s.M) {
+          for (int j = 0; j < CC; ++j)
+            if (n0 + at + j < s.N) finish1<T, O>(e, n0 + at + j, m, v[j]);
+        }
+      } else if (m0 + warp * 32 < s.M && n0 + at < s.N) {
+        finish_turned<T, O>(e, m0 + warp * 32, s.M, n0 + at, s.N, v, part + warp * kTurnFloats, lane);
+      }
+    };
     if (ok) {
+      if constexpr (PROMOTE) {
 #pragma unroll
-      for (int c = 0; c < BN / CC; ++c) {
-        float v[CC];
-        if constexpr (PROMOTE) {
+        for (int at = 0; at < BN; at += CC) {
+          float v[CC];
 #pragma unroll
-          for (int j = 0; j < CC; ++j) v[j] = acc[c * CC + j];
-        } else {
+          for (int j = 0; j < CC; ++j) v[j] = acc[at + j];
+          finish(at, v);
+        }
+      } else {
+#pragma unroll 1
+        for (int at = 0; at < BN; at += CC) {
           uint32_t r[CC];
-          tmem_ld(lanes + c * CC, r);
+          tmem_ld16(lanes + at, r);
           tmem_ld_wait();
+          float v[CC];
 #pragma unroll
           for (int j = 0; j < CC; ++j) v[j] = sums ? __uint_as_float(r[j]) : 0.0f;  // K = 0: nothing was summed
-        }
-        // every product of this CTA has completed, so the stages are free
-        if (splits > 1) {
-#pragma unroll
-          for (int j = 0; j < CC; ++j) part[(c * CC + j) * 128 + warp * 32 + lane] = v[j];
-        } else if constexpr (SWAP) {
-          if (m < s.M) {
-#pragma unroll
-            for (int j = 0; j < CC; ++j)
-              if (n0 + c * CC + j < s.N) finish1<T, O>(e, n0 + c * CC + j, m, v[j]);
-          }
-        } else if (m0 + warp * 32 < s.M && n0 + c * CC < s.N) {
-          finish_turned<T, O>(e, m0 + warp * 32, s.M, n0 + c * CC, s.N, v, part + warp * 32 * 33, lane);
+          finish(at, v);
         }
       }
     }
@@ -542,72 +636,32 @@ __device__ __forceinline__ void tile_at(int t, int m_tiles, int n_tiles, int& mt
   nt = in / height;
 }
 
-// Values of the lane's row for CH consecutive columns from n on, from the accumulator (v), through
-// the epilogue, in place of the residual in the staged tile (row `lane`, 128 bytes, 16-byte pieces
-// XORed with the row's low three bits: the 128-byte swizzle).
-template <typename T, typename O, int CH>
-__device__ __forceinline__ void finish_staged(const Epilogue& e, int64_t n, int64_t N, float (&v)[CH], uint8_t* tile,
-                                              int lane) {
+// The epilogue of 16 consecutive columns from n on of the lane's row, in place of the residual in
+// the staged tile (row `lane`, 128 bytes, 16-byte pieces XORed with the row's low three bits: the
+// 128-byte swizzle); `first` is the columns' first piece.
+template <typename T, typename O>
+__device__ __forceinline__ void finish_staged(const Epilogue& e, int64_t n, int64_t N, float (&v)[16], uint8_t* tile,
+                                              int first, int lane) {
   constexpr int kPer = 16 / static_cast<int>(sizeof(O));  // columns per 16-byte piece
-  if (e.bias) {
-    if (e.wide_bias && n + CH <= N) {
+  add_bias<T, 16>(e, n, N, v);
+  activate_all<16>(v, e.act);
 #pragma unroll
-      for (int g = 0; g < CH / 8; ++g) {
-        const uint4 r = __ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(e.bias) + n) + g);
-        const uint32_t w[4] = {r.x, r.y, r.z, r.w};
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const float2 f = unpack2(w[j], T());
-          v[g * 8 + 2 * j] += f.x;
-          v[g * 8 + 2 * j + 1] += f.y;
-        }
-      }
-    } else {
-#pragma unroll
-      for (int j = 0; j < CH; ++j)
-        if (n + j < N) v[j] += load_any<T>(e.bias, n + j, e.bias_f32);
-    }
-  }
-  switch (e.act) {  // one test per chunk, not per value
-    case CDG_ACT_RELU:
-#pragma unroll
-      for (int j = 0; j < CH; ++j) v[j] = activate(v[j], CDG_ACT_RELU);
-      break;
-    case CDG_ACT_SILU:
-#pragma unroll
-      for (int j = 0; j < CH; ++j) v[j] = activate(v[j], CDG_ACT_SILU);
-      break;
-    case CDG_ACT_GELU:
-#pragma unroll
-      for (int j = 0; j < CH; ++j) v[j] = activate(v[j], CDG_ACT_GELU);
-      break;
-    case CDG_ACT_GELU_TANH:
-#pragma unroll
-      for (int j = 0; j < CH; ++j) v[j] = activate(v[j], CDG_ACT_GELU_TANH);
-      break;
-    default: break;
-  }
-#pragma unroll
-  for (int c = 0; c < CH / kPer; ++c) {
-    uint4* at = reinterpret_cast<uint4*>(tile + lane * 128 + ((c ^ (lane & 7)) << 4));
-    if (e.residual) {
-      const uint4 r = *at;
-      const uint32_t w[4] = {r.x, r.y, r.z, r.w};
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        if constexpr (sizeof(O) == 4) {
-          v[c * kPer + j] += __uint_as_float(w[j]);
-        } else {
-          const float2 f = unpack2(w[j], O());
-          v[c * kPer + 2 * j] += f.x;
-          v[c * kPer + 2 * j + 1] += f.y;
-        }
-      }
-    }
+  for (int c = 0; c < 16 / kPer; ++c) {
+    uint4* at = reinterpret_cast<uint4*>(tile + lane * 128 + (((first + c) ^ (lane & 7)) << 4));
     if constexpr (sizeof(O) == 4) {
       *at = make_uint4(__float_as_uint(v[c * 4]), __float_as_uint(v[c * 4 + 1]), __float_as_uint(v[c * 4 + 2]),
                        __float_as_uint(v[c * 4 + 3]));
     } else {
+      if (e.residual) {
+        const uint4 r = *at;
+        const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float2 f = unpack2(w[j], O());
+          v[c * 8 + 2 * j] += f.x;
+          v[c * 8 + 2 * j + 1] += f.y;
+        }
+      }
       *at = make_uint4(pack2(v[c * 8], v[c * 8 + 1], O()), pack2(v[c * 8 + 2], v[c * 8 + 3], O()),
                        pack2(v[c * 8 + 4], v[c * 8 + 5], O()), pack2(v[c * 8 + 6], v[c * 8 + 7], O()));
     }
@@ -793,31 +847,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairTileSmem<BN>::kT
         }
         tc_fence_after();
       }
-#pragma unroll
-      for (int c = 0; c < kChunks; ++c) {
-        const int n = col0 + c * CH;
-        float v[CH];
-        if constexpr (PROMOTE) {
-#pragma unroll
-          for (int j = 0; j < CH; ++j) v[j] = acc[c * CH + j];
-        } else {
-          uint32_t r0[32], r1[32];
-          tmem_ld32(lanes + (sum & 1) * BN + c * CH, r0);
-          tmem_ld32(lanes + (sum & 1) * BN + c * CH + 32, r1);
-          tmem_ld_wait();
-#pragma unroll
-          for (int j = 0; j < 32; ++j) {
-            v[j] = __uint_as_float(r0[j]);
-            v[(32 + j) % CH] = __uint_as_float(r1[j]);
-          }
-          if (c == kChunks - 1) {
-            tc_fence_before();
-            if (rank == 0) mbar_arrive(&tempty[sum & 1]); else mbar_arrive_cluster(tempty0 + (sum & 1) * 8);
-          }
+      // one 16-column group: `at` columns into the warp's half of the tile
+      auto finish = [&](int at, float (&v)[16]) {
+        const int n = col0 + at, c = at / CH;
+        if (!any || n >= s.N) return;
+        if (!e.staged) {
+          finish_turned<T, O>(e, row0, s.M, n, s.N, v, reinterpret_cast<float*>(stagings), lane);
+          return;
         }
-        if (!any || n >= s.N) continue;
-        if (e.staged) {
-          uint8_t* tile = stagings + (c & 1) * 4096;
+        uint8_t* tile = stagings + (c & 1) * 4096;
+        if (at % CH == 0) {
           if (e.residual) {
             if (!mbar_wait_cta_warp(&rfull[w * 2 + (c & 1)], turn[c & 1], nullptr, wait_code(4, 8 + w, c, turn[c & 1], 0)))
               ok = false;
@@ -827,22 +866,39 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairTileSmem<BN>::kT
             if (lane == 0) bulk_wait_read_but_one();
             __syncwarp();
           }
-          finish_staged<T, O, CH>(e, n, s.N, v, tile, lane);
+        }
+        finish_staged<T, O>(e, n, s.N, v, tile, at % CH * static_cast<int>(sizeof(O)) / 16, lane);
+        if (at % CH == CH - 16 || n + 16 >= s.N) {
           fence_proxy_async_shared();
           __syncwarp();
           if (lane == 0) {
-            tma_store_2d(&tmap_y, tile, n, row0);
+            tma_store_2d(&tmap_y, tile, col0 + c * CH, row0);
             bulk_commit();
           }
-        } else {
+        }
+      };
+      if constexpr (PROMOTE) {
 #pragma unroll
-          for (int g = 0; g < CH / 32; ++g) {
-            float u[32];
+        for (int at = 0; at < BN / 2; at += 16) {
+          float v[16];
 #pragma unroll
-            for (int j = 0; j < 32; ++j) u[j] = v[g * 32 + j];
-            if (n + g * 32 < s.N)
-              finish_turned<T, O>(e, row0, s.M, n + g * 32, s.N, u, reinterpret_cast<float*>(stagings), lane);
+          for (int j = 0; j < 16; ++j) v[j] = acc[at + j];
+          finish(at, v);
+        }
+      } else {
+#pragma unroll 1
+        for (int at = 0; at < BN / 2; at += 16) {
+          uint32_t r[16];
+          tmem_ld16(lanes + (sum & 1) * BN + at, r);
+          tmem_ld_wait();
+          if (at == BN / 2 - 16) {
+            tc_fence_before();
+            if (rank == 0) mbar_arrive(&tempty[sum & 1]); else mbar_arrive_cluster(tempty0 + (sum & 1) * 8);
           }
+          float v[16];
+#pragma unroll
+          for (int j = 0; j < 16; ++j) v[j] = __uint_as_float(r[j]);
+          finish(at, v);
         }
       }
       if constexpr (!PROMOTE) ++sum;

@@ -54,19 +54,20 @@ __device__ __forceinline__ float cta_sum(float v, float* slot, int warps) {
 }
 
 // Scale and reciprocal factor of a 128-column block with the largest magnitude `amax`.  A NaN
-// among the values does not reach the scale (fmaxf passes over it); its own code is NaN.
+// among the values does not reach the scale (fmaxf passes over it); its own code is NaN.  The FP32
+// recipe's scale and factor are a product and a fast division (two units in the last place); the
+// power-of-two recipe needs amax / 448 exactly, since its exponent is rounded up.
 __device__ __forceinline__ float block_scale(float amax, int pow2, float& factor) {
   amax = fmaxf(amax, 1e-12f);
-  float scale = amax / 448.0f;
   if (pow2) {
-    uint32_t b = __float_as_uint(scale);
+    uint32_t b = __float_as_uint(amax / 448.0f);
     if (b & 0x007FFFFFu) b = (b & 0xFF800000u) + 0x00800000u;
-    scale = __uint_as_float(b);
+    const float scale = __uint_as_float(b);
     factor = 1.0f / scale;
-  } else {
-    factor = 448.0f / amax;
+    return scale;
   }
-  return scale;
+  factor = __fdividef(448.0f, amax);
+  return amax * (1.0f / 448.0f);
 }
 
 struct NormFwd {
@@ -76,7 +77,7 @@ struct NormFwd {
   float* s;
   int64_t x_stride, r_stride, h_stride, y_stride, q_stride, s_stride_m, s_stride_k;
   int64_t T, H;
-  float eps;
+  float eps, inv_h;
   int w_f32, pow2;
 };
 
@@ -171,7 +172,7 @@ __global__ void __launch_bounds__(THREADS) add_rms_norm_kernel(const NormFwd a, 
       store8<T, WIDE>(static_cast<T*>(a.h) + row * a.h_stride, i * warps_per_row + w, lane, a.H, h[i]);
   }
   sum = cta_sum(sum, slot, warps_per_row);
-  const float rstd = 1.0f / sqrtf(sum / static_cast<float>(a.H) + a.eps);
+  const float rstd = rsqrtf(fmaf(sum, a.inv_h, a.eps));
 #pragma unroll
   for (int i = 0; i < ITER; ++i) {
     const int64_t chunk = i * warps_per_row + w;
@@ -256,7 +257,7 @@ __global__ void __launch_bounds__(THREADS) rms_norm_backward_kernel(const NormBw
       uh += __shfl_xor_sync(0xffffffffu, uh, o);
     }
     const float inv = 1.0f / static_cast<float>(a.H);
-    const float rstd = 1.0f / sqrtf(sq * inv + a.eps);
+    const float rstd = rsqrtf(fmaf(sq, inv, a.eps));
     const float k = uh * inv * rstd * rstd;
 #pragma unroll
     for (int i = 0; i < ITER; ++i) {
@@ -367,7 +368,7 @@ __global__ void __launch_bounds__(1024) rms_norm_backward_ring_kernel(const Norm
       sq += __shfl_xor_sync(0xffffffffu, sq, o);
       uh += __shfl_xor_sync(0xffffffffu, uh, o);
     }
-    const float rstd = 1.0f / sqrtf(sq * inv + a.eps);
+    const float rstd = rsqrtf(fmaf(sq, inv, a.eps));
     const float k = uh * inv * rstd * rstd;
     float out[8];
 #pragma unroll
@@ -476,7 +477,7 @@ int cdg_add_rms_norm(const cdg_norm_args* g, cdg_stream_t stream) {
   if (g->T == 0) return CDG_OK;
   if (!g->x || !g->w || (g->q && !g->s) || (!g->y && !g->q && !g->h)) return CDG_ERR_INVALID_ARGUMENT;
   NormFwd a{g->x, g->r, g->w, g->h, g->y, g->q, g->s, g->x_stride, g->r_stride, g->h_stride, g->y_stride, g->q_stride,
-            g->s_stride_m, g->s_stride_k, g->T, g->H, g->eps, g->w_dtype == CDG_DTYPE_F32, g->scale_fmt};
+            g->s_stride_m, g->s_stride_k, g->T, g->H, g->eps, 1.0f / static_cast<float>(g->H), g->w_dtype == CDG_DTYPE_F32, g->scale_fmt};
   const int64_t e = element_size(g->dtype);
   const bool wide = g->H % 8 == 0 && wide_rows(a.x, a.x_stride, e) && wide_rows(a.r, a.r_stride, e) &&
                     wide_rows(a.h, a.h_stride, e) && wide_rows(a.y, a.y_stride, e) && wide_rows(a.w, 0, e) &&
