@@ -581,24 +581,27 @@ __global__ void __launch_bounds__(kTileThreads)
 // ---------------------------------------------------------------- CTA pairs, persistent, for many tiles
 // A pair of CTAs takes tiles of 256 x BN (256) in turn: CTA r of it holds rows 128r .. 128r + 127 of A and
 // of the result and half of B's rows.  The tensor cores fill one of two accumulators in TMEM while
-// eight epilogue warps per CTA empty the other (warp w: the 32 lanes of quadrant w % 4, half of the
-// columns).  Staged (y, and the residual where there is one, of the output's type and on 16-byte
-// rows, z not stored): each epilogue warp has the residual brought into its own two shared-memory
-// tiles of 32 rows x 128 bytes by TMA, ahead of the accumulator, adds it in place and has the result
-// stored from there, so that global memory sees whole tiles; clipping at M and N is TMA's.
-// Otherwise its lanes load and store their rows themselves.
-// Warps: 0 TMA producer, 1 MMA issuer (even CTA) and TMEM owner, 4-11 epilogue.
+// sixteen epilogue warps per CTA empty the other (warp w: the 32 lanes of quadrant w % 4, a quarter of
+// the columns; eight warps of half the columns each, two per scheduler, waited for their own
+// instructions and took 4.3 us a tile, more than the products of K = 512).  Staged (y, and the
+// residual where there is one, of the output's type and on 16-byte rows, z not stored): each epilogue
+// warp has the residual brought into its own shared-memory tile of 32 rows x 128 bytes by TMA, ahead
+// of the accumulator, adds it in place and has the result stored from there, so that global memory
+// sees whole tiles; clipping at M and N is TMA's.  Otherwise its lanes turn their columns and store
+// along the rows themselves.
+// Warps: 0 TMA producer, 1 MMA issuer (even CTA) and TMEM owner, 4-19 epilogue.
 template <int BN>
 struct PairTileSmem {
   static constexpr int kA = 128 * 128;
   static constexpr int kB = BN / 2 * 128;
   static constexpr int kStageBytes = kA + kB;
   static constexpr int kStages = 5;
-  static constexpr int kEpiWarps = 8;
-  static constexpr int kStaging = kStages * kStageBytes;      // [warp][2] tiles of 4096 bytes
-  static constexpr int kBars = kStaging + kEpiWarps * 2 * 4096;
-  // full, empty [kStages]; tfull, tempty [2]; done; residual [warp][2]; TMEM address
-  static constexpr int kBytes = kBars + (2 * kStages + 5 + kEpiWarps * 2) * 8 + 16 + 1024;
+  static constexpr int kEpiWarps = 16;
+  static constexpr int kStaging = kStages * kStageBytes;      // [warp] tiles of 4096 bytes
+  static constexpr int kBars = kStaging + kEpiWarps * 4096;
+  // full, empty [kStages]; tfull, tempty [2]; done; residual [warp]; TMEM address
+  static constexpr int kBytes = kBars + (2 * kStages + 5 + kEpiWarps) * 8 + 16 + 1024;
+  static_assert(kTurnFloats * 4 <= 4096, "a warp turns its columns in its staged tile");
   static constexpr int kThreads = 128 + 32 * kEpiWarps;
   static_assert(kBytes <= 232448, "shared memory per CTA");
 };
@@ -636,17 +639,17 @@ __device__ __forceinline__ void tile_at(int t, int m_tiles, int n_tiles, int& mt
   nt = in / height;
 }
 
-// The epilogue of 16 consecutive columns from n on of the lane's row, in place of the residual in
+// The epilogue of 32 consecutive columns from n on of the lane's row, in place of the residual in
 // the staged tile (row `lane`, 128 bytes, 16-byte pieces XORed with the row's low three bits: the
 // 128-byte swizzle); `first` is the columns' first piece.
 template <typename T, typename O>
-__device__ __forceinline__ void finish_staged(const Epilogue& e, int64_t n, int64_t N, float (&v)[16], uint8_t* tile,
+__device__ __forceinline__ void finish_staged(const Epilogue& e, int64_t n, int64_t N, float (&v)[32], uint8_t* tile,
                                               int first, int lane) {
   constexpr int kPer = 16 / static_cast<int>(sizeof(O));  // columns per 16-byte piece
-  add_bias<T, 16>(e, n, N, v);
-  activate_all<16>(v, e.act);
+  add_bias<T, 32>(e, n, N, v);
+  activate_all<32>(v, e.act);
 #pragma unroll
-  for (int c = 0; c < 16 / kPer; ++c) {
+  for (int c = 0; c < 32 / kPer; ++c) {
     uint4* at = reinterpret_cast<uint4*>(tile + lane * 128 + (((first + c) ^ (lane & 7)) << 4));
     if constexpr (sizeof(O) == 4) {
       *at = make_uint4(__float_as_uint(v[c * 4]), __float_as_uint(v[c * 4 + 1]), __float_as_uint(v[c * 4 + 2]),
@@ -677,7 +680,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairTileSmem<BN>::kT
   constexpr bool PROMOTE = sizeof(O) == 4;
   constexpr int S = L::kStages;
   constexpr int CH = 128 / static_cast<int>(sizeof(O));  // columns of a staged tile
-  constexpr int kChunks = BN / 2 / CH;                   // staged tiles of a warp per output tile (2 or 4)
+  constexpr int kCols = BN / 4;                          // columns of an epilogue warp: CH, or 2 CH in FP32
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + L::kBars);
@@ -686,7 +689,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairTileSmem<BN>::kT
   uint64_t* tempty = tfull + 2;
   uint64_t* done = tempty + 2;
   uint64_t* rfull = done + 1;
-  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(rfull + L::kEpiWarps * 2);
+  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(rfull + L::kEpiWarps);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = cluster_ctarank();
   const int pair = static_cast<int>(blockIdx.x >> 1), pairs = static_cast<int>(gridDim.x >> 1);
@@ -704,7 +707,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairTileSmem<BN>::kT
       mbar_init(&tempty[i], 2 * 32 * L::kEpiWarps);
     }
     mbar_init(done, 1);
-    for (int i = 0; i < 2 * L::kEpiWarps; ++i) mbar_init(&rfull[i], 1);
+    for (int i = 0; i < L::kEpiWarps; ++i) mbar_init(&rfull[i], 1);
     fence_mbarrier_init();
   }
   if (warp == 1) {
@@ -791,36 +794,31 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairTileSmem<BN>::kT
       mbar_wait_cluster_warp(done, 0, nullptr, wait_code(5, 0, 0, 0, 0));
     }
   } else if (warp >= 4) {
-    const int w = warp - 4, half = w >> 2, q = warp & 3;
+    const int w = warp - 4, quarter = w >> 2, q = warp & 3;
     const uint32_t tempty0 = cluster_addr(&tempty[0], 0);
-    uint8_t* stagings = smem + L::kStaging + w * 2 * 4096;
-    const uint32_t lanes = tmem + (static_cast<uint32_t>(q * 32) << 16) + half * (BN / 2);
+    uint8_t* tile = smem + L::kStaging + w * 4096;
+    const uint32_t lanes = tmem + (static_cast<uint32_t>(q * 32) << 16) + quarter * kCols;
     int sum = 0;
-    uint32_t turn[2] = {};  // phase of each staged tile's residual barrier
+    uint32_t turn = 0;  // phase of the staged tile's residual barrier
     for (int t = pair; t < tiles && ok; t += pairs) {
       int mt, nt;
       tile_at(t, s.m_tiles, s.n_tiles, mt, nt);
-      const int row0 = mt * 256 + static_cast<int>(rank) * 128 + q * 32, col0 = nt * BN + half * (BN / 2);
-      const bool any = row0 < s.M;  // a warp past the last row only keeps the barriers moving
+      const int row0 = mt * 256 + static_cast<int>(rank) * 128 + q * 32, col0 = nt * BN + quarter * kCols;
+      const bool any = row0 < s.M && col0 < s.N;  // a warp past the edges only keeps the barriers moving
       if (e.staged && any) {
         if (lane == 0) {
-          bulk_wait_read();  // the last tile's stores have read the staged tiles
-          if (e.residual) {  // with 16-bit results alone, where a warp has two chunks
-#pragma unroll
-            for (int c = 0; c < 2; ++c) {
-              if (col0 + c * CH < s.N) {
-                mbar_arrive_expect_tx(&rfull[w * 2 + c], 4096);
-                tma_load_2d(stagings + c * 4096, &tmap_r, &rfull[w * 2 + c], col0 + c * CH, row0);
-              }
-            }
+          bulk_wait_read();  // the last tile's store has read the staged tile
+          if (e.residual) {  // with 16-bit results alone
+            mbar_arrive_expect_tx(&rfull[w], 4096);
+            tma_load_2d(tile, &tmap_r, &rfull[w], col0, row0);
           }
         }
         __syncwarp();
       }
-      float acc[PROMOTE ? BN / 2 : 1];
       if constexpr (PROMOTE) {
+        float acc[kCols];
 #pragma unroll
-        for (int j = 0; j < BN / 2; ++j) acc[j] = 0.0f;
+        for (int j = 0; j < kCols; ++j) acc[j] = 0.0f;
         for (int k = 0; k < s.k_steps; k += kPromoteSteps, ++sum) {
           const int buf = sum & 1;
           if (!mbar_wait_cluster_warp(&tfull[buf], (sum >> 1) & 1, nullptr, wait_code(4, static_cast<int>(rank), buf, sum >> 1, k))) {
@@ -829,7 +827,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairTileSmem<BN>::kT
           }
           tc_fence_after();
 #pragma unroll
-          for (int c = 0; c < BN / 32; ++c) {  // 16 at a time: the sums take most of the registers
+          for (int c = 0; c < kCols / 16; ++c) {
             uint32_t r[16];
             tmem_ld16(lanes + buf * BN + c * 16, r);
             tmem_ld_wait();
@@ -840,68 +838,91 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairTileSmem<BN>::kT
           if (rank == 0) mbar_arrive(&tempty[buf]); else mbar_arrive_cluster(tempty0 + buf * 8);
         }
         if (!ok) break;
+        if (!any) continue;
+        if (e.staged) {
+#pragma unroll
+          for (int c = 0; c < kCols / 32; ++c) {
+            const int n = col0 + c * 32;
+            if (n >= s.N) break;
+            float v[32];
+#pragma unroll
+            for (int j = 0; j < 32; ++j) v[j] = acc[c * 32 + j];
+            if (c > 0) {
+              if (lane == 0) bulk_wait_read();
+              __syncwarp();
+            }
+            finish_staged<T, O>(e, n, s.N, v, tile, 0, lane);
+            fence_proxy_async_shared();
+            __syncwarp();
+            if (lane == 0) {
+              tma_store_2d(&tmap_y, tile, n, row0);
+              bulk_commit();
+            }
+          }
+        } else {
+#pragma unroll
+          for (int c = 0; c < kCols / 16; ++c) {
+            float v[16];
+#pragma unroll
+            for (int j = 0; j < 16; ++j) v[j] = acc[c * 16 + j];
+            if (col0 + c * 16 < s.N)
+              finish_turned<T, O>(e, row0, s.M, col0 + c * 16, s.N, v, reinterpret_cast<float*>(tile), lane);
+          }
+        }
       } else {
-        if (!mbar_wait_cluster_warp(&tfull[sum & 1], (sum >> 1) & 1, nullptr, wait_code(4, static_cast<int>(rank), sum & 1, sum >> 1, 0))) {
+        const int buf = sum & 1;
+        if (!mbar_wait_cluster_warp(&tfull[buf], (sum >> 1) & 1, nullptr, wait_code(4, static_cast<int>(rank), buf, sum >> 1, 0))) {
           ok = false;
           break;
         }
+        ++sum;
         tc_fence_after();
-      }
-      // one 16-column group: `at` columns into the warp's half of the tile
-      auto finish = [&](int at, float (&v)[16]) {
-        const int n = col0 + at, c = at / CH;
-        if (!any || n >= s.N) return;
-        if (!e.staged) {
-          finish_turned<T, O>(e, row0, s.M, n, s.N, v, reinterpret_cast<float*>(stagings), lane);
-          return;
+        auto drained = [&]() {  // this thread has taken its part of the accumulator
+          tc_fence_before();
+          if (rank == 0) mbar_arrive(&tempty[buf]); else mbar_arrive_cluster(tempty0 + buf * 8);
+        };
+        if (!any) {
+          drained();
+          continue;
         }
-        uint8_t* tile = stagings + (c & 1) * 4096;
-        if (at % CH == 0) {
+        if (e.staged) {
           if (e.residual) {
-            if (!mbar_wait_cta_warp(&rfull[w * 2 + (c & 1)], turn[c & 1], nullptr, wait_code(4, 8 + w, c, turn[c & 1], 0)))
-              ok = false;
-            turn[c & 1] ^= 1;
+            if (!mbar_wait_cta_warp(&rfull[w], turn, nullptr, wait_code(4, 8 + w % 8, w, turn, 0))) ok = false;
+            turn ^= 1;
           }
-          if (c >= 2) {  // the store of two chunks ago has read the tile
-            if (lane == 0) bulk_wait_read_but_one();
-            __syncwarp();
+#pragma unroll 1
+          for (int c = 0; c < kCols; c += 32) {
+            uint32_t r[2][16];
+            tmem_ld16(lanes + buf * BN + c, r[0]);
+            tmem_ld16(lanes + buf * BN + c + 16, r[1]);
+            tmem_ld_wait();
+            if (c + 32 >= kCols) drained();
+            float v[32];
+#pragma unroll
+            for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(r[j / 16][j % 16]);
+            if (col0 + c < s.N) finish_staged<T, O>(e, col0 + c, s.N, v, tile, c * static_cast<int>(sizeof(O)) / 16, lane);
           }
-        }
-        finish_staged<T, O>(e, n, s.N, v, tile, at % CH * static_cast<int>(sizeof(O)) / 16, lane);
-        if (at % CH == CH - 16 || n + 16 >= s.N) {
           fence_proxy_async_shared();
           __syncwarp();
           if (lane == 0) {
-            tma_store_2d(&tmap_y, tile, col0 + c * CH, row0);
+            tma_store_2d(&tmap_y, tile, col0, row0);
             bulk_commit();
           }
-        }
-      };
-      if constexpr (PROMOTE) {
-#pragma unroll
-        for (int at = 0; at < BN / 2; at += 16) {
-          float v[16];
-#pragma unroll
-          for (int j = 0; j < 16; ++j) v[j] = acc[at + j];
-          finish(at, v);
-        }
-      } else {
+        } else {
 #pragma unroll 1
-        for (int at = 0; at < BN / 2; at += 16) {
-          uint32_t r[16];
-          tmem_ld16(lanes + (sum & 1) * BN + at, r);
-          tmem_ld_wait();
-          if (at == BN / 2 - 16) {
-            tc_fence_before();
-            if (rank == 0) mbar_arrive(&tempty[sum & 1]); else mbar_arrive_cluster(tempty0 + (sum & 1) * 8);
-          }
-          float v[16];
+          for (int c = 0; c < kCols; c += 16) {
+            uint32_t r[16];
+            tmem_ld16(lanes + buf * BN + c, r);
+            tmem_ld_wait();
+            if (c + 16 >= kCols) drained();
+            float v[16];
 #pragma unroll
-          for (int j = 0; j < 16; ++j) v[j] = __uint_as_float(r[j]);
-          finish(at, v);
+            for (int j = 0; j < 16; ++j) v[j] = __uint_as_float(r[j]);
+            if (col0 + c < s.N)
+              finish_turned<T, O>(e, row0, s.M, col0 + c, s.N, v, reinterpret_cast<float*>(tile), lane);
+          }
         }
       }
-      if constexpr (!PROMOTE) ++sum;
     }
     if (e.staged && lane == 0) bulk_wait_all();
     __syncwarp();
