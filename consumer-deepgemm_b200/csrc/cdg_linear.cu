@@ -248,9 +248,9 @@ int launch_pairs(const Matrix& A, const Matrix& B, const LinearShape& s, Epilogu
   const Matrix y{e.y, e.y_stride, M, N}, r{e.residual, e.residual_stride, M, N};
   const bool apart = M == 1 || (y.stride >= N && (!e.residual || r.stride >= N));
   // (FP32 results have four chunks a warp and tile, and no staged residual)
-  e.staged = e.wide && !e.z && apart && (!e.residual || (sizeof(O) == 2 && !e.residual_f32));
-  if (rc == CDG_OK && e.staged) rc = make_map(&ty, y, kOut, 32);
-  if (rc == CDG_OK && e.staged && e.residual) rc = make_map(&tr, r, kOut, 32);
+  e.staged = e.z || (e.residual && (sizeof(O) == 4 || e.residual_f32)) ? 0 : e.wide && apart ? 1 : 2;
+  if (rc == CDG_OK && e.staged == 1) rc = make_map(&ty, y, kOut, 32);
+  if (rc == CDG_OK && e.staged == 1 && e.residual) rc = make_map(&tr, r, kOut, 32);
   if (rc != CDG_OK) return rc;
   const unsigned grid =
       static_cast<unsigned>(2 * std::min<int64_t>(int64_t(s.m_tiles) * s.n_tiles, std::max(1, sm_count() / 2)));

@@ -24,6 +24,12 @@ U = 2.0 ** -24
 UNIT = {torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11, torch.float32: 2.0 ** -24}
 
 
+@pytest.fixture(autouse=True)
+def _seed():
+    """The same inputs in every run and order."""
+    torch.manual_seed(20)
+
+
 def _cdg():
     import consumer_deep_gemm
 
