@@ -222,7 +222,7 @@ int launch_tiles(const CUtensorMap& ta, const CUtensorMap& tb, LinearShape s, co
   s.stages = ctas <= sm_count() ? L::kStagesAlone : L::kStages;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(static_cast<unsigned>(ctas));
-  cfg.blockDim = dim3(kTileThreads);
+  cfg.blockDim = dim3(kThreadsOf<SWAP>);
   cfg.dynamicSmemBytes = L::bytes(s.stages);
   cfg.stream = st;
   cudaLaunchAttribute at[1];

@@ -376,7 +376,9 @@ struct LinearShape {
 // the latency of its epilogue's few warps: with four warps alone, one lane per row, 2910 x 94 x 192
 // with a residual took 26 us.
 // Warps: 0-3 accumulator (one per TMEM lane quadrant), 4 TMA producer, 5 MMA issuer and TMEM owner.
-constexpr int kTileThreads = 320;
+// Threads: the ten warps named above; swapped tiles have few columns to finish and start sooner with six.
+template <bool SWAP>
+constexpr int kThreadsOf = SWAP ? 192 : 320;
 constexpr int kPartStride = 129;
 
 template <int BN, bool PROMOTE>
@@ -401,12 +403,13 @@ struct TileSmem {
 constexpr int kPromoteSteps = 8;  // K steps of 64 per running sum
 
 template <typename T, typename O, int BN, bool PROMOTE, bool SWAP>
-__global__ void __launch_bounds__(kTileThreads)
+__global__ void __launch_bounds__(kThreadsOf<SWAP>)
     cdg_linear_tile_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_b,
                            const LinearShape s, const Epilogue e, const int splits) {
   using L = TileSmem<BN, PROMOTE>;
   const int S = s.stages;
   constexpr int CC = 16;  // columns taken out of TMEM at a time
+  constexpr int kTileThreads = kThreadsOf<SWAP>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + S * L::kStageBytes);
@@ -565,6 +568,20 @@ __global__ void __launch_bounds__(kTileThreads)
   const int share = 128 / splits, row0 = split * share;  // this CTA's rows of the tile
   const int rows = static_cast<int>(s.M - m0 - row0 < share ? s.M - m0 - row0 : share);  // below 1: none
   const int cols = static_cast<int>(s.N - n0 < BN ? s.N - n0 : BN);
+  // The accumulator at one place: the sum over the cluster's CTAs (eight at most), in rank order, all
+  // of the (remote) reads in flight together.
+  auto total = [&](const float* at) {
+    if (splits == 1) return *at;
+    float f[8], v = 0.0f;
+#pragma unroll
+    for (int r = 0; r < 8; ++r) {
+      f[r] = 0.0f;
+      if (r < splits) asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(f[r]) : "r"(cluster_addr(at, r)));
+    }
+#pragma unroll
+    for (int r = 0; r < 8; ++r) v += f[r];
+    return v;
+  };
   // The accumulator at eight places: each the sum over the cluster's CTAs, in rank order; the eight
   // (remote) reads of a CTA are in flight together.
   auto totals = [&](const float* at, int step, int count, float (&v)[8]) {
@@ -589,30 +606,28 @@ __global__ void __launch_bounds__(kTileThreads)
     }
   };
   if constexpr (SWAP) {
-    // rows of the weight run along y: a thread keeps one of this CTA's, and takes columns, eight at a
-    // time so that their residual loads are in flight together
+    // rows of the weight run along y: a thread keeps one of this CTA's and takes columns, two at a time
+    // (one, mostly, where K is split; eight at a time cost 1.4 us of predicated work)
     const int row = row0 + t % share, lanes = kTileThreads / share;
     const int64_t n = m0 + row;
     if (n < s.M && t < lanes * share) {
       const float bias = e.bias ? load_any<T>(e.bias, n, e.bias_f32) : 0.0f;
-      for (int c = t / share; c < cols; c += lanes * 8) {
-        float v[8], r[8];
+      for (int c = t / share; c < cols; c += lanes * 2) {
+        float v[2], r[2];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
+        for (int j = 0; j < 2; ++j) {
           const int col = c + j * lanes;
           r[j] = e.residual && col < cols ? load_any<T>(e.residual, (n0 + col) * e.residual_stride + n, e.residual_f32) : 0.0f;
+          v[j] = bias + (col < cols ? total(part + col * kPartStride + row) : 0.0f);
         }
-        totals(part + c * kPartStride + row, lanes * kPartStride, (cols - c + lanes - 1) / lanes, v);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] += bias;
         if (e.z) {
 #pragma unroll
-          for (int j = 0; j < 8; ++j)
+          for (int j = 0; j < 2; ++j)
             if (c + j * lanes < cols) static_cast<T*>(e.z)[(n0 + c + j * lanes) * e.z_stride + n] = from_f<T>(v[j]);
         }
-        activate_all<8>(v, e.act);
+        activate_all<2>(v, e.act);
 #pragma unroll
-        for (int j = 0; j < 8; ++j)
+        for (int j = 0; j < 2; ++j)
           if (c + j * lanes < cols) static_cast<O*>(e.y)[(n0 + c + j * lanes) * e.y_stride + n] = from_f<O>(v[j] + r[j]);
       }
     }

@@ -118,10 +118,14 @@ __device__ __forceinline__ void quant_chunk(const NormFwd& a, int64_t row, int64
       for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
       float f;
       const float scale = block_scale(m, a.pow2, f);
+      uint8_t* to = q + column<false>(chunk, lane, 4 * b);
+      const bool full = (kb + b + 1) * 128 <= a.H;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int64_t c = column<false>(chunk, lane, 4 * b + j);
-        if (c < a.H) q[c] = __nv_cvt_float_to_fp8(y[4 * b + j] * f, __NV_SATFINITE, __NV_E4M3);
+      for (int j = 0; j < 4; j += 2) {
+        const uint32_t two =
+            __nv_cvt_float2_to_fp8x2(make_float2(y[4 * b + j] * f, y[4 * b + j + 1] * f), __NV_SATFINITE, __NV_E4M3);
+        if (full || column<false>(chunk, lane, 4 * b + j) < a.H) to[j * 32] = static_cast<uint8_t>(two);
+        if (full || column<false>(chunk, lane, 4 * b + j + 1) < a.H) to[(j + 1) * 32] = static_cast<uint8_t>(two >> 8);
       }
       if (lane == 0 && (kb + b) * 128 < a.H) s[(kb + b) * a.s_stride_k] = scale;
     }

@@ -93,14 +93,26 @@ __device__ __forceinline__ Raw<T> load8(const T* row, int64_t chunk, int lane, i
       }
     }
   } else {
+    // a chunk that lies in the row needs no test per column
+    const T* from = row + column<false>(chunk, lane, 0);
+    const int left = static_cast<int>(H - chunk * 256 < 256 ? H - chunk * 256 : 256);
+    if (left == 256) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const int64_t c = column<false>(chunk, lane, j);
-      if (c < H) {
+      for (int j = 0; j < 8; ++j) {
         if constexpr (sizeof(T) == 4)
-          raw.w[j] = reinterpret_cast<const uint32_t*>(row)[c];
+          raw.w[j] = reinterpret_cast<const uint32_t*>(from)[j * 32];
         else
-          raw.w[j / 2] |= static_cast<uint32_t>(reinterpret_cast<const uint16_t*>(row)[c]) << (16 * (j & 1));
+          raw.w[j / 2] |= static_cast<uint32_t>(reinterpret_cast<const uint16_t*>(from)[j * 32]) << (16 * (j & 1));
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        if (j * 32 + lane < left) {
+          if constexpr (sizeof(T) == 4)
+            raw.w[j] = reinterpret_cast<const uint32_t*>(from)[j * 32];
+          else
+            raw.w[j / 2] |= static_cast<uint32_t>(reinterpret_cast<const uint16_t*>(from)[j * 32]) << (16 * (j & 1));
+        }
       }
     }
   }
@@ -120,10 +132,15 @@ __device__ __forceinline__ void store8(T* row, int64_t chunk, int lane, int64_t 
       p[0] = make_uint4(pack2(v[0], v[1], T()), pack2(v[2], v[3], T()), pack2(v[4], v[5], T()), pack2(v[6], v[7], T()));
     }
   } else {
+    T* to = row + column<false>(chunk, lane, 0);
+    const int left = static_cast<int>(H - chunk * 256 < 256 ? H - chunk * 256 : 256);
+    if (left == 256) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const int64_t c = column<false>(chunk, lane, j);
-      if (c < H) row[c] = from_f<T>(v[j]);
+      for (int j = 0; j < 8; ++j) to[j * 32] = from_f<T>(v[j]);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (j * 32 + lane < left) to[j * 32] = from_f<T>(v[j]);
     }
   }
 }
@@ -137,7 +154,7 @@ __global__ void __launch_bounds__(1024) column_sum_kernel(const float* partial, 
   const int64_t c = static_cast<int64_t>(blockIdx.x) * 32 + lane;
   float v = 0.0f;
   if (c < H) {
-#pragma unroll 4
+#pragma unroll 8
     for (int p = g; p < parts; p += 32) v += partial[static_cast<int64_t>(p) * H + c];
   }
   sums[g][lane] = v;
