@@ -437,6 +437,9 @@ __global__ void __launch_bounds__(kThreadsOf<SWAP>)
     }
     fence_mbarrier_init();
   }
+  // operands may be the previous kernel's results; nor does this kernel take TMEM from it
+  grid_dependency_wait();
+  grid_launch_dependents();
   if (warp == 5) {
     tmem_alloc(tmem_holder, L::kTmemCols);
     tmem_relinquish();
@@ -879,6 +882,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairTileSmem<BN>::kT
     for (int i = 0; i < L::kEpiWarps; ++i) mbar_init(&rfull[i], 1);
     fence_mbarrier_init();
   }
+  // operands may be the previous kernel's results; nor does this kernel take TMEM from it
+  grid_dependency_wait();
+  grid_launch_dependents();
   if (warp == 1) {
     tmem_alloc_pair(tmem_holder, 2 * BN);
     tmem_relinquish_pair();

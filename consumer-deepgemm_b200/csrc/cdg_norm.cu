@@ -21,7 +21,6 @@
 #include <mutex>
 
 #include "cdg_b200.h"
-#include "cdg_ptx.cuh"
 #include "cdg_rows.cuh"
 
 namespace cdg {
@@ -208,6 +207,7 @@ struct NormBwd {
 template <typename T, bool WIDE, int ITER, int THREADS>
 __global__ void __launch_bounds__(THREADS) rms_norm_backward_kernel(const NormBwd a) {
   __shared__ float2 slot[2][32];
+  grid_launch_dependents();  // the sum over the CTAs' weight gradients
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
   const T* dy = static_cast<const T*>(a.dy);
   const T* h = static_cast<const T*>(a.h);
@@ -305,6 +305,7 @@ __global__ void __launch_bounds__(1024) rms_norm_backward_ring_kernel(const Norm
   extern __shared__ __align__(128) uint8_t ring[];
   __shared__ float2 slot_sum[2][32];
   __shared__ __align__(8) uint64_t full[kRingMax];
+  grid_launch_dependents();  // the sum over the CTAs' weight gradients
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
   const uint32_t row_bytes = static_cast<uint32_t>(a.H * sizeof(T));
   const int arrays = a.dh ? 3 : 2;
@@ -525,12 +526,10 @@ int cdg_rms_norm_backward(const cdg_norm_backward_args* g, void* workspace, size
   if (rc != CDG_OK) return rc;
   const unsigned grid = static_cast<unsigned>((g->H + 31) / 32);
   if (g->w_dtype == CDG_DTYPE_BF16)
-    column_sum_kernel<__nv_bfloat16><<<grid, 1024, 0, st>>>(a.partial, s.grid, g->H, static_cast<__nv_bfloat16*>(g->dw));
-  else if (g->w_dtype == CDG_DTYPE_F16)
-    column_sum_kernel<__half><<<grid, 1024, 0, st>>>(a.partial, s.grid, g->H, static_cast<__half*>(g->dw));
-  else
-    column_sum_kernel<float><<<grid, 1024, 0, st>>>(a.partial, s.grid, g->H, static_cast<float*>(g->dw));
-  return launched();
+    return launch_after(column_sum_kernel<__nv_bfloat16>, dim3(grid), 1024, 0, st, a.partial, s.grid, g->H, static_cast<__nv_bfloat16*>(g->dw));
+  if (g->w_dtype == CDG_DTYPE_F16)
+    return launch_after(column_sum_kernel<__half>, dim3(grid), 1024, 0, st, a.partial, s.grid, g->H, static_cast<__half*>(g->dw));
+  return launch_after(column_sum_kernel<float>, dim3(grid), 1024, 0, st, a.partial, s.grid, g->H, static_cast<float*>(g->dw));
 }
 
 }  // extern "C"

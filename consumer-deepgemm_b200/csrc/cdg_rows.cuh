@@ -9,6 +9,7 @@
 #include <cstdint>
 
 #include "cdg_b200.h"
+#include "cdg_ptx.cuh"
 
 namespace cdg {
 namespace {
@@ -150,6 +151,8 @@ __device__ __forceinline__ void store8(T* row, int64_t chunk, int lane, int64_t 
 template <typename W>
 __global__ void __launch_bounds__(1024) column_sum_kernel(const float* partial, int parts, int64_t H, W* out) {
   __shared__ float sums[32][33];
+  grid_dependency_wait();  // the partial sums are the previous kernel's
+  grid_launch_dependents();
   const int lane = threadIdx.x & 31, g = threadIdx.x >> 5;
   const int64_t c = static_cast<int64_t>(blockIdx.x) * 32 + lane;
   float v = 0.0f;
@@ -169,6 +172,24 @@ __global__ void __launch_bounds__(1024) column_sum_kernel(const float* partial, 
 
 // ------------------------------------------------------------------ host
 inline int launched() { return cudaGetLastError() == cudaSuccess ? CDG_OK : CDG_ERR_CUDA; }
+
+// Launch of a call's second or later kernel: scheduled while its predecessor drains (unless
+// cdg_set_pdl(0)); the kernel itself waits for the predecessor's end (griddepcontrol.wait) before it
+// touches global memory.
+template <typename... K, typename... A>
+inline int launch_after(void (*kernel)(K...), dim3 grid, unsigned block, size_t smem, cudaStream_t st, A&&... args) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(block);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = cdg_get_pdl() ? 1 : 0;
+  return cudaLaunchKernelEx(&cfg, kernel, static_cast<K>(args)...) == cudaSuccess ? CDG_OK : CDG_ERR_CUDA;
+}
 
 // SM count of the current device (looked up at each call: a cheap attribute query).
 inline int sm_count() {
