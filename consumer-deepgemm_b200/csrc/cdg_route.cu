@@ -54,48 +54,66 @@ __device__ __forceinline__ float warp_sum(float v) {
 
 // Fast exponential and division (errors of a few units in the last place): the gate's weights
 // and gradients stay within 1e-6 of the exact ones.
-__device__ __forceinline__ float sigmoid_fast(float v) { return __fdividef(1.0f, 1.0f + __expf(-v)); }
+__device__ __forceinline__ float exp_fast(float v) {
+  // 2^(v log2 e), results below the normal range taken as 0 (__expf spends three instructions on them)
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v * 1.4426950408889634f));
+  return r;
+}
+__device__ __forceinline__ float sigmoid_fast(float v) { return __fdividef(1.0f, 1.0f + exp_fast(-v)); }
 
 // The k experts of the largest keys of a row, of equal keys the lowest first: lane j gets the j-th
 // (x its key, y the expert), or y = -1 where no key that can be chosen is left.  key[i] is that of
 // expert i * 32 + lane, mine the lane's largest.
 //
 // The k-th largest of the 32 lanes' maxima is a lower bound of the k-th largest key, and few keys
-// reach it (with 256 experts and k = 8 about ten), so: k rounds over the maxima alone give the
-// bound; the keys that reach it are listed in the order of their experts; each lane takes one of
-// the list and counts how many of the others go before it.  A list of more than 32 (many equal
-// keys, or k near 32) is chosen from round by round.  At 32,768 x 256, k = 8 the choice round by
-// round alone took the kernel 43 us.
+// reach it (with 256 experts and k = 8 about ten), so: the maxima are sorted across the lanes (a
+// bitonic network) for the bound; the keys that reach it are listed, each with its expert; each lane
+// takes one of the list and counts how many of the others go before it.  A list of more than 32, or
+// a lane with more than four of them (many equal keys, or k near 32), is chosen from round by round,
+// a warp-wide maximum each; at 32,768 x 256, k = 8 that alone took the kernel 43 us.
 template <int N>
-__device__ __forceinline__ int2 choose(uint32_t (&key)[N], uint32_t mine, int k, int lane, uint2* list) {
-  uint32_t bound = 0;
+__device__ __forceinline__ int2 choose(uint32_t (&key)[N], uint32_t mine, int k, int lane, unsigned long long* list) {
   uint32_t top = mine;
-  for (int j = 0; j < k; ++j) {
-    bound = __reduce_max_sync(kAll, top);
-    if (bound < kFirstKey) break;
-    if (lane == __ffs(__ballot_sync(kAll, top == bound)) - 1) top = 0;
-  }
-  bound = max(bound, kFirstKey);
-  int count = 0;
 #pragma unroll
-  for (int i = 0; i < N; ++i) {
-    const unsigned at = __ballot_sync(kAll, key[i] >= bound);
-    if (at == 0) continue;
-    const int place = count + __popc(at & ((1u << lane) - 1u));
-    if (key[i] >= bound && place < 32) list[place] = make_uint2(key[i], i * 32 + lane);
-    count += __popc(at);
+  for (int size = 2; size <= 32; size *= 2) {
+#pragma unroll
+    for (int j = size / 2; j > 0; j /= 2) {
+      const uint32_t other = __shfl_xor_sync(kAll, top, j);
+      top = ((lane & j) == 0) == ((lane & size) == 0) ? max(top, other) : min(top, other);  // falling order
+    }
   }
+  const uint32_t bound = max(__shfl_sync(kAll, top, k - 1), kFirstKey);
+  int reach = 0;
+#pragma unroll
+  for (int i = 0; i < N; ++i) reach += key[i] >= bound ? 1 : 0;
+  const unsigned one = __ballot_sync(kAll, reach > 0), two = __ballot_sync(kAll, reach > 1),
+                 three = __ballot_sync(kAll, reach > 2), four = __ballot_sync(kAll, reach > 3);
+  const int count = __popc(one) + __popc(two) + __popc(three) + __popc(four);
   int2 got = make_int2(0, -1);
-  if (count <= 32) {
+  if (count <= 32 && !__any_sync(kAll, reach > 4)) {
+    if (reach > 0) {
+      const unsigned below = (1u << lane) - 1u;
+      int place = __popc(one & below) + __popc(two & below) + __popc(three & below) + __popc(four & below);
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        // key first, then the lower expert
+        if (key[i] >= bound)
+          list[place++] = (static_cast<unsigned long long>(key[i]) << 32) | (0xFFFFFFFFu - static_cast<uint32_t>(i * 32 + lane));
+      }
+    }
     __syncwarp();
-    const uint2 own = lane < count ? list[lane] : make_uint2(0, 0);
+    const unsigned long long own = lane < count ? list[lane] : 0;
     int before = 0;
-    for (int j = 0; j < count; ++j)  // of equal keys the one listed first, the lower expert, goes first
-      before += __shfl_sync(kAll, own.x, j) >= own.x + (j < lane ? 0u : 1u) ? 1 : 0;
+#pragma unroll 4
+    for (int j = 0; j < count; ++j) before += list[j] > own ? 1 : 0;
     __syncwarp();
     if (lane < count && before < k) list[before] = own;
     __syncwarp();
-    if (lane < min(count, k)) got = make_int2(static_cast<int>(list[lane].x), static_cast<int>(list[lane].y));
+    if (lane < min(count, k)) {
+      const unsigned long long v = list[lane];
+      got = make_int2(static_cast<int>(v >> 32), static_cast<int>(0xFFFFFFFFu - static_cast<uint32_t>(v)));
+    }
     __syncwarp();
     return got;
   }
@@ -164,7 +182,7 @@ __global__ void __launch_bounds__(WARPS * 32) moe_route_kernel(const Route a) {
   extern __shared__ int32_t route_smem[];
   __shared__ double scratch[WARPS];
   __shared__ int32_t s_tokens, s_last;
-  __shared__ uint2 s_list[WARPS][32];
+  __shared__ unsigned long long s_list[WARPS][32];
   int32_t* s_counts = route_smem;
   float* s_psum = reinterpret_cast<float*>(route_smem + a.E);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -179,10 +197,16 @@ __global__ void __launch_bounds__(WARPS * 32) moe_route_kernel(const Route a) {
   int32_t tokens = 0;
   const int64_t step = static_cast<int64_t>(gridDim.x) * WARPS;
   float next[N];
+  const int left = a.E - lane;  // expert i * 32 + lane exists where i * 32 < left
   auto load_row = [&](int64_t row) {
+    const T* at = logits + row * a.stride + lane;
+    if (a.E == N * 32) {
 #pragma unroll
-    for (int i = 0; i < N; ++i)
-      next[i] = i * 32 + lane < a.E ? to_f(logits[row * a.stride + i * 32 + lane]) : -INFINITY;
+      for (int i = 0; i < N; ++i) next[i] = to_f(at[i * 32]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < N; ++i) next[i] = i * 32 < left ? to_f(at[i * 32]) : -INFINITY;
+    }
   };
   int64_t row = static_cast<int64_t>(blockIdx.x) * WARPS + warp;
   if (row < a.T) load_row(row);
@@ -208,11 +232,11 @@ __global__ void __launch_bounds__(WARPS * 32) moe_route_kernel(const Route a) {
         float total = 0.0f;
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-          v[i] = a.sigmoid ? sigmoid_fast(v[i]) : __expf(v[i] - m);
+          v[i] = a.sigmoid ? sigmoid_fast(v[i]) : exp_fast(v[i] - m);
           total += v[i];
         }
         total = warp_sum(total);
-        part = total > 0.0f ? 1.0f / total : 0.0f;
+        part = total > 0.0f ? __fdividef(1.0f, total) : 0.0f;
         if (!a.sigmoid) inv = part;
         if (a.bias) {
 #pragma unroll
@@ -235,13 +259,13 @@ __global__ void __launch_bounds__(WARPS * 32) moe_route_kernel(const Route a) {
         if (id >= 0) {
           // the key is that of the logit itself, unless a bias went into it
           const float l = a.bias ? clean_logit(to_f(logits[row * a.stride + id])) : key_value(got.x);
-          w = a.sigmoid ? sigmoid_fast(l) : __expf(l - m) * inv;
+          w = a.sigmoid ? sigmoid_fast(l) : exp_fast(l - m) * inv;
           atomicAdd(&s_counts[id], 1);
         }
       }
       if (a.renormalize) {
         const float total = warp_sum(w);
-        w = total > 0.0f ? w / total : 0.0f;
+        w = total > 0.0f ? __fdividef(w, total) : 0.0f;
       }
       w *= a.scale;
     }
@@ -345,10 +369,11 @@ __global__ void __launch_bounds__(WARPS * 32) moe_route_backward_kernel(const Ro
   float next[N];
   int32_t next_id = -1;
   float next_g = 0.0f;
+  const int left = a.E - lane;  // expert i * 32 + lane exists where i * 32 < left
   auto load_row = [&](int64_t row) {
+    const T* at = logits + row * a.stride + lane;
 #pragma unroll
-    for (int i = 0; i < N; ++i)
-      next[i] = i * 32 + lane < a.E ? to_f(logits[row * a.stride + i * 32 + lane]) : -INFINITY;
+    for (int i = 0; i < N; ++i) next[i] = i * 32 < left ? to_f(at[i * 32]) : -INFINITY;
     if (lane < a.k) {
       next_id = __ldg(a.ids + row * a.k + lane);
       if (a.gw) next_g = __ldg(a.gw + row * a.k + lane);
@@ -378,11 +403,11 @@ __global__ void __launch_bounds__(WARPS * 32) moe_route_backward_kernel(const Ro
     float total = 0.0f;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      s[i] = a.sigmoid ? sigmoid_fast(s[i]) : __expf(s[i] - m);
+      s[i] = a.sigmoid ? sigmoid_fast(s[i]) : exp_fast(s[i] - m);
       total += s[i];
     }
     total = warp_sum(total);
-    const float inv = total > 0.0f ? 1.0f / total : 0.0f;
+    const float inv = total > 0.0f ? __fdividef(1.0f, total) : 0.0f;
     if (!a.sigmoid) {
 #pragma unroll
       for (int i = 0; i < N; ++i) s[i] *= inv;  // the scores are the probabilities
@@ -392,10 +417,10 @@ __global__ void __launch_bounds__(WARPS * 32) moe_route_backward_kernel(const Ro
         float c = 0.0f;
         if (id >= 0) {
           const float l = clean_logit(to_f(logits[row * a.stride + id]));
-          c = a.sigmoid ? sigmoid_fast(l) : __expf(l - m) * inv;
+          c = a.sigmoid ? sigmoid_fast(l) : exp_fast(l - m) * inv;
         }
         float chosen = warp_sum(c);
-        chosen = chosen > 0.0f ? 1.0f / chosen : 1.0f;
+        chosen = chosen > 0.0f ? __fdividef(1.0f, chosen) : 1.0f;
         g = (g - warp_sum(g * c) * chosen) * chosen;
       }
       if (id >= 0) atomicAdd(&sg[id], g);
@@ -405,7 +430,7 @@ __global__ void __launch_bounds__(WARPS * 32) moe_route_backward_kernel(const Ro
     float dot = 0.0f;  // of what meets the probabilities: everything (softmax) or the loss alone
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      d[i] = a.gw && i * 32 + lane < a.E ? sg[i * 32 + lane] : 0.0f;
+      d[i] = a.gw && i * 32 < left ? sg[i * 32 + lane] : 0.0f;
       dot = fmaf(a.sigmoid ? load[i] : d[i] + load[i], s[i], dot);
     }
     dot = warp_sum(dot);
@@ -421,7 +446,7 @@ __global__ void __launch_bounds__(WARPS * 32) moe_route_backward_kernel(const Ro
         v = (d[i] + (load[i] - dot * inv) * inv) * s[i] * (1.0f - s[i]);
       else
         v = s[i] * (d[i] + load[i] - dot);
-      if (i * 32 + lane < a.E) out[i * 32 + lane] = from_f<T>(v);
+      if (i * 32 < left) out[i * 32 + lane] = from_f<T>(v);
     }
   }
 }
