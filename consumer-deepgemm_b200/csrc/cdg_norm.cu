@@ -297,11 +297,12 @@ __global__ void __launch_bounds__(THREADS) rms_norm_backward_kernel(const NormBw
 }
 
 // The same with the rows brought into shared memory by bulk copies, for rows on 16-byte boundaries
-// of up to 8192 columns: thread t holds columns 8t .. 8t + 7 of every row of its CTA, and a ring of
+// of up to 8192 columns: warp w holds chunks w and w + warps of every row of its CTA, and a ring of
 // `slots` rows (h, dy and dh side by side) keeps the loads of the next rows in flight whatever the
-// registers hold.  At 16,384 x 4096 BF16 the register form moved 3.9 TB/s at its best shape.
+// registers hold.  At 16,384 x 4096 BF16 with dh (537 MB) it takes 93 us, 5.8 TB/s; with one chunk a
+// warp, twice the warps at each row's barrier, 110 us; the register form at its best shape 137 us.
 template <typename T>
-__global__ void __launch_bounds__(1024) rms_norm_backward_ring_kernel(const NormBwd a, const int slots) {
+__global__ void __launch_bounds__(512) rms_norm_backward_ring_kernel(const NormBwd a, const int slots) {
   extern __shared__ __align__(128) uint8_t ring[];
   __shared__ float2 slot_sum[2][32];
   __shared__ __align__(8) uint64_t full[kRingMax];
@@ -329,27 +330,33 @@ __global__ void __launch_bounds__(1024) rms_norm_backward_ring_kernel(const Norm
     for (int i = 0; i < slots; ++i)
       if (blockIdx.x + i * step < a.T) load_row(blockIdx.x + i * step, i);
   }
-  float w[8], acc[8] = {};
-  load_weight8<T, true>(a.w, a.w_f32, warp, lane, a.H, w);
-  const int64_t c = column<true>(warp, lane, 0);
+  constexpr int V = 2;  // chunks of a warp
+  float w[V][8], acc[V][8] = {};
+#pragma unroll
+  for (int u = 0; u < V; ++u) load_weight8<T, true>(a.w, a.w_f32, u * warps + warp, lane, a.H, w[u]);
   const float inv = 1.0f / static_cast<float>(a.H);
   int s = 0, turn = 0;
   uint32_t phase = 0;
   bool ok = true;
   for (int64_t row = blockIdx.x; row < a.T; row += step, turn ^= 1) {
     ok = mbar_wait_cta(&full[s], phase, nullptr, wait_code(1, 1, s, phase, static_cast<int>(row)));
-    const uint8_t* at = ring + static_cast<size_t>(s) * arrays * row_bytes + c * sizeof(T);
-    float hv[8] = {}, g[8] = {}, d[8] = {};
-    if (c < a.H) {
-      unpack8<T>(*reinterpret_cast<const Raw<T>*>(at), hv);
-      unpack8<T>(*reinterpret_cast<const Raw<T>*>(at + row_bytes), g);
-      if (dh) unpack8<T>(*reinterpret_cast<const Raw<T>*>(at + 2 * row_bytes), d);
-    }
+    const uint8_t* at = ring + static_cast<size_t>(s) * arrays * row_bytes;
+    float hv[V][8] = {}, g[V][8] = {}, d[V][8] = {};
     float sq = 0.0f, uh = 0.0f;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      sq = fmaf(hv[j], hv[j], sq);
-      uh = fmaf(g[j] * w[j], hv[j], uh);
+    for (int u = 0; u < V; ++u) {
+      const int64_t c = column<true>(u * warps + warp, lane, 0);
+      if (c < a.H) {
+        const uint8_t* p = at + c * sizeof(T);
+        unpack8<T>(*reinterpret_cast<const Raw<T>*>(p), hv[u]);
+        unpack8<T>(*reinterpret_cast<const Raw<T>*>(p + row_bytes), g[u]);
+        if (dh) unpack8<T>(*reinterpret_cast<const Raw<T>*>(p + 2 * row_bytes), d[u]);
+      }
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        sq = fmaf(hv[u][j], hv[u][j], sq);
+        uh = fmaf(g[u][j] * w[u][j], hv[u][j], uh);
+      }
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
@@ -375,19 +382,26 @@ __global__ void __launch_bounds__(1024) rms_norm_backward_ring_kernel(const Norm
     }
     const float rstd = rsqrtf(fmaf(sq, inv, a.eps));
     const float k = uh * inv * rstd * rstd;
-    float out[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      acc[j] = fmaf(g[j], hv[j] * rstd, acc[j]);
-      out[j] = fmaf(rstd, fmaf(-hv[j], k, g[j] * w[j]), d[j]);
+    for (int u = 0; u < V; ++u) {
+      float out[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        acc[u][j] = fmaf(g[u][j], hv[u][j] * rstd, acc[u][j]);
+        out[j] = fmaf(rstd, fmaf(-hv[u][j], k, g[u][j] * w[u][j]), d[u][j]);
+      }
+      store8<T, true>(static_cast<T*>(a.dx) + row * a.dx_stride, u * warps + warp, lane, a.H, out);
     }
-    store8<T, true>(static_cast<T*>(a.dx) + row * a.dx_stride, warp, lane, a.H, out);
     if (++s == slots) { s = 0; phase ^= 1; }
   }
-  if (c < a.H) {
-    float4* partial = reinterpret_cast<float4*>(a.partial + static_cast<int64_t>(blockIdx.x) * a.H + c);
-    partial[0] = make_float4(acc[0], acc[1], acc[2], acc[3]);
-    partial[1] = make_float4(acc[4], acc[5], acc[6], acc[7]);
+#pragma unroll
+  for (int u = 0; u < V; ++u) {
+    const int64_t c = column<true>(u * warps + warp, lane, 0);
+    if (c < a.H) {
+      float4* partial = reinterpret_cast<float4*>(a.partial + static_cast<int64_t>(blockIdx.x) * a.H + c);
+      partial[0] = make_float4(acc[u][0], acc[u][1], acc[u][2], acc[u][3]);
+      partial[1] = make_float4(acc[u][4], acc[u][5], acc[u][6], acc[u][7]);
+    }
   }
 }
 
@@ -423,17 +437,17 @@ struct BwdShape {
   int warps, grid;
 };
 
-constexpr int64_t kRingMaxH = 8192;  // 1024 threads of eight columns
+constexpr int64_t kRingMaxH = 8192;  // 16 warps of two chunks
 
-int backward_warps(int64_t H) {
+// Two chunks a warp and sixteen warps an SM (16,384 x 4096 BF16: 93 us; eight warps leave the loads
+// waiting, 128 us, 24 and more gain nothing, 96 to 122 us), but for 16-bit rows on odd boundaries, whose
+// loads of single elements want warps rather than registers: one chunk and 32 (6007 x 2503: 53 us
+// against 75).  Rows of more than 8192 columns take four chunks a warp.
+BwdShape backward_shape(int64_t T, int64_t H, bool single) {
   const int chunks = static_cast<int>((H + 255) / 256);
-  return H <= kRingMaxH ? chunks : (chunks + 3) / 4;
-}
-
-BwdShape backward_shape(int64_t T, int64_t H) {
   BwdShape s;
-  s.warps = backward_warps(H);
-  const int per_sm = std::max(1, std::min(16, 32 / s.warps));
+  s.warps = H > kRingMaxH ? (chunks + 3) / 4 : single ? chunks : (chunks + 1) / 2;
+  const int per_sm = std::max(1, std::min(16, (single ? 32 : 16) / s.warps));
   s.grid = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(T, int64_t(sm_count()) * per_sm)));
   return s;
 }
@@ -442,7 +456,7 @@ template <typename T>
 int launch_norm_backward(const NormBwd& a, const BwdShape& s, bool wide, cudaStream_t st) {
   if (wide && a.H <= kRingMaxH) {
     const int64_t row = a.H * static_cast<int64_t>(sizeof(T)) * (a.dh ? 3 : 2);
-    const int per_sm = std::max(1, std::min(16, 32 / s.warps));
+    const int per_sm = std::max(1, std::min(16, 16 / s.warps));
     const int slots = static_cast<int>(std::max<int64_t>(2, std::min<int64_t>(kRingMax, 200 * 1024 / per_sm / row)));
     static std::once_flag flags[kMaxDevices];
     int dev = 0;
@@ -454,8 +468,10 @@ int launch_norm_backward(const NormBwd& a, const BwdShape& s, bool wide, cudaStr
     rms_norm_backward_ring_kernel<T><<<s.grid, s.warps * 32, slots * row, st>>>(a, slots);
     return launched();
   }
-  if (a.H <= kRingMaxH)
+  if (a.H <= kRingMaxH && sizeof(T) == 2)
     rms_norm_backward_kernel<T, false, 1, 1024><<<s.grid, s.warps * 32, 0, st>>>(a);
+  else if (a.H <= kRingMaxH)
+    rms_norm_backward_kernel<T, false, 2, 512><<<s.grid, s.warps * 32, 0, st>>>(a);
   else if (wide)
     rms_norm_backward_kernel<T, true, 4, 1024><<<s.grid, s.warps * 32, 0, st>>>(a);
   else
@@ -496,7 +512,9 @@ int cdg_add_rms_norm(const cdg_norm_args* g, cdg_stream_t stream) {
 
 size_t cdg_rms_norm_backward_workspace_bytes(int64_t T, int64_t H) {
   if (T < 0 || H <= 0 || H > cdg::kNormMaxH) return 0;
-  return static_cast<size_t>(cdg::backward_shape(T, H).grid) * H * sizeof(float);
+  // whichever form the rows' type and boundaries select
+  return static_cast<size_t>(std::max(cdg::backward_shape(T, H, false).grid, cdg::backward_shape(T, H, true).grid)) * H *
+         sizeof(float);
 }
 
 int cdg_rms_norm_backward(const cdg_norm_backward_args* g, void* workspace, size_t workspace_bytes,
@@ -515,7 +533,7 @@ int cdg_rms_norm_backward(const cdg_norm_backward_args* g, void* workspace, size
   const bool wide = g->H % 8 == 0 && wide_rows(a.dy, a.dy_stride, e) && wide_rows(a.h, a.h_stride, e) &&
                     wide_rows(a.dh, a.dh_stride, e) && wide_rows(a.dx, a.dx_stride, e) && wide_rows(a.w, 0, e);
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  const BwdShape s = backward_shape(g->T, g->H);
+  const BwdShape s = backward_shape(g->T, g->H, !wide && e == 2);
   int rc;
   if (g->dtype == CDG_DTYPE_BF16)
     rc = launch_norm_backward<__nv_bfloat16>(a, s, wide, st);
