@@ -83,6 +83,7 @@ __global__ void __launch_bounds__(256) linear_dz_kernel(const T* dy, int64_t dy_
                                                         int act, int64_t M, int64_t N, T* dz, int64_t dz_stride,
                                                         float* partial) {
   __shared__ float sums[8][256];
+  grid_dependency_wait();
   grid_launch_dependents();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int64_t chunk = blockIdx.x;
@@ -176,7 +177,7 @@ size_t repack_bytes(const Matrix& m) {
 }
 
 // Replaces the operands that TMA cannot load (b may be NULL) by copies in the workspace.
-int repack(Matrix* a, Matrix* b, uint8_t*& ws, cudaStream_t st, bool& after) {
+int repack(Matrix* a, Matrix* b, uint8_t*& ws, cudaStream_t st) {
   Repack todo[2];
   int n = 0;
   int64_t most = 0;
@@ -192,11 +193,7 @@ int repack(Matrix* a, Matrix* b, uint8_t*& ws, cudaStream_t st, bool& after) {
   }
   if (n == 0 || most == 0) return CDG_OK;
   const dim3 grid(static_cast<unsigned>(std::min<int64_t>((most + 7) / 8, int64_t(sm_count()) * 16)), n);
-  const Repack& second = n == 2 ? todo[1] : todo[0];
-  if (after) return launch_after(repack_rows_kernel, grid, 256, 0, st, todo[0], second);
-  repack_rows_kernel<<<grid, 256, 0, st>>>(todo[0], second);
-  after = true;
-  return launched();
+  return launch(repack_rows_kernel, grid, 256, 0, st, todo[0], n == 2 ? todo[1] : todo[0]);
 }
 
 // Boxes of 128 bytes x box_rows in the 128-byte swizzle.
@@ -221,7 +218,7 @@ int make_map(CUtensorMap* map, const Matrix& m, int dtype, uint32_t box_rows) {
 
 template <typename T, typename O, int BN, bool SWAP>
 int launch_tiles(const CUtensorMap& ta, const CUtensorMap& tb, LinearShape s, const Epilogue& e, int splits,
-                 cudaStream_t st, bool after) {
+                 cudaStream_t st) {
   constexpr bool PROMOTE = sizeof(O) == 4;
   using L = TileSmem<BN, PROMOTE>;
   const int64_t ctas = int64_t(s.m_tiles) * s.n_tiles * splits;
@@ -235,10 +232,10 @@ int launch_tiles(const CUtensorMap& ta, const CUtensorMap& tb, LinearShape s, co
   at[0].id = cudaLaunchAttributeClusterDimension;
   at[0].val.clusterDim.x = splits;
   at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
-  at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;  // as launch_after
+  at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;  // as launch()
   at[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = at;
-  cfg.numAttrs = after && cdg_get_pdl() ? 2 : 1;
+  cfg.numAttrs = cdg_get_pdl() ? 2 : 1;
   return cudaLaunchKernelEx(&cfg, cdg_linear_tile_kernel<T, O, BN, PROMOTE, SWAP>, ta, tb, s, e, splits) == cudaSuccess
              ? CDG_OK
              : CDG_ERR_CUDA;
@@ -246,7 +243,7 @@ int launch_tiles(const CUtensorMap& ta, const CUtensorMap& tb, LinearShape s, co
 
 template <typename T, typename O, int BN>
 int launch_pairs(const Matrix& A, const Matrix& B, const LinearShape& s, Epilogue e, int64_t M, int64_t N,
-                 cudaStream_t st, bool after) {
+                 cudaStream_t st) {
   constexpr int kType = std::is_same<T, __nv_bfloat16>::value ? CDG_DTYPE_BF16 : CDG_DTYPE_F16;
   constexpr int kOut = sizeof(O) == 4 ? CDG_DTYPE_F32 : kType;
   CUtensorMap ta{}, tb{}, ty{}, tr{};
@@ -262,12 +259,8 @@ int launch_pairs(const Matrix& A, const Matrix& B, const LinearShape& s, Epilogu
   if (rc != CDG_OK) return rc;
   const unsigned grid =
       static_cast<unsigned>(2 * std::min<int64_t>(int64_t(s.m_tiles) * s.n_tiles, std::max(1, sm_count() / 2)));
-  if (after)
-    return launch_after(cdg_linear_pair_kernel<T, O, BN>, dim3(grid), PairTileSmem<BN>::kThreads, PairTileSmem<BN>::kBytes, st,
-                        ta, tb, ty, tr, s, e);
-  cdg_linear_pair_kernel<T, O, BN>
-      <<<grid, PairTileSmem<BN>::kThreads, PairTileSmem<BN>::kBytes, st>>>(ta, tb, ty, tr, s, e);
-  return launched();
+  return launch(cdg_linear_pair_kernel<T, O, BN>, dim3(grid), PairTileSmem<BN>::kThreads, PairTileSmem<BN>::kBytes, st, ta, tb,
+                ty, tr, s, e);
 }
 
 // How a product is cut: pairs (256 x 256 tiles), tiles (128 x 64 or 128 x 128, K split or not), or
@@ -318,7 +311,7 @@ Plan make_plan(int64_t M, int64_t N, int64_t k_steps, int sms) {
 // [K, N], else [N, K].  Rows of both on 16-byte boundaries.
 template <typename T, typename O>
 int product(const Matrix& A, bool a_mn, const Matrix& B, bool b_mn, int64_t M, int64_t N, int64_t K,
-            const Epilogue& e, cudaStream_t st, bool after) {
+            const Epilogue& e, cudaStream_t st) {
   constexpr int kType = std::is_same<T, __nv_bfloat16>::value ? CDG_DTYPE_BF16 : CDG_DTYPE_F16;
   if (M == 0 || N == 0) return CDG_OK;
   LinearShape s{};
@@ -340,7 +333,7 @@ int product(const Matrix& A, bool a_mn, const Matrix& B, bool b_mn, int64_t M, i
   if (m_tiles * n_tiles * 8 > 0x7fffffff) return CDG_ERR_UNSUPPORTED;
   s.m_tiles = static_cast<int>(m_tiles);
   s.n_tiles = static_cast<int>(n_tiles);
-  if (p.kind == Plan::kPairs) return launch_pairs<T, O, 256>(A, B, s, e, M, N, st, after);
+  if (p.kind == Plan::kPairs) return launch_pairs<T, O, 256>(A, B, s, e, M, N, st);
   CUtensorMap ta{}, tb{};
   if (p.kind == Plan::kSwapped) {
     std::swap(s.M, s.N);
@@ -352,16 +345,16 @@ int product(const Matrix& A, bool a_mn, const Matrix& B, bool b_mn, int64_t M, i
       if (rc == CDG_OK) rc = make_map(&tb, A, kType, p.bn);
       if (rc != CDG_OK) return rc;
     }
-    return p.bn == 16 ? launch_tiles<T, O, 16, true>(ta, tb, s, e, p.splits, st, after)
-                      : launch_tiles<T, O, 32, true>(ta, tb, s, e, p.splits, st, after);
+    return p.bn == 16 ? launch_tiles<T, O, 16, true>(ta, tb, s, e, p.splits, st)
+                      : launch_tiles<T, O, 32, true>(ta, tb, s, e, p.splits, st);
   }
   if (K > 0) {
     int rc = make_map(&ta, A, kType, a_mn ? 64 : s.a_rows);
     if (rc == CDG_OK) rc = make_map(&tb, B, kType, b_mn ? 64 : p.bn);
     if (rc != CDG_OK) return rc;
   }
-  return p.bn == 128 ? launch_tiles<T, O, 128, false>(ta, tb, s, e, p.splits, st, after)
-                     : launch_tiles<T, O, 64, false>(ta, tb, s, e, p.splits, st, after);
+  return p.bn == 128 ? launch_tiles<T, O, 128, false>(ta, tb, s, e, p.splits, st)
+                     : launch_tiles<T, O, 64, false>(ta, tb, s, e, p.splits, st);
 }
 
 bool operand_dtype(int dtype) { return dtype == CDG_DTYPE_BF16 || dtype == CDG_DTYPE_F16; }
@@ -377,9 +370,8 @@ template <typename T>
 int forward(const cdg_linear_args* g, uint8_t* ws, cudaStream_t st) {
   Matrix x{g->x, g->x_stride, g->M, g->K}, w{g->w, g->w_stride, g->N, g->K};
   int rc = CDG_OK;
-  bool after = false;  // whether this call has launched a kernel already
   if (g->K > 0) {
-    rc = repack(&x, &w, ws, st, after);
+    rc = repack(&x, &w, ws, st);
     if (rc != CDG_OK) return rc;
   }
   Epilogue e{};
@@ -396,8 +388,8 @@ int forward(const cdg_linear_args* g, uint8_t* ws, cudaStream_t st) {
   e.wide_bias = e.bias && !e.bias_f32 && reinterpret_cast<uintptr_t>(e.bias) % 16 == 0;
   e.wide = wide_columns(e.y, e.y_stride, element_size(g->out_dtype)) && wide_columns(e.z, e.z_stride, 2) &&
            wide_columns(e.residual, e.residual_stride, e.residual_f32 ? 4 : 2);
-  return g->out_dtype == CDG_DTYPE_F32 ? product<T, float>(x, false, w, false, g->M, g->N, g->K, e, st, after)
-                                       : product<T, T>(x, false, w, false, g->M, g->N, g->K, e, st, after);
+  return g->out_dtype == CDG_DTYPE_F32 ? product<T, float>(x, false, w, false, g->M, g->N, g->K, e, st)
+                                       : product<T, T>(x, false, w, false, g->M, g->N, g->K, e, st);
 }
 
 // Row groups of the elementwise backward pass: a few CTAs per SM, each summing many rows.
@@ -417,7 +409,6 @@ template <typename T>
 int backward(const cdg_linear_backward_args* g, uint8_t* ws, cudaStream_t st) {
   Matrix x{g->x, g->x_stride, g->M, g->K}, w{g->w, g->w_stride, g->N, g->K};
   Matrix dz{g->dy, g->dy_stride, g->M, g->N};
-  bool after = false;  // whether this call has launched a kernel already
   const bool store = needs_dz(g) && (g->dx || g->dw);
   if ((store || g->db) && g->M > 0) {
     T* out = nullptr;
@@ -435,20 +426,14 @@ int backward(const cdg_linear_backward_args* g, uint8_t* ws, cudaStream_t st) {
     const T* z = g->activation != CDG_ACT_NONE ? static_cast<const T*>(g->z) : nullptr;
     const bool wide = g->N % 8 == 0 && wide_rows(g->dy, g->dy_stride, 2) && (!z || wide_rows(z, g->z_stride, 2));
     const dim3 grid(static_cast<unsigned>((g->N + 255) / 256), static_cast<unsigned>(groups));
-    if (wide)
-      linear_dz_kernel<T, true><<<grid, 256, 0, st>>>(static_cast<const T*>(g->dy), g->dy_stride, z, g->z_stride,
-                                                      g->activation, g->M, g->N, out, stride, partial);
-    else
-      linear_dz_kernel<T, false><<<grid, 256, 0, st>>>(static_cast<const T*>(g->dy), g->dy_stride, z, g->z_stride,
-                                                       g->activation, g->M, g->N, out, stride, partial);
-    int rc = launched();
+    int rc = launch(wide ? linear_dz_kernel<T, true> : linear_dz_kernel<T, false>, grid, 256, 0, st, static_cast<const T*>(g->dy),
+                    g->dy_stride, z, g->z_stride, g->activation, g->M, g->N, out, stride, partial);
     if (rc != CDG_OK) return rc;
-    after = true;
     if (g->db) {
       const unsigned blocks = static_cast<unsigned>((g->N + 31) / 32);
       rc = g->db_dtype == CDG_DTYPE_F32
-               ? launch_after(column_sum_kernel<float>, dim3(blocks), 1024, 0, st, partial, groups, g->N, static_cast<float*>(g->db))
-               : launch_after(column_sum_kernel<T>, dim3(blocks), 1024, 0, st, partial, groups, g->N, static_cast<T*>(g->db));
+               ? launch(column_sum_kernel<float>, dim3(blocks), 1024, 0, st, partial, groups, g->N, static_cast<float*>(g->db))
+               : launch(column_sum_kernel<T>, dim3(blocks), 1024, 0, st, partial, groups, g->N, static_cast<T*>(g->db));
       if (rc != CDG_OK) return rc;
     }
     if (store) {
@@ -459,22 +444,21 @@ int backward(const cdg_linear_backward_args* g, uint8_t* ws, cudaStream_t st) {
     if (cudaMemsetAsync(g->db, 0, g->N * element_size(g->db_dtype), st) != cudaSuccess) return CDG_ERR_CUDA;
   }
   if (g->dx) {
-    int rc = g->N > 0 && g->M > 0 ? repack(&w, nullptr, ws, st, after) : CDG_OK;
+    int rc = g->N > 0 && g->M > 0 ? repack(&w, nullptr, ws, st) : CDG_OK;
     Epilogue e{};
     e.y = g->dx;
     e.y_stride = g->dx_stride;
     e.wide = wide_columns(e.y, e.y_stride, 2);
-    if (rc == CDG_OK) rc = product<T, T>(dz, false, w, true, g->M, g->K, g->N, e, st, after);
-    after = after || (g->M > 0 && g->K > 0);
+    if (rc == CDG_OK) rc = product<T, T>(dz, false, w, true, g->M, g->K, g->N, e, st);
     if (rc != CDG_OK) return rc;
   }
   if (g->dw) {
-    int rc = g->M > 0 ? repack(&x, nullptr, ws, st, after) : CDG_OK;
+    int rc = g->M > 0 ? repack(&x, nullptr, ws, st) : CDG_OK;
     Epilogue e{};
     e.y = g->dw;
     e.y_stride = g->dw_stride;
     e.wide = wide_columns(e.y, e.y_stride, 2);
-    if (rc == CDG_OK) rc = product<T, T>(dz, true, x, true, g->N, g->K, g->M, e, st, after);
+    if (rc == CDG_OK) rc = product<T, T>(dz, true, x, true, g->N, g->K, g->M, e, st);
     if (rc != CDG_OK) return rc;
   }
   return CDG_OK;

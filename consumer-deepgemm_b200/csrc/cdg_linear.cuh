@@ -10,6 +10,8 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <type_traits>
+
 #include "cdg_ptx.cuh"
 #include "cdg_rows.cuh"
 
@@ -425,8 +427,10 @@ __global__ void __launch_bounds__(kThreadsOf<SWAP>)
   const int sums = PROMOTE ? (k_last - k_first + kPromoteSteps - 1) / kPromoteSteps : (k_last > k_first ? 1 : 0);
 
   if (warp == 4 && lane == 0) {
-    prefetch_tmap(&tmap_a);
-    prefetch_tmap(&tmap_b);
+    if (s.k_steps > 0) {  // K = 0 has no operands and no maps
+      prefetch_tmap(&tmap_a);
+      prefetch_tmap(&tmap_b);
+    }
     for (int i = 0; i < S; ++i) {
       mbar_init(&full[i], 1);
       mbar_init(&empty[i], 1);
@@ -610,29 +614,37 @@ __global__ void __launch_bounds__(kThreadsOf<SWAP>)
   };
   if constexpr (SWAP) {
     // rows of the weight run along y: a thread keeps one of this CTA's and takes columns, two at a time
-    // (one, mostly, where K is split; eight at a time cost 1.4 us of predicated work)
+    // where K is split (it mostly has one; eight cost 1.4 us of predicated work), else eight, so that
+    // their residual loads are in flight together
     const int row = row0 + t % share, lanes = kTileThreads / share;
     const int64_t n = m0 + row;
-    if (n < s.M && t < lanes * share) {
+    auto columns = [&](auto width) {
+      constexpr int U = decltype(width)::value;
       const float bias = e.bias ? load_any<T>(e.bias, n, e.bias_f32) : 0.0f;
-      for (int c = t / share; c < cols; c += lanes * 2) {
-        float v[2], r[2];
+      for (int c = t / share; c < cols; c += lanes * U) {
+        float v[U], r[U];
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
+        for (int j = 0; j < U; ++j) {
           const int col = c + j * lanes;
           r[j] = e.residual && col < cols ? load_any<T>(e.residual, (n0 + col) * e.residual_stride + n, e.residual_f32) : 0.0f;
           v[j] = bias + (col < cols ? total(part + col * kPartStride + row) : 0.0f);
         }
         if (e.z) {
 #pragma unroll
-          for (int j = 0; j < 2; ++j)
+          for (int j = 0; j < U; ++j)
             if (c + j * lanes < cols) static_cast<T*>(e.z)[(n0 + c + j * lanes) * e.z_stride + n] = from_f<T>(v[j]);
         }
-        activate_all<2>(v, e.act);
+        activate_all<U>(v, e.act);
 #pragma unroll
-        for (int j = 0; j < 2; ++j)
+        for (int j = 0; j < U; ++j)
           if (c + j * lanes < cols) static_cast<O*>(e.y)[(n0 + c + j * lanes) * e.y_stride + n] = from_f<O>(v[j] + r[j]);
       }
+    };
+    if (n < s.M && t < lanes * share) {
+      if (splits == 1)
+        columns(std::integral_constant<int, 8>());
+      else
+        columns(std::integral_constant<int, 2>());
     }
   } else if (e.wide && splits > 1) {
     // consecutive threads take consecutive rows, so that remote reads are contiguous

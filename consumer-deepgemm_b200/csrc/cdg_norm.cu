@@ -136,6 +136,8 @@ __device__ __forceinline__ void quant_chunk(const NormFwd& a, int64_t row, int64
 template <typename T, bool WIDE, int ITER, int THREADS>
 __global__ void __launch_bounds__(THREADS) add_rms_norm_kernel(const NormFwd a, int warps_per_row) {
   __shared__ float slot[32];
+  grid_dependency_wait();
+  grid_launch_dependents();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   int64_t row = blockIdx.x;
   int w = warp;
@@ -207,7 +209,8 @@ struct NormBwd {
 template <typename T, bool WIDE, int ITER, int THREADS>
 __global__ void __launch_bounds__(THREADS) rms_norm_backward_kernel(const NormBwd a) {
   __shared__ float2 slot[2][32];
-  grid_launch_dependents();  // the sum over the CTAs' weight gradients
+  grid_dependency_wait();
+  grid_launch_dependents();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
   const T* dy = static_cast<const T*>(a.dy);
   const T* h = static_cast<const T*>(a.h);
@@ -306,7 +309,8 @@ __global__ void __launch_bounds__(512) rms_norm_backward_ring_kernel(const NormB
   extern __shared__ __align__(128) uint8_t ring[];
   __shared__ float2 slot_sum[2][32];
   __shared__ __align__(8) uint64_t full[kRingMax];
-  grid_launch_dependents();  // the sum over the CTAs' weight gradients
+  grid_dependency_wait();
+  grid_launch_dependents();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
   const uint32_t row_bytes = static_cast<uint32_t>(a.H * sizeof(T));
   const int arrays = a.dh ? 3 : 2;
@@ -427,8 +431,7 @@ int launch_norm(const NormFwd& a, cudaStream_t st) {
   auto kernel = iter == 1   ? add_rms_norm_kernel<T, WIDE, 1, 1024>
                 : iter == 2 ? add_rms_norm_kernel<T, WIDE, 2, 1024>
                             : add_rms_norm_kernel<T, WIDE, 4, 1024>;
-  kernel<<<grid, warps * rows * 32, 0, st>>>(a, warps);
-  return launched();
+  return launch(kernel, dim3(grid), warps * rows * 32, 0, st, a, warps);
 }
 
 // CTAs of the backward kernels: every SM filled, each CTA taking several rows where there are
@@ -465,18 +468,12 @@ int launch_norm_backward(const NormBwd& a, const BwdShape& s, bool wide, cudaStr
       (void)cudaFuncSetAttribute(rms_norm_backward_ring_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                  200 * 1024);
     });
-    rms_norm_backward_ring_kernel<T><<<s.grid, s.warps * 32, slots * row, st>>>(a, slots);
-    return launched();
+    return launch(rms_norm_backward_ring_kernel<T>, dim3(s.grid), s.warps * 32, slots * row, st, a, slots);
   }
-  if (a.H <= kRingMaxH && sizeof(T) == 2)
-    rms_norm_backward_kernel<T, false, 1, 1024><<<s.grid, s.warps * 32, 0, st>>>(a);
-  else if (a.H <= kRingMaxH)
-    rms_norm_backward_kernel<T, false, 2, 512><<<s.grid, s.warps * 32, 0, st>>>(a);
-  else if (wide)
-    rms_norm_backward_kernel<T, true, 4, 1024><<<s.grid, s.warps * 32, 0, st>>>(a);
-  else
-    rms_norm_backward_kernel<T, false, 4, 1024><<<s.grid, s.warps * 32, 0, st>>>(a);
-  return launched();
+  auto kernel = a.H > kRingMaxH    ? (wide ? rms_norm_backward_kernel<T, true, 4, 1024> : rms_norm_backward_kernel<T, false, 4, 1024>)
+                : sizeof(T) == 2 ? rms_norm_backward_kernel<T, false, 1, 1024>
+                                 : rms_norm_backward_kernel<T, false, 2, 512>;
+  return launch(kernel, dim3(s.grid), s.warps * 32, 0, st, a);
 }
 
 }  // namespace
@@ -544,10 +541,10 @@ int cdg_rms_norm_backward(const cdg_norm_backward_args* g, void* workspace, size
   if (rc != CDG_OK) return rc;
   const unsigned grid = static_cast<unsigned>((g->H + 31) / 32);
   if (g->w_dtype == CDG_DTYPE_BF16)
-    return launch_after(column_sum_kernel<__nv_bfloat16>, dim3(grid), 1024, 0, st, a.partial, s.grid, g->H, static_cast<__nv_bfloat16*>(g->dw));
+    return launch(column_sum_kernel<__nv_bfloat16>, dim3(grid), 1024, 0, st, a.partial, s.grid, g->H, static_cast<__nv_bfloat16*>(g->dw));
   if (g->w_dtype == CDG_DTYPE_F16)
-    return launch_after(column_sum_kernel<__half>, dim3(grid), 1024, 0, st, a.partial, s.grid, g->H, static_cast<__half*>(g->dw));
-  return launch_after(column_sum_kernel<float>, dim3(grid), 1024, 0, st, a.partial, s.grid, g->H, static_cast<float*>(g->dw));
+    return launch(column_sum_kernel<__half>, dim3(grid), 1024, 0, st, a.partial, s.grid, g->H, static_cast<__half*>(g->dw));
+  return launch(column_sum_kernel<float>, dim3(grid), 1024, 0, st, a.partial, s.grid, g->H, static_cast<float*>(g->dw));
 }
 
 }  // extern "C"

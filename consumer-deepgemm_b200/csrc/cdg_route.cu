@@ -19,6 +19,7 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <atomic>
 #include <cfloat>
 #include <cstdint>
 
@@ -189,6 +190,8 @@ __global__ void __launch_bounds__(WARPS * 32) moe_route_kernel(const Route a) {
   for (int e = threadIdx.x; e < a.E; e += blockDim.x) s_counts[e] = 0;
   if (threadIdx.x == 0) s_tokens = 0;
   __syncthreads();
+  grid_dependency_wait();
+  grid_launch_dependents();
 
   const T* logits = static_cast<const T*>(a.logits);
   float psum[N];
@@ -354,6 +357,8 @@ __global__ void __launch_bounds__(WARPS * 32) moe_route_backward_kernel(const Ro
   float* sg = s_grad + warp * a.E;
   for (int e = lane; e < a.E; e += 32) sg[e] = 0.0f;
   __syncwarp();
+  grid_dependency_wait();
+  grid_launch_dependents();
   float load[N];  // a_e of the lane's experts
 #pragma unroll
   for (int i = 0; i < N; ++i) load[i] = 0.0f;
@@ -458,15 +463,15 @@ constexpr int64_t kOneCtaTokens = 64;
 constexpr int kOneCtaExperts = 256;
 bool one_cta(int64_t T, int64_t E) { return T <= kOneCtaTokens && E <= kOneCtaExperts; }
 
-// CTAs of a kernel that an SM holds at once (looked up once per device).
+// CTAs of a kernel that an SM holds at once (looked up once: the library runs on one kind of device).
 template <typename K>
-int resident_ctas(K kernel, int threads, size_t smem, int* known) {
-  if (*known == 0) {
-    int n = 0;
+int resident_ctas(K kernel, int threads, size_t smem, std::atomic<int>* known) {
+  int n = known->load(std::memory_order_relaxed);
+  if (n == 0) {
     if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kernel, threads, smem) != cudaSuccess || n < 1) n = 1;
-    *known = n;
+    known->store(n, std::memory_order_relaxed);
   }
-  return *known;
+  return n;
 }
 
 template <typename T, int N>
@@ -474,30 +479,28 @@ int launch_route(const Route& a, cudaStream_t st) {
   if constexpr (N * 32 <= kOneCtaExperts) {
     if (one_cta(a.T, a.E)) {
       const size_t smem = a.E * 4 + (a.balance ? size_t(32) * a.E * 4 : 0);
-      moe_route_kernel<T, N, 32><<<1, 1024, smem, st>>>(a);
-      return launched();
+      return launch(moe_route_kernel<T, N, 32>, dim3(1), 1024, smem, st, a);
     }
   }
   // the largest dynamic shared memory of this N, so that one look-up serves every call
-  static int known = 0;
+  static std::atomic<int> known{0};
   const int per_sm = resident_ctas(moe_route_kernel<T, N, kRouteWarps>, kRouteWarps * 32,
                                    size_t(N) * 32 * 4 * (kRouteWarps + 1), &known);
   const int64_t ctas = (a.T + kRouteWarps - 1) / kRouteWarps;
   const unsigned grid = static_cast<unsigned>(std::min<int64_t>(ctas, int64_t(sm_count()) * per_sm));
   const size_t smem = a.E * 4 + (a.balance ? size_t(kRouteWarps) * a.E * 4 : 0);
-  moe_route_kernel<T, N, kRouteWarps><<<grid, kRouteWarps * 32, smem, st>>>(a);
-  return launched();
+  return launch(moe_route_kernel<T, N, kRouteWarps>, dim3(grid), kRouteWarps * 32, smem, st, a);
 }
 
 template <typename T, int N>
 int launch_route_backward(const RouteBwd& a, cudaStream_t st) {
-  static int known = 0;
+  static std::atomic<int> known{0};
   const int per_sm = resident_ctas(moe_route_backward_kernel<T, N, kRouteWarps>, kRouteWarps * 32,
                                    size_t(N) * 32 * 4 * kRouteWarps, &known);
   const int64_t ctas = (a.T + kRouteWarps - 1) / kRouteWarps;
   const unsigned grid = static_cast<unsigned>(std::min<int64_t>(ctas, int64_t(sm_count()) * per_sm));
-  moe_route_backward_kernel<T, N, kRouteWarps><<<grid, kRouteWarps * 32, size_t(kRouteWarps) * a.E * 4, st>>>(a);
-  return launched();
+  return launch(moe_route_backward_kernel<T, N, kRouteWarps>, dim3(grid), kRouteWarps * 32, size_t(kRouteWarps) * a.E * 4, st,
+                a);
 }
 
 template <typename T>

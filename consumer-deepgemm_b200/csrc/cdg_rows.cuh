@@ -171,13 +171,12 @@ __global__ void __launch_bounds__(1024) column_sum_kernel(const float* partial, 
 }
 
 // ------------------------------------------------------------------ host
-inline int launched() { return cudaGetLastError() == cudaSuccess ? CDG_OK : CDG_ERR_CUDA; }
-
-// Launch of a call's second or later kernel: scheduled while its predecessor drains (unless
-// cdg_set_pdl(0)); the kernel itself waits for the predecessor's end (griddepcontrol.wait) before it
-// touches global memory.
+// Launch with programmatic stream serialization (unless cdg_set_pdl(0)): the kernel may be scheduled
+// while its predecessor on the stream, of this call or of another, drains; it waits for the
+// predecessor's end (griddepcontrol.wait) before it touches global memory.  Calls of a few
+// microseconds in a row lose about one less between them.
 template <typename... K, typename... A>
-inline int launch_after(void (*kernel)(K...), dim3 grid, unsigned block, size_t smem, cudaStream_t st, A&&... args) {
+inline int launch(void (*kernel)(K...), dim3 grid, unsigned block, size_t smem, cudaStream_t st, A&&... args) {
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = grid;
   cfg.blockDim = dim3(block);

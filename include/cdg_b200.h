@@ -223,8 +223,8 @@ int cdg_device_status(int32_t clear, int32_t* where);
 int cdg_set_num_sms(int32_t num_sms);
 int cdg_get_num_sms(void);
 
-/* Whether the GEMM's kernels after the first are launched with programmatic stream
- * serialization (1, the default: each may be scheduled while its predecessor drains and
+/* Whether the GEMM's kernels after the first, and every kernel of the norm, the router and the dense
+ * product, are launched with programmatic stream serialization (1, the default: each may be scheduled while its predecessor drains and
  * waits for it on the device) or as plain stream-ordered launches (0).  Process-wide.
  * Replaces set_pdl / get_pdl (consumer_deep_gemm/utils.py:44-50), stored there unused. */
 int cdg_set_pdl(int32_t enable);
