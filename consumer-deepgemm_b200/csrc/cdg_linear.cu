@@ -264,37 +264,45 @@ int launch_pairs(const Matrix& A, const Matrix& B, const LinearShape& s, Epilogu
 }
 
 // How a product is cut: pairs (256 x 256 tiles), tiles (128 x 64 or 128 x 128, K split or not), or
-// swapped tiles (up to 32 rows of x).  The costs are microseconds, fitted to the GPU times of 11
-// shapes under every cut, from 64 x 4096 x 4096 to 16,384 x 64 x 1024 (one B200, launch apart).  What
-// they decide, for instance: 64 x 4096 x 4096 pairs 25.8, 128 x 64 in 4 parts 13.8 us; 1024 x 2048 x
-// 2048 pairs 17.1, 128 x 64 16.7, 128 x 128 in 2 parts 18.0 us; 300 x 8192 x 512 pairs 10.4, 128 x 128
-// 12.5 us; 3000 x 3000 x 256 pairs 12.5, 128 x 128 22.3 us.
+// swapped tiles (up to 32 rows of x).  The costs are microseconds, fitted to the GPU times of 24
+// shapes under every cut, from 64 x 512 x 512 to 16,384 x 64 x 1024 (one B200, calls in a row).  What they
+// decide, for instance: 128 x 4096 x 4096 pairs 26.2, 128 x 64 in 2 parts 14.0 us; 1024 x 2048 x 2048 pairs
+// 16.8, 128 x 128 13.7, 128 x 64 15.2 us; 300 x 8192 x 512 pairs 9.9, 128 x 64 12.9 us; 3000 x 3000 x 256
+// pairs 12.0, 128 x 128 16.9 us; 2910 x 94 x 192 128 x 64 7.8, 128 x 128 11.8 us.
 struct Plan {
   enum Kind { kPairs, kTiles, kSwapped } kind;
   int bn, splits;
 };
 
-Plan make_plan(int64_t M, int64_t N, int64_t k_steps, int sms) {
+// Whether K may go to clusters of `parts` CTAs: two CTAs per SM, but clusters of eight, which few SMs
+// can hold at the same time, on half the SMs only (1 x 256 x 4096 in 4 parts 7.2, in 8 5.2 us;
+// 8 x 2048 x 8192 in 4 parts 12.0, in 8, 128 CTAs, 16.8 us).
+bool may_split(int64_t ctas, int parts, int sms) {
+  return parts <= 4 ? ctas <= 2 * sms : parts == 8 && ctas <= sms / 2;
+}
+
+Plan make_plan(int64_t M, int64_t N, int64_t k_steps, bool narrow, int sms) {
   if (M <= 32) {
     Plan p{Plan::kSwapped, M <= 16 ? 16 : 32, 1};
     const int64_t tiles = (N + 127) / 128;
-    // two CTAs per SM and at least four K steps each
-    while (p.splits < 8 && tiles * p.splits * 2 <= 2 * sms && k_steps / (p.splits * 2) >= 4) p.splits *= 2;
+    while (may_split(tiles * p.splits * 2, p.splits * 2, sms) && k_steps / (p.splits * 2) >= 4) p.splits *= 2;
     return p;
   }
-  Plan best{Plan::kTiles, 128, 1};
+  Plan best{Plan::kTiles, 64, 1};
   double least = 1e300;
   for (int bn : {64, 128}) {
     for (int s = 1; s <= 8; s *= 2) {
       const int64_t ctas = (M + 127) / 128 * ((N + bn - 1) / bn) * s;
-      if (s > 1 && (ctas > 2 * sms || k_steps / s < 4)) break;
+      if (s > 1 && (!may_split(ctas, s, sms) || k_steps / s < 2)) break;
       const double steps = static_cast<double>((k_steps + s - 1) / s);
+      const double waves = static_cast<double>((ctas + 2 * sms - 1) / (2 * sms));
       double cost;
       if (ctas <= sms)  // a CTA has its SM alone
-        cost = bn == 64 ? 5.5 + 0.22 * steps : 4.9 + 0.29 * steps + (s > 1 ? 0.5 * s : 0.0);
+        cost = bn == 64 ? 4.0 + 0.235 * steps : 4.9 + 0.245 * steps;
       else
-        cost = static_cast<double>((ctas + 2 * sms - 1) / (2 * sms)) *
-               (bn == 64 ? 7.5 + 0.2 * steps + (s > 1 ? 1.5 : 0.0) : 7.0 + 0.4 * steps + (s > 1 ? 1.0 + 0.6 * s : 0.0));
+        cost = 1.0 + waves * (bn == 64 ? 4.7 + 0.3 * steps : 6.5 + 0.41 * steps);
+      if (s > 1) cost += (bn == 64 ? 0.8 : 2.5) + 0.2 * s + (ctas > sms ? 1.0 : 0.0);
+      if (narrow) cost += waves * (bn == 64 ? 3.0 : 6.0);
       if (cost < least) {
         least = cost;
         best = Plan{Plan::kTiles, bn, s};
@@ -303,7 +311,8 @@ Plan make_plan(int64_t M, int64_t N, int64_t k_steps, int sms) {
   }
   const int64_t pairs = std::max(1, sms / 2), pair_tiles = (M + 255) / 256 * ((N + 255) / 256);
   const double waves = static_cast<double>((pair_tiles + pairs - 1) / pairs);
-  if (k_steps > 0 && waves * (0.28 * static_cast<double>(k_steps) + 0.8) + 4.8 < least) best.kind = Plan::kPairs;
+  if (k_steps > 0 && 4.0 + waves * (2.6 + 0.293 * static_cast<double>(k_steps) + (narrow ? 4.0 : 0.0)) < least)
+    best.kind = Plan::kPairs;
   return best;
 }
 
@@ -322,7 +331,7 @@ int product(const Matrix& A, bool a_mn, const Matrix& B, bool b_mn, int64_t M, i
   s.b_mn = b_mn;
   s.bf16 = kType == CDG_DTYPE_BF16;
   s.a_rows = static_cast<int>(std::min<int64_t>(128, (M + 7) / 8 * 8));
-  Plan p = make_plan(M, N, s.k_steps, sm_count());
+  Plan p = make_plan(M, N, s.k_steps, !e.wide, sm_count());
   if (p.kind == Plan::kSwapped && a_mn) {  // x's place is loaded in boxes of 16 to 64 rows, K-major
     p.kind = Plan::kTiles;
     p.bn = 64;
