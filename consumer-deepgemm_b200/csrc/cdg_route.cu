@@ -12,8 +12,11 @@
 //   softmax: dl_i = p_i (d_i - sum_j d_j p_j),  d = scatter(g) + a
 //   sigmoid: dl_i = (scatter(g)_i + (a_i - sum_j a_j p_j) / S) s_i (1 - s_i),  S = sum s
 //
-// A warp takes a row, lane l the experts l, l + 32, ...; a row is read once and its next row's
-// loads are in flight meanwhile.  Bound by instructions rather than memory: the choice.
+// Sixteen lanes take a row (32 where the choice is long or the experts are many), lane l the experts l,
+// l + 16, ...; a row is read once and its next row's loads are in flight meanwhile.  Bound by
+// instructions (about 300 a row forward, most of them the choice), not by memory: one B200,
+// calls in a row, 32,768 x 256 FP32, k = 8 with the balance loss 20.8 us forward (1.7 TB/s) and 16.8 us
+// backward (4.0 TB/s); 64 x 256 4.9 us and 3.2 us.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -24,6 +27,7 @@
 #include <cstdint>
 
 #include "cdg_b200.h"
+#include "cdg_ptx.cuh"
 #include "cdg_rows.cuh"
 
 namespace cdg {
@@ -47,12 +51,6 @@ __device__ __forceinline__ float key_value(uint32_t key) {
   return __uint_as_float(key ^ (key & 0x80000000u ? 0x80000000u : 0xFFFFFFFFu));
 }
 
-__device__ __forceinline__ float warp_sum(float v) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(kAll, v, o);
-  return v;
-}
-
 // Fast exponential and division (errors of a few units in the last place): the gate's weights
 // and gradients stay within 1e-6 of the exact ones.
 __device__ __forceinline__ float exp_fast(float v) {
@@ -63,80 +61,144 @@ __device__ __forceinline__ float exp_fast(float v) {
 }
 __device__ __forceinline__ float sigmoid_fast(float v) { return __fdividef(1.0f, 1.0f + exp_fast(-v)); }
 
-// The k experts of the largest keys of a row, of equal keys the lowest first: lane j gets the j-th
-// (x its key, y the expert), or y = -1 where no key that can be chosen is left.  key[i] is that of
-// expert i * 32 + lane, mine the lane's largest.
-//
-// The k-th largest of the 32 lanes' maxima is a lower bound of the k-th largest key, and few keys
-// reach it (with 256 experts and k = 8 about ten), so: the maxima are sorted across the lanes (a
-// bitonic network) for the bound; the keys that reach it are listed, each with its expert; each lane
-// takes one of the list and counts how many of the others go before it.  A list of more than 32, or
-// a lane with more than four of them (many equal keys, or k near 32), is chosen from round by round,
-// a warp-wide maximum each; at 32,768 x 256, k = 8 that alone took the kernel 43 us.
-template <int N>
-__device__ __forceinline__ int2 choose(uint32_t (&key)[N], uint32_t mine, int k, int lane, unsigned long long* list) {
-  uint32_t top = mine;
+// Sum and maximum over the lanes of a row.
+template <int LANES>
+__device__ __forceinline__ float lanes_sum(float v) {
 #pragma unroll
-  for (int size = 2; size <= 32; size *= 2) {
+  for (int o = LANES / 2; o > 0; o >>= 1) v += __shfl_xor_sync(kAll, v, o);
+  return v;
+}
+template <int LANES>
+__device__ __forceinline__ float lanes_max(float v) {
 #pragma unroll
-    for (int j = size / 2; j > 0; j /= 2) {
-      const uint32_t other = __shfl_xor_sync(kAll, top, j);
-      top = ((lane & j) == 0) == ((lane & size) == 0) ? max(top, other) : min(top, other);  // falling order
+  for (int o = LANES / 2; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(kAll, v, o));
+  return v;
+}
+
+// Where the lane keeps the larger value in each stage of lanes_sorted, a bit per stage.
+template <int LANES>
+__device__ __forceinline__ uint32_t sort_sides(int sub) {
+  uint32_t sides = 0;
+  int stage = 0;
+#pragma unroll
+  for (int size = 2; size <= LANES; size *= 2)
+#pragma unroll
+    for (int j = size / 2; j > 0; j /= 2, ++stage)
+      if (((sub & j) == 0) == ((sub & size & (LANES - 1)) == 0)) sides |= 1u << stage;
+  return sides;
+}
+
+// One value per lane, sorted over the lanes of a row in falling order (a bitonic network).
+template <int LANES>
+__device__ __forceinline__ float lanes_sorted(float v, uint32_t sides) {
+  int stage = 0;
+#pragma unroll
+  for (int size = 2; size <= LANES; size *= 2)
+#pragma unroll
+    for (int j = size / 2; j > 0; j /= 2, ++stage) {
+      const float other = __shfl_xor_sync(kAll, v, j);
+      v = sides & (1u << stage) ? fmaxf(v, other) : fminf(v, other);
     }
-  }
-  const uint32_t bound = max(__shfl_sync(kAll, top, k - 1), kFirstKey);
+  return v;
+}
+
+constexpr int kListed = 32;   // candidates of a row that are ranked by counting
+constexpr int kPerLane = 7;   // of them, those of one lane
+struct Candidates {
+  // x the value, y the expert; a full four are compared at a time
+  alignas(16) float2 listed[kListed + 4];
+};
+
+// The k experts of the largest values of a row, of equal values the lowest expert first: lane j of the
+// row's LANES gets the j-th (x its value, y the expert), or y = -1 where no value that can be chosen is
+// left.  v[i] is that of expert i * LANES + sub (NaN and -inf cannot be chosen, +inf counts as the
+// largest finite value); most is the row's largest value and kth the k-th largest of the lanes'
+// maxima, a lower bound of the k-th largest value.  Few values reach it (with 256 experts and k = 8
+// about ten), so: they are listed, each with its expert; each lane takes one of the list and counts how
+// many of the others go before it.  A list of more than 32, a lane with more than seven of them (many
+// equal values, or k near 32) or a value of +inf is chosen from round by round, a maximum over the lanes
+// each; at 32,768 x 256, k = 8 that alone took the kernel 43 us.
+template <int N, int LANES>
+__device__ __forceinline__ float2 choose(const float (&v)[N], float most, float kth, int k, int lane, Candidates& c) {
+  const int sub = lane & (LANES - 1);
+  const float bound = fmaxf(kth, -FLT_MAX);
   int reach = 0;
 #pragma unroll
-  for (int i = 0; i < N; ++i) reach += key[i] >= bound ? 1 : 0;
-  const unsigned one = __ballot_sync(kAll, reach > 0), two = __ballot_sync(kAll, reach > 1),
-                 three = __ballot_sync(kAll, reach > 2), four = __ballot_sync(kAll, reach > 3);
-  const int count = __popc(one) + __popc(two) + __popc(three) + __popc(four);
-  int2 got = make_int2(0, -1);
-  if (count <= 32 && !__any_sync(kAll, reach > 4)) {
-    if (reach > 0) {
-      const unsigned below = (1u << lane) - 1u;
-      int place = __popc(one & below) + __popc(two & below) + __popc(three & below) + __popc(four & below);
+  for (int i = 0; i < N; ++i) reach += v[i] >= bound ? 1 : 0;
+  // the lane's place in the list: what the lanes before it have, from the bits of their counts
+  const unsigned b0 = __ballot_sync(kAll, reach & 1), b1 = __ballot_sync(kAll, reach & 2), b2 = __ballot_sync(kAll, reach & 4);
+  const unsigned row = LANES == 32 ? kAll : 0xFFFFu << (lane & 16), below = row & ((1u << lane) - 1u);
+  const int count = __popc(b0 & row) + 2 * __popc(b1 & row) + 4 * __popc(b2 & row);
+  if (!__any_sync(kAll, count > kListed || reach > kPerLane || most > FLT_MAX)) {
+    int place = __popc(b0 & below) + 2 * __popc(b1 & below) + 4 * __popc(b2 & below);
 #pragma unroll
-      for (int i = 0; i < N; ++i) {
-        // key first, then the lower expert
-        if (key[i] >= bound)
-          list[place++] = (static_cast<unsigned long long>(key[i]) << 32) | (0xFFFFFFFFu - static_cast<uint32_t>(i * 32 + lane));
+    for (int i = 0; i < N; ++i)
+      if (v[i] >= bound) c.listed[place++] = make_float2(v[i], __int_as_float(i * LANES + sub));
+    if (sub < 4) c.listed[count + sub] = make_float2(-INFINITY, 0.0f);
+    __syncwarp();
+    float2 own[kListed / LANES];
+    int before[kListed / LANES];
+#pragma unroll
+    for (int h = 0; h < kListed / LANES; ++h) {
+      before[h] = k;
+      if (h * LANES + sub < count) {
+        own[h] = c.listed[h * LANES + sub];
+        const int expert = __float_as_int(own[h].y);
+        int n = 0;
+        auto goes_before = [&](float value, float index) {
+          if (value > own[h].x || (value == own[h].x && __float_as_int(index) < expert)) ++n;
+        };
+        for (int i = 0; i < count; i += 4) {
+          const float4 two = *reinterpret_cast<const float4*>(&c.listed[i]);
+          const float4 more = *reinterpret_cast<const float4*>(&c.listed[i + 2]);
+          goes_before(two.x, two.y);
+          goes_before(two.z, two.w);
+          goes_before(more.x, more.y);
+          goes_before(more.z, more.w);
+        }
+        before[h] = n;
       }
     }
     __syncwarp();
-    const unsigned long long own = lane < count ? list[lane] : 0;
-    int before = 0;
-#pragma unroll 4
-    for (int j = 0; j < count; ++j) before += list[j] > own ? 1 : 0;
+#pragma unroll
+    for (int h = 0; h < kListed / LANES; ++h)
+      if (before[h] < k) c.listed[before[h]] = own[h];
     __syncwarp();
-    if (lane < count && before < k) list[before] = own;
-    __syncwarp();
-    if (lane < min(count, k)) {
-      const unsigned long long v = list[lane];
-      got = make_int2(static_cast<int>(v >> 32), static_cast<int>(0xFFFFFFFFu - static_cast<uint32_t>(v)));
-    }
+    const float2 got = sub < min(count, k) ? c.listed[sub] : make_float2(0.0f, __int_as_float(-1));
     __syncwarp();
     return got;
   }
+  float2 got = make_float2(0.0f, __int_as_float(-1));
+  uint32_t key[N], mine = 0;
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    key[i] = order_key(clean_logit(v[i]));
+    mine = max(mine, key[i]);
+  }
   for (int j = 0; j < k; ++j) {
-    const uint32_t best = __reduce_max_sync(kAll, mine);
-    if (best < kFirstKey) break;
-    int e = 0x7fffffff;
-    if (mine == best) {
+    uint32_t best = mine;
+#pragma unroll
+    for (int o = LANES / 2; o > 0; o >>= 1) best = max(best, __shfl_xor_sync(kAll, best, o));
+    int winner = 0x7fffffff;
+    if (best >= kFirstKey && mine == best) {
 #pragma unroll
       for (int i = N - 1; i >= 0; --i)
-        if (key[i] == best) e = i * 32 + lane;
+        if (key[i] == best) winner = i * LANES + sub;
     }
-    const int winner = static_cast<int>(__reduce_min_sync(kAll, static_cast<unsigned>(e)));
-    if (e == winner) {
-      mine = 0;
+    const int own = winner;
 #pragma unroll
-      for (int i = 0; i < N; ++i) {
-        if (i * 32 + lane == winner) key[i] = 0;
-        mine = max(mine, key[i]);
+    for (int o = LANES / 2; o > 0; o >>= 1) winner = min(winner, __shfl_xor_sync(kAll, winner, o));
+    if (best >= kFirstKey) {  // the warp's other row may have more or fewer
+      if (own == winner) {
+        mine = 0;
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+          if (i * LANES + sub == winner) key[i] = 0;
+          mine = max(mine, key[i]);
+        }
       }
+      if (sub == j) got = make_float2(key_value(best), __int_as_float(winner));
     }
-    if (lane == j) got = make_int2(static_cast<int>(best), winner);
   }
   return got;
 }
@@ -148,12 +210,12 @@ struct Route {
   const float* bias;
   int64_t T;
   int E, k;
-  int sigmoid, renormalize, balance;
+  int sigmoid, renormalize, balance, clustered;
   float scale;
   float* weights;
   int32_t *ids, *counts, *tokens;
   float* loss;
-  // zeroed before the launch (several CTAs): sum of p per expert in units of 2^-40, rows per
+  // zeroed before the launch, unless the grid is one cluster: sum of p per expert in units of 2^-40, rows per
   // expert, valid tokens, finished CTAs
   unsigned long long* psum;
   int32_t *acc_counts, *acc_tokens, *ticket;
@@ -162,6 +224,7 @@ struct Route {
 // Sums of p leave a CTA as 64-bit integers in units of 2^-40, so that the order in which the
 // CTAs add them does not change the result.  2^23 tokens fit.
 constexpr float kFixed = 1099511627776.0f;
+constexpr unsigned kClusterCtas = 8;  // as many as a cluster may always have
 constexpr int64_t kRouteMaxTokens = int64_t(1) << 23;
 
 // Sum of one value per thread, in a fixed order; thread 0 gets it.
@@ -177,16 +240,19 @@ __device__ double cta_sum64(double v, double* scratch) {
   return v;
 }
 
-// N experts per lane.  Dynamic shared memory: E counts, then one row of E sums of p per warp.
-template <typename T, int N, int WARPS>
-__global__ void __launch_bounds__(WARPS * 32) moe_route_kernel(const Route a) {
+// N experts per lane, LANES lanes per row.  Dynamic shared memory: E counts, then one row of E sums of p
+// per row that the CTA works on at a time.
+template <typename T, int N, int LANES, bool BIAS, int WARPS>
+__global__ void __launch_bounds__(WARPS * 32, N <= 16 ? 2 : 1) moe_route_kernel(const Route a) {
+  constexpr int kRows = 32 / LANES;  // per warp
   extern __shared__ int32_t route_smem[];
   __shared__ double scratch[WARPS];
   __shared__ int32_t s_tokens, s_last;
-  __shared__ unsigned long long s_list[WARPS][32];
+  __shared__ Candidates s_list[WARPS * kRows];
   int32_t* s_counts = route_smem;
   float* s_psum = reinterpret_cast<float*>(route_smem + a.E);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, sub = lane & (LANES - 1);
+  const int slot = threadIdx.x / LANES;  // of the CTA's rows
   for (int e = threadIdx.x; e < a.E; e += blockDim.x) s_counts[e] = 0;
   if (threadIdx.x == 0) s_tokens = 0;
   __syncthreads();
@@ -194,120 +260,172 @@ __global__ void __launch_bounds__(WARPS * 32) moe_route_kernel(const Route a) {
   grid_launch_dependents();
 
   const T* logits = static_cast<const T*>(a.logits);
+  const uint32_t sides = sort_sides<LANES>(sub);
   float psum[N];
 #pragma unroll
   for (int i = 0; i < N; ++i) psum[i] = 0.0f;
   int32_t tokens = 0;
-  const int64_t step = static_cast<int64_t>(gridDim.x) * WARPS;
-  float next[N];
-  const int left = a.E - lane;  // expert i * 32 + lane exists where i * 32 < left
+  const int64_t step = static_cast<int64_t>(gridDim.x) * WARPS * kRows;
+  T next[N];
+  const int left = a.E - sub;  // expert i * LANES + sub exists where i * LANES < left
+  const bool full = a.E == N * LANES;
   auto load_row = [&](int64_t row) {
-    const T* at = logits + row * a.stride + lane;
-    if (a.E == N * 32) {
+    const T* at = logits + min(row, a.T - 1) * a.stride + sub;
+    if (full) {
 #pragma unroll
-      for (int i = 0; i < N; ++i) next[i] = to_f(at[i * 32]);
+      for (int i = 0; i < N; ++i) next[i] = at[i * LANES];
     } else {
 #pragma unroll
-      for (int i = 0; i < N; ++i) next[i] = i * 32 < left ? to_f(at[i * 32]) : -INFINITY;
+      for (int i = 0; i < N; ++i) next[i] = i * LANES < left ? at[i * LANES] : from_f<T>(-INFINITY);
     }
   };
-  int64_t row = static_cast<int64_t>(blockIdx.x) * WARPS + warp;
-  if (row < a.T) load_row(row);
-  for (; row < a.T; row += step) {
-    uint32_t key[N];
+  int64_t first = (static_cast<int64_t>(blockIdx.x) * WARPS + warp) * kRows;  // of the warp's rows
+  if (first < a.T) load_row(first + lane / LANES);
+  for (; first < a.T; first += step) {
+    const int64_t row = first + lane / LANES;
     float v[N];
-    uint32_t top = 0;
+    float top = -INFINITY;  // fmaxf passes over NaN
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      v[i] = clean_logit(next[i]);
-      key[i] = order_key(v[i]);
-      top = max(top, key[i]);
+      v[i] = to_f(next[i]);
+      top = fmaxf(top, v[i]);
     }
-    if (row + step < a.T) load_row(row + step);
-    top = __reduce_max_sync(kAll, top);
-    int32_t id = -1;
-    float w = 0.0f;
-    if (top >= kFirstKey && (!a.mask || a.mask[row])) {  // warp-uniform
-      const float m = a.sigmoid ? 0.0f : key_value(top);
-      float inv = 1.0f;   // 1 / sum of exponentials (softmax)
-      float part = 0.0f;  // 1 / sum of scores
-      if (a.balance || a.bias || !a.renormalize) {
-        float total = 0.0f;
+    if (first + step < a.T) load_row(row + step);
+    bool valid = row < a.T && (!a.mask || a.mask[row]);
+    float2 got;
+    float m;
+    if constexpr (!BIAS) {
+      top = lanes_sorted<LANES>(top, sides);
+      m = __shfl_sync(kAll, top, 0, LANES);
+      got = choose<N, LANES>(v, m, __shfl_sync(kAll, top, a.k - 1, LANES), a.k, lane, s_list[slot]);
+    } else {
+      m = lanes_max<LANES>(top);
+    }
+    valid = valid && m > -INFINITY;
+    m = fminf(m, FLT_MAX);
+    const float shift = a.sigmoid || m == -INFINITY ? 0.0f : m;
+    float inv = 1.0f;   // 1 / sum of exponentials (softmax)
+    float part = 0.0f;  // 1 / sum of scores
+    if (a.balance || BIAS || !a.renormalize) {
+      float score[N];
+      float total = 0.0f;
+      if (a.sigmoid) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) total += score[i] = sigmoid_fast(v[i]);
+      } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i) total += score[i] = exp_fast(v[i] - shift);
+      }
+      total = lanes_sum<LANES>(total);
+      if (__any_sync(kAll, !(total < INFINITY))) {  // NaN or +inf among the logits
+        total = 0.0f;
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-          v[i] = a.sigmoid ? sigmoid_fast(v[i]) : exp_fast(v[i] - m);
-          total += v[i];
+          const float l = row < a.T && i * LANES < left ? clean_logit(to_f(logits[row * a.stride + i * LANES + sub])) : -INFINITY;
+          score[i] = a.sigmoid ? sigmoid_fast(l) : exp_fast(l - shift);
+          total += score[i];
         }
-        total = warp_sum(total);
-        part = total > 0.0f ? __fdividef(1.0f, total) : 0.0f;
-        if (!a.sigmoid) inv = part;
-        if (a.bias) {
-#pragma unroll
-          for (int i = 0; i < N; ++i)
-            if (key[i] >= kFirstKey) key[i] = order_key(clean_logit(v[i] * inv + __ldg(a.bias + i * 32 + lane)));
-        }
+        total = lanes_sum<LANES>(total);
       }
-      uint32_t mine = 0;
+      part = total > 0.0f ? __fdividef(1.0f, total) : 0.0f;
+      if (!a.sigmoid) inv = part;
+      if constexpr (BIAS) {
+        top = -INFINITY;
 #pragma unroll
-      for (int i = 0; i < N; ++i) mine = max(mine, key[i]);
-      const bool valid = __any_sync(kAll, mine >= kFirstKey);  // a bias of -inf may have left nothing
-      if (valid) {
-        ++tokens;
-        if (a.balance) {
+        for (int i = 0; i < N; ++i) {
+          // NaN and -inf stay what they are: not chosen
+          v[i] = v[i] >= -FLT_MAX ? clean_logit(score[i] * inv + __ldg(a.bias + i * LANES + sub)) : -INFINITY;
+          top = fmaxf(top, v[i]);
+        }
+        top = lanes_sorted<LANES>(top, sides);
+        const float most = __shfl_sync(kAll, top, 0, LANES);  // by every lane: valid differs between rows
+        valid = valid && most > -INFINITY;                    // a bias of -inf may have left nothing
+        got = choose<N, LANES>(v, most, __shfl_sync(kAll, top, a.k - 1, LANES), a.k, lane, s_list[slot]);
+      }
+      if (a.balance) {
+        if (!valid) part = 0.0f;
 #pragma unroll
-          for (int i = 0; i < N; ++i) psum[i] = fmaf(v[i], part, psum[i]);
-        }
-        const int2 got = choose<N>(key, mine, a.k, lane, s_list[warp]);
-        id = got.y;
-        if (id >= 0) {
-          // the key is that of the logit itself, unless a bias went into it
-          const float l = a.bias ? clean_logit(to_f(logits[row * a.stride + id])) : key_value(got.x);
-          w = a.sigmoid ? sigmoid_fast(l) : exp_fast(l - m) * inv;
-          atomicAdd(&s_counts[id], 1);
-        }
+        for (int i = 0; i < N; ++i) psum[i] = fmaf(score[i], part, psum[i]);
       }
-      if (a.renormalize) {
-        const float total = warp_sum(w);
-        w = total > 0.0f ? __fdividef(w, total) : 0.0f;
-      }
-      w *= a.scale;
     }
-    if (lane < a.k) {
-      a.ids[row * a.k + lane] = id;
-      a.weights[row * a.k + lane] = w;
+    const int32_t id = valid ? __float_as_int(got.y) : -1;
+    float w = 0.0f;
+    if (id >= 0) {
+      // the value is the logit itself, unless a bias went into it
+      const float l = BIAS ? clean_logit(to_f(logits[row * a.stride + id])) : got.x;
+      w = a.sigmoid ? sigmoid_fast(l) : exp_fast(l - m) * inv;
+      atomicAdd(&s_counts[id], 1);
+    }
+    if (valid) ++tokens;
+    if (a.renormalize) {
+      const float total = lanes_sum<LANES>(w);
+      w = total > 0.0f ? __fdividef(w, total) : 0.0f;
+    }
+    if (sub < a.k && row < a.T) {
+      a.ids[row * a.k + sub] = id;
+      a.weights[row * a.k + sub] = w * a.scale;
     }
   }
 
-  if (lane == 0 && tokens) atomicAdd(&s_tokens, tokens);
+  if (sub == 0 && tokens) atomicAdd(&s_tokens, tokens);
   if (a.balance) {
 #pragma unroll
     for (int i = 0; i < N; ++i)
-      if (i * 32 + lane < a.E) s_psum[warp * a.E + i * 32 + lane] = psum[i];
+      if (i * LANES < left) s_psum[slot * a.E + i * LANES + sub] = psum[i];
   }
   __syncthreads();
-  if (gridDim.x == 1) {  // one CTA saw every row
-    double sum = 0.0;
-    for (int e = threadIdx.x; e < a.E; e += blockDim.x) {
-      a.counts[e] = s_counts[e];
-      if (a.balance) {
-        double p = 0.0;
-        for (int i = 0; i < WARPS; ++i) p += s_psum[i * a.E + e];
-        sum += p * s_counts[e];
+  if (a.clustered) {  // the grid is one cluster: its first CTA reads the others' sums, in rank order
+    for (int e = threadIdx.x; a.balance && e < a.E; e += blockDim.x) {
+      float p = s_psum[e];
+      for (int i = 1; i < WARPS * kRows; ++i) p += s_psum[i * a.E + e];
+      s_psum[e] = p;
+    }
+    cluster_sync();
+    if (blockIdx.x == 0) {
+      double sum = 0.0;
+      for (int e = threadIdx.x; e < a.E; e += blockDim.x) {
+        int32_t count[kClusterCtas];
+        float p[kClusterCtas];
+#pragma unroll
+        for (int r = 0; r < kClusterCtas; ++r) {
+          count[r] = 0;
+          p[r] = 0.0f;
+          if (r < gridDim.x) {
+            asm volatile("ld.shared::cluster.b32 %0, [%1];" : "=r"(count[r]) : "r"(cluster_addr(s_counts + e, r)));
+            if (a.balance) asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(p[r]) : "r"(cluster_addr(s_psum + e, r)));
+          }
+        }
+        int32_t count_all = 0;
+        double p_all = 0.0;
+#pragma unroll
+        for (int r = 0; r < kClusterCtas; ++r) {
+          count_all += count[r];
+          p_all += p[r];
+        }
+        a.counts[e] = count_all;
+        sum += p_all * count_all;
+      }
+      if (a.balance) sum = cta_sum64<WARPS>(sum, scratch);
+      if (threadIdx.x == 0) {
+        int32_t tokens_all = 0;
+        for (int r = 0; r < gridDim.x; ++r) {
+          int32_t n;
+          asm volatile("ld.shared::cluster.b32 %0, [%1];" : "=r"(n) : "r"(cluster_addr(&s_tokens, r)));
+          tokens_all += n;
+        }
+        const double n = tokens_all > 0 ? tokens_all : 1;
+        *a.tokens = tokens_all;
+        if (a.balance) *a.loss = static_cast<float>(sum * a.E / a.k / n / n);
       }
     }
-    const double n = s_tokens > 0 ? s_tokens : 1;
-    if (a.balance) sum = cta_sum64<WARPS>(sum, scratch);
-    if (threadIdx.x == 0) {
-      *a.tokens = s_tokens;
-      if (a.balance) *a.loss = static_cast<float>(sum * a.E / a.k / n / n);
-    }
+    cluster_sync();  // no CTA leaves while its sums are read
     return;
   }
   for (int e = threadIdx.x; e < a.E; e += blockDim.x) {
     if (s_counts[e]) atomicAdd(&a.acc_counts[e], s_counts[e]);
     if (a.balance) {
       float p = 0.0f;
-      for (int i = 0; i < WARPS; ++i) p += s_psum[i * a.E + e];
+      for (int i = 0; i < WARPS * kRows; ++i) p += s_psum[i * a.E + e];
       atomicAdd(&a.psum[e], static_cast<unsigned long long>(__float2ull_rn(p * kFixed)));
     }
   }
@@ -333,6 +451,14 @@ __global__ void __launch_bounds__(WARPS * 32) moe_route_kernel(const Route a) {
   }
 }
 
+// The workspace's sums to zero.  A kernel and not a memset, so that the next kernel starts while it runs.
+__global__ void __launch_bounds__(256) route_clear_kernel(uint32_t* words, int n) {
+  grid_dependency_wait();
+  grid_launch_dependents();
+  const int i = blockIdx.x * 256 + threadIdx.x;
+  if (i < n) words[i] = 0;
+}
+
 struct RouteBwd {
   const void* logits;
   int64_t stride;
@@ -348,18 +474,20 @@ struct RouteBwd {
   int64_t d_stride;
 };
 
-// Dynamic shared memory: one row of E floats per warp, the scattered gradient of the chosen
-// scores (zero between rows).
-template <typename T, int N, int WARPS>
-__global__ void __launch_bounds__(WARPS * 32) moe_route_backward_kernel(const RouteBwd a) {
+// N experts per lane, LANES lanes per row.  Dynamic shared memory: E floats per row that the CTA works on
+// at a time, the scattered gradient of the chosen scores (zero between rows).
+template <typename T, int N, int LANES, bool SIGMOID, int WARPS>
+__global__ void __launch_bounds__(WARPS * 32, N <= 16 ? 2 : 1) moe_route_backward_kernel(const RouteBwd a) {
+  constexpr int kRows = 32 / LANES;  // per warp
   extern __shared__ float s_grad[];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  float* sg = s_grad + warp * a.E;
-  for (int e = lane; e < a.E; e += 32) sg[e] = 0.0f;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, sub = lane & (LANES - 1);
+  float* sg = s_grad + static_cast<int>(threadIdx.x / LANES) * a.E;
+  for (int e = sub; e < a.E; e += LANES) sg[e] = 0.0f;
   __syncwarp();
   grid_dependency_wait();
   grid_launch_dependents();
-  float load[N];  // a_e of the lane's experts
+  const int left = a.E - sub;  // expert i * LANES + sub exists where i * LANES < left
+  float load[N];               // a_e of the lane's experts
 #pragma unroll
   for (int i = 0; i < N; ++i) load[i] = 0.0f;
   if (a.gloss) {
@@ -367,66 +495,83 @@ __global__ void __launch_bounds__(WARPS * 32) moe_route_backward_kernel(const Ro
     const float f = *a.gloss * (static_cast<float>(a.E) / static_cast<float>(a.k)) / n / n;
 #pragma unroll
     for (int i = 0; i < N; ++i)
-      if (i * 32 + lane < a.E) load[i] = f * static_cast<float>(a.counts[i * 32 + lane]);
+      if (i * LANES < left) load[i] = f * static_cast<float>(a.counts[i * LANES + sub]);
   }
   const T* logits = static_cast<const T*>(a.logits);
-  const int64_t step = static_cast<int64_t>(gridDim.x) * WARPS;
-  float next[N];
+  const int64_t step = static_cast<int64_t>(gridDim.x) * WARPS * kRows;
+  T next[N];
   int32_t next_id = -1;
   float next_g = 0.0f;
-  const int left = a.E - lane;  // expert i * 32 + lane exists where i * 32 < left
   auto load_row = [&](int64_t row) {
-    const T* at = logits + row * a.stride + lane;
+    const T* at = logits + min(row, a.T - 1) * a.stride + sub;
 #pragma unroll
-    for (int i = 0; i < N; ++i) next[i] = i * 32 < left ? to_f(at[i * 32]) : -INFINITY;
-    if (lane < a.k) {
-      next_id = __ldg(a.ids + row * a.k + lane);
-      if (a.gw) next_g = __ldg(a.gw + row * a.k + lane);
+    for (int i = 0; i < N; ++i) next[i] = i * LANES < left ? at[i * LANES] : from_f<T>(-INFINITY);
+    next_id = -1;
+    if (sub < a.k && row < a.T) {
+      next_id = __ldg(a.ids + row * a.k + sub);
+      if (a.gw) next_g = __ldg(a.gw + row * a.k + sub);
     }
   };
-  int64_t row = static_cast<int64_t>(blockIdx.x) * WARPS + warp;
-  if (row < a.T) load_row(row);
-  for (; row < a.T; row += step) {
+  int64_t first = (static_cast<int64_t>(blockIdx.x) * WARPS + warp) * kRows;  // of the warp's rows
+  if (first < a.T) load_row(first + lane / LANES);
+  for (; first < a.T; first += step) {
+    const int64_t row = first + lane / LANES;
     float s[N];
-    float m = -INFINITY;
+    float m = -INFINITY;  // fmaxf passes over NaN
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      s[i] = clean_logit(next[i]);
+      s[i] = to_f(next[i]);
       m = fmaxf(m, s[i]);
     }
     const int32_t id = next_id >= 0 && next_id < a.E ? next_id : -1;
     float g = id >= 0 ? next_g * a.scale : 0.0f;
-    if (row + step < a.T) load_row(row + step);
-    T* out = static_cast<T*>(a.dlogits) + row * a.d_stride;
-    if (!__any_sync(kAll, id >= 0)) {  // masked token: no gradient
+    if (first + step < a.T) load_row(row + step);
+    T* out = static_cast<T*>(a.dlogits) + row * a.d_stride + sub;
+    const unsigned chosen_lanes = __ballot_sync(kAll, id >= 0);
+    const bool live = LANES == 32 ? chosen_lanes != 0 : (chosen_lanes & (0xFFFFu << (lane & 16))) != 0;
+    if (chosen_lanes == 0) {  // masked tokens: no gradient
 #pragma unroll
       for (int i = 0; i < N; ++i)
-        if (i * 32 + lane < a.E) out[i * 32 + lane] = from_f<T>(0.0f);
+        if (i * LANES < left && row < a.T) out[i * LANES] = from_f<T>(0.0f);
       continue;
     }
-    m = a.sigmoid ? 0.0f : key_value(__reduce_max_sync(kAll, order_key(m)));
+    float shift = 0.0f;
+    if constexpr (!SIGMOID) {
+      m = fminf(lanes_max<LANES>(m), FLT_MAX);
+      shift = m == -INFINITY ? 0.0f : m;
+    }
     float total = 0.0f;
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-      s[i] = a.sigmoid ? sigmoid_fast(s[i]) : exp_fast(s[i] - m);
-      total += s[i];
-    }
-    total = warp_sum(total);
-    const float inv = total > 0.0f ? __fdividef(1.0f, total) : 0.0f;
-    if (!a.sigmoid) {
+    for (int i = 0; i < N; ++i) total += s[i] = SIGMOID ? sigmoid_fast(s[i]) : exp_fast(s[i] - shift);
+    total = lanes_sum<LANES>(total);
+    if (__any_sync(kAll, !(total < INFINITY))) {  // NaN or +inf among the logits
+      total = 0.0f;
 #pragma unroll
-      for (int i = 0; i < N; ++i) s[i] *= inv;  // the scores are the probabilities
+      for (int i = 0; i < N; ++i) {
+        const float l = row < a.T && i * LANES < left ? clean_logit(to_f(logits[row * a.stride + i * LANES + sub])) : -INFINITY;
+        total += s[i] = SIGMOID ? sigmoid_fast(l) : exp_fast(l - shift);
+      }
+      total = lanes_sum<LANES>(total);
+    }
+    // a row without a choice: all terms zero
+    const float inv = live && total > 0.0f ? __fdividef(1.0f, total) : 0.0f;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      if constexpr (SIGMOID)
+        s[i] = live ? s[i] : 0.0f;
+      else
+        s[i] *= inv;  // the scores are the probabilities
     }
     if (a.gw) {
       if (a.renormalize) {
         float c = 0.0f;
         if (id >= 0) {
           const float l = clean_logit(to_f(logits[row * a.stride + id]));
-          c = a.sigmoid ? sigmoid_fast(l) : exp_fast(l - m) * inv;
+          c = SIGMOID ? sigmoid_fast(l) : exp_fast(l - shift) * inv;
         }
-        float chosen = warp_sum(c);
+        float chosen = lanes_sum<LANES>(c);
         chosen = chosen > 0.0f ? __fdividef(1.0f, chosen) : 1.0f;
-        g = (g - warp_sum(g * c) * chosen) * chosen;
+        g = (g - lanes_sum<LANES>(g * c) * chosen) * chosen;
       }
       if (id >= 0) atomicAdd(&sg[id], g);
       __syncwarp();
@@ -435,10 +580,11 @@ __global__ void __launch_bounds__(WARPS * 32) moe_route_backward_kernel(const Ro
     float dot = 0.0f;  // of what meets the probabilities: everything (softmax) or the loss alone
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      d[i] = a.gw && i * 32 < left ? sg[i * 32 + lane] : 0.0f;
-      dot = fmaf(a.sigmoid ? load[i] : d[i] + load[i], s[i], dot);
+      d[i] = a.gw && i * LANES < left ? sg[i * LANES + sub] : 0.0f;
+      if constexpr (!SIGMOID) d[i] += load[i];
+      dot = fmaf(SIGMOID ? load[i] : d[i], s[i], dot);
     }
-    dot = warp_sum(dot);
+    dot = lanes_sum<LANES>(dot);
     if (a.gw) {
       __syncwarp();
       if (id >= 0) sg[id] = 0.0f;
@@ -447,21 +593,25 @@ __global__ void __launch_bounds__(WARPS * 32) moe_route_backward_kernel(const Ro
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       float v;
-      if (a.sigmoid)
+      if constexpr (SIGMOID)
         v = (d[i] + (load[i] - dot * inv) * inv) * s[i] * (1.0f - s[i]);
       else
-        v = s[i] * (d[i] + load[i] - dot);
-      if (i * 32 < left) out[i * 32 + lane] = from_f<T>(v);
+        v = s[i] * (d[i] - dot);
+      if (i * LANES < left && row < a.T) out[i * LANES] = from_f<T>(v);
     }
   }
 }
 
 constexpr int kRouteWarps = 8;
-// Few tokens over few experts run in one CTA of 32 warps, which needs neither zeroed sums (a
-// memset before the kernel) nor a last CTA.
-constexpr int64_t kOneCtaTokens = 64;
-constexpr int kOneCtaExperts = 256;
-bool one_cta(int64_t T, int64_t E) { return T <= kOneCtaTokens && E <= kOneCtaExperts; }
+// Lanes per row.  What a row costs beside its experts (sorting, listing and ranking, the sums) is most
+// of it, and two rows to a warp share that; but 16 lanes' maxima bound only a short choice well, and
+// more experts would not stay in registers.  Forward at 32,768 x 256, k = 8: 20.8 us with 16 lanes, 26.3
+// with 32; at 32,768 x 32, k = 2: 12.9 and 19.8 us.
+int lanes_per_row(int E, int k) { return k <= 8 && E <= 256 ? 16 : 32; }
+int64_t rows_per_cta(int E, int k) { return kRouteWarps * 32 / lanes_per_row(E, k); }
+// What one cluster does in one pass runs in one cluster, which needs neither zeroed sums nor a last
+// CTA: 64 x 256, k = 8 in 4.9 us, over the GPU in 6.1 us; two passes cost more than the whole grid.
+bool one_cluster(int64_t T, int E, int k) { return T <= int64_t(kClusterCtas) * rows_per_cta(E, k); }
 
 // CTAs of a kernel that an SM holds at once (looked up once: the library runs on one kind of device).
 template <typename K>
@@ -474,55 +624,76 @@ int resident_ctas(K kernel, int threads, size_t smem, std::atomic<int>* known) {
   return n;
 }
 
-template <typename T, int N>
-int launch_route(const Route& a, cudaStream_t st) {
-  if constexpr (N * 32 <= kOneCtaExperts) {
-    if (one_cta(a.T, a.E)) {
-      const size_t smem = a.E * 4 + (a.balance ? size_t(32) * a.E * 4 : 0);
-      return launch(moe_route_kernel<T, N, 32>, dim3(1), 1024, smem, st, a);
-    }
-  }
+template <typename T, int N, int LANES, bool BIAS>
+int launch_route_as(const Route& a, cudaStream_t st) {
+  constexpr int kRows = kRouteWarps * 32 / LANES;
   // the largest dynamic shared memory of this N, so that one look-up serves every call
   static std::atomic<int> known{0};
-  const int per_sm = resident_ctas(moe_route_kernel<T, N, kRouteWarps>, kRouteWarps * 32,
-                                   size_t(N) * 32 * 4 * (kRouteWarps + 1), &known);
-  const int64_t ctas = (a.T + kRouteWarps - 1) / kRouteWarps;
+  const int per_sm = resident_ctas(moe_route_kernel<T, N, LANES, BIAS, kRouteWarps>, kRouteWarps * 32,
+                                   size_t(N) * LANES * 4 * (kRows + 1), &known);
+  const int64_t ctas = (a.T + kRows - 1) / kRows;
+  const size_t smem = a.E * 4 + (a.balance ? size_t(kRows) * a.E * 4 : 0);
+  const auto kernel = moe_route_kernel<T, N, LANES, BIAS, kRouteWarps>;
+  if (a.clustered) {
+    unsigned cluster = 1;
+    while (cluster < kClusterCtas && cluster < ctas) cluster *= 2;
+    return launch_clusters(kernel, dim3(cluster), cluster, kRouteWarps * 32, smem, st, a);
+  }
   const unsigned grid = static_cast<unsigned>(std::min<int64_t>(ctas, int64_t(sm_count()) * per_sm));
-  const size_t smem = a.E * 4 + (a.balance ? size_t(kRouteWarps) * a.E * 4 : 0);
-  return launch(moe_route_kernel<T, N, kRouteWarps>, dim3(grid), kRouteWarps * 32, smem, st, a);
+  return launch(kernel, dim3(grid), kRouteWarps * 32, smem, st, a);
 }
 
-template <typename T, int N>
-int launch_route_backward(const RouteBwd& a, cudaStream_t st) {
+template <typename T, int N, int LANES>
+int launch_route(const Route& a, cudaStream_t st) {
+  return a.bias ? launch_route_as<T, N, LANES, true>(a, st) : launch_route_as<T, N, LANES, false>(a, st);
+}
+
+template <typename T, int N, int LANES, bool SIGMOID>
+int launch_route_backward_as(const RouteBwd& a, cudaStream_t st) {
+  constexpr int kRows = kRouteWarps * 32 / LANES;
   static std::atomic<int> known{0};
-  const int per_sm = resident_ctas(moe_route_backward_kernel<T, N, kRouteWarps>, kRouteWarps * 32,
-                                   size_t(N) * 32 * 4 * kRouteWarps, &known);
-  const int64_t ctas = (a.T + kRouteWarps - 1) / kRouteWarps;
+  const auto kernel = moe_route_backward_kernel<T, N, LANES, SIGMOID, kRouteWarps>;
+  const int per_sm = resident_ctas(kernel, kRouteWarps * 32, size_t(N) * LANES * 4 * kRows, &known);
+  const int64_t ctas = (a.T + kRows - 1) / kRows;
   const unsigned grid = static_cast<unsigned>(std::min<int64_t>(ctas, int64_t(sm_count()) * per_sm));
-  return launch(moe_route_backward_kernel<T, N, kRouteWarps>, dim3(grid), kRouteWarps * 32, size_t(kRouteWarps) * a.E * 4, st,
-                a);
+  return launch(kernel, dim3(grid), kRouteWarps * 32, size_t(kRows) * a.E * 4, st, a);
+}
+
+template <typename T, int N, int LANES>
+int launch_route_backward(const RouteBwd& a, cudaStream_t st) {
+  return a.sigmoid ? launch_route_backward_as<T, N, LANES, true>(a, st) : launch_route_backward_as<T, N, LANES, false>(a, st);
 }
 
 template <typename T>
 int dispatch_route(const Route& a, cudaStream_t st) {
+  if (lanes_per_row(a.E, a.k) == 16) {
+    const int n = (a.E + 15) / 16;
+    if (n <= 4) return launch_route<T, 4, 16>(a, st);
+    if (n <= 8) return launch_route<T, 8, 16>(a, st);
+    if (n <= 12) return launch_route<T, 12, 16>(a, st);
+    return launch_route<T, 16, 16>(a, st);
+  }
   const int n = (a.E + 31) / 32;
-  if (n <= 1) return launch_route<T, 1>(a, st);
-  if (n <= 2) return launch_route<T, 2>(a, st);
-  if (n <= 4) return launch_route<T, 4>(a, st);
-  if (n <= 8) return launch_route<T, 8>(a, st);
-  if (n <= 16) return launch_route<T, 16>(a, st);
-  return launch_route<T, 32>(a, st);
+  if (n <= 2) return launch_route<T, 2, 32>(a, st);
+  if (n <= 8) return launch_route<T, 8, 32>(a, st);
+  if (n <= 16) return launch_route<T, 16, 32>(a, st);
+  return launch_route<T, 32, 32>(a, st);
 }
 
 template <typename T>
 int dispatch_route_backward(const RouteBwd& a, cudaStream_t st) {
+  if (lanes_per_row(a.E, a.k) == 16) {
+    const int n = (a.E + 15) / 16;
+    if (n <= 4) return launch_route_backward<T, 4, 16>(a, st);
+    if (n <= 8) return launch_route_backward<T, 8, 16>(a, st);
+    if (n <= 12) return launch_route_backward<T, 12, 16>(a, st);
+    return launch_route_backward<T, 16, 16>(a, st);
+  }
   const int n = (a.E + 31) / 32;
-  if (n <= 1) return launch_route_backward<T, 1>(a, st);
-  if (n <= 2) return launch_route_backward<T, 2>(a, st);
-  if (n <= 4) return launch_route_backward<T, 4>(a, st);
-  if (n <= 8) return launch_route_backward<T, 8>(a, st);
-  if (n <= 16) return launch_route_backward<T, 16>(a, st);
-  return launch_route_backward<T, 32>(a, st);
+  if (n <= 2) return launch_route_backward<T, 2, 32>(a, st);
+  if (n <= 8) return launch_route_backward<T, 8, 32>(a, st);
+  if (n <= 16) return launch_route_backward<T, 16, 32>(a, st);
+  return launch_route_backward<T, 32, 32>(a, st);
 }
 
 }  // namespace
@@ -552,10 +723,8 @@ int cdg_moe_route(const cdg_route_args* g, void* workspace, size_t workspace_byt
       return CDG_ERR_CUDA;
     return CDG_OK;
   }
-  if (!one_cta(g->T, g->E) &&
-      cudaMemsetAsync(workspace, 0, cdg_moe_route_workspace_bytes(g->E), st) != cudaSuccess)
-    return CDG_ERR_CUDA;
   Route a{};
+  a.clustered = one_cluster(g->T, static_cast<int>(g->E), static_cast<int>(g->topk));
   a.logits = g->logits;
   a.stride = g->stride;
   a.mask = g->token_mask;
@@ -576,6 +745,11 @@ int cdg_moe_route(const cdg_route_args* g, void* workspace, size_t workspace_byt
   a.acc_counts = reinterpret_cast<int32_t*>(a.psum + a.E);
   a.acc_tokens = a.acc_counts + a.E;
   a.ticket = a.acc_tokens + 1;
+  if (!a.clustered) {
+    const int words = static_cast<int>(cdg_moe_route_workspace_bytes(g->E) / 4);
+    const int rc = launch(route_clear_kernel, dim3((words + 255) / 256), 256, 0, st, static_cast<uint32_t*>(workspace), words);
+    if (rc != CDG_OK) return rc;
+  }
   if (g->dtype == CDG_DTYPE_BF16) return dispatch_route<__nv_bfloat16>(a, st);
   if (g->dtype == CDG_DTYPE_F16) return dispatch_route<__half>(a, st);
   return dispatch_route<float>(a, st);

@@ -174,20 +174,35 @@ __global__ void __launch_bounds__(1024) column_sum_kernel(const float* partial, 
 // Launch with programmatic stream serialization (unless cdg_set_pdl(0)): the kernel may be scheduled
 // while its predecessor on the stream, of this call or of another, drains; it waits for the
 // predecessor's end (griddepcontrol.wait) before it touches global memory.  Calls of a few
-// microseconds in a row lose about one less between them.
+// microseconds in a row lose about one less between them.  cluster: CTAs of a cluster, 0 as the
+// kernel says.
 template <typename... K, typename... A>
-inline int launch(void (*kernel)(K...), dim3 grid, unsigned block, size_t smem, cudaStream_t st, A&&... args) {
+inline int launch_clusters(void (*kernel)(K...), dim3 grid, unsigned cluster, unsigned block, size_t smem, cudaStream_t st,
+                           A&&... args) {
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = grid;
   cfg.blockDim = dim3(block);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
-  cudaLaunchAttribute at[1];
-  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchAttribute at[2];
+  unsigned n = 0;
+  if (cluster > 0) {
+    at[n].id = cudaLaunchAttributeClusterDimension;
+    at[n].val.clusterDim.x = cluster;
+    at[n].val.clusterDim.y = 1;
+    at[n++].val.clusterDim.z = 1;
+  }
+  if (cdg_get_pdl()) {
+    at[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[n++].val.programmaticStreamSerializationAllowed = 1;
+  }
   cfg.attrs = at;
-  cfg.numAttrs = cdg_get_pdl() ? 1 : 0;
+  cfg.numAttrs = n;
   return cudaLaunchKernelEx(&cfg, kernel, static_cast<K>(args)...) == cudaSuccess ? CDG_OK : CDG_ERR_CUDA;
+}
+template <typename... K, typename... A>
+inline int launch(void (*kernel)(K...), dim3 grid, unsigned block, size_t smem, cudaStream_t st, A&&... args) {
+  return launch_clusters(kernel, grid, 0, block, smem, st, static_cast<A&&>(args)...);
 }
 
 // SM count of the current device (looked up at each call: a cheap attribute query).
