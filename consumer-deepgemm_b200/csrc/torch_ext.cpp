@@ -6,6 +6,8 @@
 // workspace taken from PyTorch's caching allocator.  There is no host fallback:
 // CPU tensors are rejected.
 #include <ATen/cuda/CUDAContext.h>
+#include <ATen/cuda/EmptyTensor.h>
+#include <c10/cuda/CUDACachingAllocator.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/extension.h>
 
@@ -613,6 +615,15 @@ torch::Tensor ep_unpermute_combine(const torch::Tensor& Y, const torch::Tensor& 
 }
 
 // ------------------------------------------------------------------ around the experts: norm, router, dense product
+// A new tensor on `dev`, and a workspace that goes back to the allocator (in the stream's order) when it goes
+// out of scope.  What torch::empty calls in the end: small calls cost what their allocations cost on the host.
+torch::Tensor fresh(at::IntArrayRef sizes, at::ScalarType dtype, const torch::Device& dev) {
+  return at::Tensor(at::detail::empty_cuda(sizes, dtype, dev, c10::nullopt));
+}
+c10::DataPtr scratch(size_t bytes) {
+  return bytes ? c10::cuda::CUDACachingAllocator::get()->allocate(bytes) : c10::DataPtr();
+}
+
 // A [rows, columns] tensor with unit stride along its columns, on `dev`.
 void check_rows(const torch::Tensor& t, const char* name, const torch::Device& dev, int64_t rows, int64_t cols) {
   check_cuda(t, name, dev);
@@ -654,18 +665,18 @@ py::tuple add_rms_norm(const torch::Tensor& x, const torch::Tensor& w, const c10
     TORCH_CHECK_VALUE(residual->scalar_type() == x.scalar_type(), "residual must have x's dtype");
     g.r = residual->data_ptr();
     g.r_stride = residual->stride(0);
-    h = torch::empty({T, H}, x.options());
+    h = fresh({T, H}, x.scalar_type(), dev);
     g.h = h.data_ptr();
     g.h_stride = H;
   }
   if (normed) {
-    y = torch::empty({T, H}, x.options());
+    y = fresh({T, H}, x.scalar_type(), dev);
     g.y = y.data_ptr();
     g.y_stride = H;
   }
   if (quantize) {
-    q = torch::empty({T, H}, x.options().dtype(torch::kFloat8_e4m3fn));
-    s = torch::empty({T, (H + 127) / 128}, x.options().dtype(torch::kFloat32));
+    q = fresh({T, H}, torch::kFloat8_e4m3fn, dev);
+    s = fresh({T, (H + 127) / 128}, torch::kFloat32, dev);
     g.q = reinterpret_cast<uint8_t*>(q.data_ptr());
     g.q_stride = H;
     g.s = s.data_ptr<float>();
@@ -708,10 +719,10 @@ std::vector<torch::Tensor> rms_norm_backward(const torch::Tensor& dy, const torc
     g.dh_stride = dh->stride(0);
   }
   const c10::cuda::CUDAGuard guard(dev);
-  auto dx = torch::empty({T, H}, h.options());
-  auto dw = torch::empty({H}, w.options());
+  auto dx = fresh({T, H}, h.scalar_type(), dev);
+  auto dw = fresh({H}, w.scalar_type(), dev);
   const size_t ws_bytes = cdg_rms_norm_backward_workspace_bytes(T, H);
-  auto ws = torch::empty({static_cast<int64_t>(ws_bytes)}, h.options().dtype(torch::kUInt8));
+  const c10::DataPtr ws = scratch(ws_bytes);
   g.dy = dy.data_ptr();
   g.dy_stride = dy.stride(0);
   g.h = h.data_ptr();
@@ -725,7 +736,7 @@ std::vector<torch::Tensor> rms_norm_backward(const torch::Tensor& dy, const torc
   g.dx = dx.data_ptr();
   g.dx_stride = H;
   g.dw = dw.data_ptr();
-  check_status(cdg_rms_norm_backward(&g, ws.data_ptr(), ws_bytes, cur_stream(h)), "add_rms_norm_backward");
+  check_status(cdg_rms_norm_backward(&g, ws.get(), ws_bytes, cur_stream(h)), "add_rms_norm_backward");
   return {dx, dw};
 }
 
@@ -756,19 +767,17 @@ py::tuple moe_route(const torch::Tensor& logits, int64_t topk, bool sigmoid, boo
     g.token_mask = static_cast<const uint8_t*>(mask->data_ptr());
   }
   const c10::cuda::CUDAGuard guard(dev);
-  auto f32 = logits.options().dtype(torch::kFloat32);
-  auto i32 = logits.options().dtype(torch::kInt32);
-  auto weights = torch::empty({T, topk}, f32);
-  auto ids = torch::empty({T, topk}, i32);
-  auto counts = torch::empty({E}, i32);
-  auto tokens = torch::empty({1}, i32);
+  auto weights = fresh({T, topk}, torch::kFloat32, dev);
+  auto ids = fresh({T, topk}, torch::kInt32, dev);
+  auto counts = fresh({E}, torch::kInt32, dev);
+  auto tokens = fresh({1}, torch::kInt32, dev);
   torch::Tensor loss;
   if (balance) {
-    loss = torch::empty({1}, f32);
+    loss = fresh({1}, torch::kFloat32, dev);
     g.loss = loss.data_ptr<float>();
   }
   const size_t ws_bytes = cdg_moe_route_workspace_bytes(E);
-  auto ws = torch::empty({static_cast<int64_t>(ws_bytes)}, logits.options().dtype(torch::kUInt8));
+  const c10::DataPtr ws = scratch(ws_bytes);
   g.logits = logits.data_ptr();
   g.stride = logits.stride(0);
   g.dtype = dtype_code(logits);
@@ -782,7 +791,7 @@ py::tuple moe_route(const torch::Tensor& logits, int64_t topk, bool sigmoid, boo
   g.ids = ids.data_ptr<int32_t>();
   g.counts = counts.data_ptr<int32_t>();
   g.tokens = tokens.data_ptr<int32_t>();
-  check_status(cdg_moe_route(&g, ws_bytes ? ws.data_ptr() : nullptr, ws_bytes, cur_stream(logits)), "moe_route");
+  check_status(cdg_moe_route(&g, ws.get(), ws_bytes, cur_stream(logits)), "moe_route");
   return py::make_tuple(weights, ids, counts, tokens, balance ? py::cast(loss) : py::none());
 }
 
@@ -819,7 +828,7 @@ torch::Tensor moe_route_backward(const torch::Tensor& logits, const torch::Tenso
     g.tokens = tokens->data_ptr<int32_t>();
   }
   const c10::cuda::CUDAGuard guard(dev);
-  auto out = torch::empty({T, E}, logits.options());
+  auto out = fresh({T, E}, logits.scalar_type(), dev);
   g.logits = logits.data_ptr();
   g.stride = logits.stride(0);
   g.dtype = dtype_code(logits);
@@ -869,10 +878,10 @@ py::tuple linear(const torch::Tensor& x, const torch::Tensor& w, const c10::opti
     g.residual_dtype = dtype_code(*residual);
   }
   const c10::cuda::CUDAGuard guard(dev);
-  auto y = torch::empty({M, N}, out_f32 ? x.options().dtype(torch::kFloat32) : x.options());
+  auto y = fresh({M, N}, out_f32 ? torch::kFloat32 : x.scalar_type(), dev);
   torch::Tensor z;
   if (preact) {
-    z = torch::empty({M, N}, x.options());
+    z = fresh({M, N}, x.scalar_type(), dev);
     g.z_out = z.data_ptr();
     g.z_stride = N;
   }
@@ -889,9 +898,8 @@ py::tuple linear(const torch::Tensor& x, const torch::Tensor& w, const c10::opti
   g.y = y.data_ptr();
   g.y_stride = N;
   const size_t ws_bytes = cdg_linear_workspace_bytes(&g);
-  torch::Tensor ws;
-  if (ws_bytes) ws = torch::empty({static_cast<int64_t>(ws_bytes)}, x.options().dtype(torch::kUInt8));
-  check_status(cdg_linear(&g, ws_bytes ? ws.data_ptr() : nullptr, ws_bytes, cur_stream(x)), "linear");
+  const c10::DataPtr ws = scratch(ws_bytes);
+  check_status(cdg_linear(&g, ws.get(), ws_bytes, cur_stream(x)), "linear");
   return py::make_tuple(y, preact ? py::cast(z) : py::none());
 }
 
@@ -922,17 +930,17 @@ py::tuple linear_backward(const torch::Tensor& dy, const torch::Tensor& x, const
   const c10::cuda::CUDAGuard guard(dev);
   torch::Tensor dx, dw, db;
   if (want_dx) {
-    dx = torch::empty({M, K}, x.options());
+    dx = fresh({M, K}, x.scalar_type(), dev);
     g.dx = dx.data_ptr();
     g.dx_stride = K;
   }
   if (want_dw) {
-    dw = torch::empty({N, K}, x.options());
+    dw = fresh({N, K}, x.scalar_type(), dev);
     g.dw = dw.data_ptr();
     g.dw_stride = K;
   }
   if (want_db) {
-    db = torch::empty({N}, x.options());
+    db = fresh({N}, x.scalar_type(), dev);
     g.db = db.data_ptr();
   }
   g.db_dtype = dtype_code(x);
@@ -948,9 +956,8 @@ py::tuple linear_backward(const torch::Tensor& dy, const torch::Tensor& x, const
   g.N = N;
   g.K = K;
   const size_t ws_bytes = cdg_linear_backward_workspace_bytes(&g);
-  torch::Tensor ws;
-  if (ws_bytes) ws = torch::empty({static_cast<int64_t>(ws_bytes)}, x.options().dtype(torch::kUInt8));
-  check_status(cdg_linear_backward(&g, ws_bytes ? ws.data_ptr() : nullptr, ws_bytes, cur_stream(x)), "linear_backward");
+  const c10::DataPtr ws = scratch(ws_bytes);
+  check_status(cdg_linear_backward(&g, ws.get(), ws_bytes, cur_stream(x)), "linear_backward");
   auto give = [](const torch::Tensor& t) -> py::object { return t.defined() ? py::cast(t) : py::none(); };
   return py::make_tuple(give(dx), give(dw), give(db));
 }
