@@ -10,7 +10,9 @@
 //
 // Both directions are bound by memory: the forward pass reads x and r once and writes h, y, q and
 // the scales once, the backward pass reads dy, h and dh once and writes dx once.  A row stays in
-// its CTA's registers between the sum of squares and the stores.
+// its CTA's registers between the sum of squares and the stores.  One B200: 32,768 x 4096 BF16 with
+// residual and codes 192 us (6.3 TB/s; a plain copy 6.5), 8 x 4096 2.3 us; backward of 16,384 x 4096
+// with dh 94 us (5.7 TB/s) with the sums of dw.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
@@ -420,9 +422,9 @@ template <typename T, bool WIDE>
 int launch_norm(const NormFwd& a, cudaStream_t st) {
   const int chunks = static_cast<int>((a.H + 255) / 256);
   // Few rows are spread over as many warps as they have chunks (latency).  Otherwise a warp holds
-  // two chunks: 32,768 x 4096 BF16 with residual and codes takes 203 us so, 259 us with one (more
-  // warps wait at each row's barrier) and 236 us with four (100 registers a thread leave too few
-  // warps to cover the loads); 65,536 x 1024 takes 96 us, 118 us and 119 us.  Only rows of more
+  // two chunks: 32,768 x 4096 BF16 with residual and codes takes 192 us so; in one comparison, single
+  // launches, 203 us, 259 us with one (more warps wait at each row's barrier) and 236 us with four (100
+  // registers a thread leave too few warps to cover the loads); 65,536 x 1024 96 us, 118 us and 119 us.  Only rows of more
   // than 16,384 columns need four, with some spilling.
   const int iter = chunks <= 32 && a.T <= 2 * sm_count() ? 1 : chunks > 64 ? 4 : chunks >= 2 ? 2 : 1;
   const int warps = (chunks + iter - 1) / iter;
