@@ -273,7 +273,7 @@ int launch_pairs(const Matrix& A, const Matrix& B, const LinearShape& s, Epilogu
 // shapes under every cut, from 64 x 512 x 512 to 16,384 x 64 x 1024 (one B200, calls in a row).  What they
 // decide, for instance: 128 x 4096 x 4096 pairs 26.2, 128 x 64 in 2 parts 14.0 us; 1024 x 2048 x 2048 pairs
 // 16.8, 128 x 128 13.7, 128 x 64 15.2 us; 300 x 8192 x 512 pairs 9.9, 128 x 64 12.9 us; 3000 x 3000 x 256
-// pairs 12.0, 128 x 128 16.9 us; 2910 x 94 x 192 128 x 64 7.8, 128 x 128 11.8 us.
+// pairs 12.0, 128 x 128 16.9 us; 2910 x 94 x 192 128 x 64 7.8, pairs 8.3, 128 x 128 11.8 us.
 struct Plan {
   enum Kind { kPairs, kTiles, kSwapped } kind;
   int bn, splits;
@@ -316,7 +316,7 @@ Plan make_plan(int64_t M, int64_t N, int64_t k_steps, bool narrow, int sms) {
   }
   const int64_t pairs = std::max(1, sms / 2), pair_tiles = (M + 255) / 256 * ((N + 255) / 256);
   const double waves = static_cast<double>((pair_tiles + pairs - 1) / pairs);
-  if (k_steps > 0 && 4.0 + waves * (2.6 + 0.293 * static_cast<double>(k_steps) + (narrow ? 4.0 : 0.0)) < least)
+  if (k_steps > 0 && 4.0 + waves * (2.6 + 0.293 * static_cast<double>(k_steps) + (narrow ? 2.0 : 0.0)) < least)
     best.kind = Plan::kPairs;
   return best;
 }

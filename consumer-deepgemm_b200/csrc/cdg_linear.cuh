@@ -352,6 +352,67 @@ __device__ __forceinline__ void store_row_word(uint16_t* row, int len, int lane,
   if (lane == 31 && 63 < len && odd) row[63] = static_cast<uint16_t>(columns >> 16);
 }
 
+// The same for up to 32 rows of 64 columns, word(r) being where the lane's word of row r is kept: the rows
+// that start on words and those that do not each in a loop of their own, without tests per row; a row's
+// single columns at its ends are lane r's.  Reading is in two steps, so that all rows are on their way
+// at once (asynchronous copies of words, which lie one column too far left in odd rows until the
+// second step).  With tests per row and eight rows at a time 10,861 x 3278 x 48 took 65 us, with a residual 134
+// us; now 38 and 75 us (odd rows, N = 3279: 43 and 89 us; rows that TMA stores, N = 3280: 26 and 43 us).
+template <typename W>
+__device__ __forceinline__ void store_rows(uint16_t* first, int64_t stride, int rows, int lane, const uint8_t* tile, const W& word) {
+  const int classes = 1 + static_cast<int>(stride & 1);
+  const int64_t step = stride * classes;  // even
+#pragma unroll 1
+  for (int c = 0; c < classes; ++c) {
+    uint16_t* row = first + c * stride;
+    if (!odd_row(row)) {
+      uint32_t* to = reinterpret_cast<uint32_t*>(row) + lane;
+#pragma unroll 8
+      for (int r = c; r < rows; r += classes, to += step / 2) *to = *word(r);
+    } else {
+      uint32_t* to = reinterpret_cast<uint32_t*>(row - 1) + lane;  // lane 0's is half another's: not stored
+#pragma unroll 8
+      for (int r = c; r < rows; r += classes, to += step / 2) {
+        const uint32_t columns = *word(r), before = __shfl_up_sync(0xffffffffu, columns, 1);
+        if (lane > 0) *to = (before >> 16) | (columns << 16);
+      }
+    }
+  }
+  uint16_t* own = first + lane * stride;
+  if (lane < rows && odd_row(own)) {
+    own[0] = *reinterpret_cast<const uint16_t*>(tile + lane * 128 + ((lane & 7) << 4));
+    own[63] = *reinterpret_cast<const uint16_t*>(tile + lane * 128 + ((7 ^ (lane & 7)) << 4) + 14);
+  }
+}
+
+// First step; the result is the lane's row's first (low half) and last column, where it starts on an odd one.
+template <typename W>
+__device__ __forceinline__ uint32_t begin_rows(const uint16_t* first, int64_t stride, int rows, int lane, const W& word) {
+  uint32_t ends = 0;
+  const uint16_t* own = first + lane * stride;
+  if (lane < rows && odd_row(own)) ends = __ldg(own) | static_cast<uint32_t>(__ldg(own + 63)) << 16;
+#pragma unroll 8
+  for (int r = 0; r < rows; ++r) {
+    const int odd = odd_row(first + r * stride);
+    const uint32_t* from = reinterpret_cast<const uint32_t*>(first + r * stride - odd) + lane;
+    if (lane >= odd)
+      asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(word(r))), "l"(from) : "memory");
+  }
+  return ends;
+}
+template <typename W>
+__device__ __forceinline__ void finish_rows(const uint16_t* first, int64_t stride, int rows, int lane, uint32_t ends, const W& word) {
+  asm volatile("cp.async.wait_all;" ::: "memory");
+#pragma unroll 4
+  for (int r = 0; r < rows; ++r) {
+    if (!odd_row(first + r * stride)) continue;  // warp-uniform
+    const uint32_t end = __shfl_sync(0xffffffffu, ends, r);
+    const uint32_t mine = lane == 0 ? end << 16 : *word(r), next = __shfl_down_sync(0xffffffffu, mine, 1);
+    *word(r) = (mine >> 16) | (lane == 31 ? end & 0xffff0000u : next << 16);
+  }
+  __syncwarp();
+}
+
 struct LinearShape {
   int64_t M, N;
   int k_steps;         // of 64 columns of K
@@ -771,7 +832,7 @@ __global__ void __launch_bounds__(kThreadsOf<SWAP>)
 // of the accumulator, adds it in place and has the result stored from there, so that global memory
 // sees whole tiles; clipping at M and N is TMA's.  Where rows start on other boundaries, the warp
 // itself copies the residual's rows in and the result's out, in whole words (10,861 x 3279 x 48 with a
-// residual: 226 us with single elements).  With z, or a residual of another type, its lanes turn
+// residual: 226 us with single elements, 89 us so).  With z, or a residual of another type, its lanes turn
 // their columns and store along the rows.
 // Warps: 0 TMA producer, 1 MMA issuer (even CTA) and TMEM owner, 4-19 epilogue.
 template <int BN>
@@ -1007,17 +1068,22 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairTileSmem<BN>::kT
       const int len = any ? static_cast<int>(s.N - col0 < CH ? s.N - col0 : CH) : 0;
       // word l of row r of the staged tile
       auto word = [&](int r) { return reinterpret_cast<uint32_t*>(tile + r * 128 + (((lane >> 2) ^ (r & 7)) << 4) + (lane & 3) * 4); };
-      if (e.staged == 2 && e.residual) {
-        const uint16_t* r0 = static_cast<const uint16_t*>(e.residual) + row0 * e.residual_stride + col0;
+      uint32_t ends = 0;
+      const uint16_t* r0 = static_cast<const uint16_t*>(e.residual) + row0 * e.residual_stride + col0;
+      if (!PROMOTE && e.staged == 2 && e.residual) {
+        if (len == CH) {
+          ends = begin_rows(r0, e.residual_stride, rows, lane, word);
+        } else {
 #pragma unroll 1
-        for (int r = 0; r < rows; r += 8) {
-          RowWord raw[8];
+          for (int r = 0; r < rows; r += 8) {
+            RowWord raw[8];
 #pragma unroll
-          for (int i = 0; i < 8; ++i) raw[i] = load_row_word(r0 + (r + i) * e.residual_stride, r + i < rows ? len : 0, lane);
+            for (int i = 0; i < 8; ++i) raw[i] = load_row_word(r0 + (r + i) * e.residual_stride, r + i < rows ? len : 0, lane);
 #pragma unroll
-          for (int i = 0; i < 8; ++i) *word(r + i) = row_columns(raw[i], odd_row(r0 + (r + i) * e.residual_stride), lane);
+            for (int i = 0; i < 8; ++i) *word(r + i) = row_columns(raw[i], odd_row(r0 + (r + i) * e.residual_stride), lane);
+          }
+          __syncwarp();
         }
-        __syncwarp();
       }
       if constexpr (PROMOTE) {
         float acc[kCols];
@@ -1104,6 +1170,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairTileSmem<BN>::kT
             if (!mbar_wait_cta_warp(&rfull[w], turn, nullptr, wait_code(4, 8 + w % 8, w, turn, 0))) ok = false;
             turn ^= 1;
           }
+          if (e.residual && e.staged == 2 && len == CH) finish_rows(r0, e.residual_stride, rows, lane, ends, word);
 #pragma unroll 1
           for (int c = 0; c < kCols; c += 32) {
             uint32_t r[2][16];
@@ -1119,8 +1186,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairTileSmem<BN>::kT
           if (e.staged == 2) {
             __syncwarp();
             uint16_t* y0 = static_cast<uint16_t*>(e.y) + row0 * e.y_stride + col0;
+            if (len == CH) {
+              store_rows(y0, e.y_stride, rows, lane, tile, word);
+            } else {
 #pragma unroll 4
-            for (int r = 0; r < rows; ++r) store_row_word(y0 + r * e.y_stride, len, lane, *word(r));
+              for (int r = 0; r < rows; ++r) store_row_word(y0 + r * e.y_stride, len, lane, *word(r));
+            }
             __syncwarp();
             continue;
           }

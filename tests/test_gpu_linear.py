@@ -135,6 +135,18 @@ def test_linear_many_tiles(M, N, K, dtype, out_dtype):
     _check(y, x, w, bias, None, "silu", out_dtype)
 
 
+@pytest.mark.parametrize("N,wide,off", [(2306, 2400, 0), (2306, 2401, 5), (2307, 2400, 1), (2307, 2307, 0), (2312, 2322, 3)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_linear_many_tiles_on_odd_rows(N, wide, off, dtype):
+    """Rows of the result and of the residual on word boundaries, between them, and on each in turn."""
+    M, K = 2593, 264
+    x, w = _operands(M, N, K, dtype, seed=9)
+    residual = torch.randn(M, wide, device=DEV).to(dtype)[:, off:off + N]
+    for r in (None, residual, residual[:1].expand(M, N)):
+        got = _cdg().linear(x, w, None, r, activation="silu")
+        _check(got, x, w, None, r, "silu", dtype)
+
+
 def test_linear_preactivation_output():
     x, w = _operands(130, 200, 96, torch.float16, seed=2)
     bias = torch.randn(200, device=DEV).half()
