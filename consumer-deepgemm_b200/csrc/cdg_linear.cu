@@ -316,7 +316,7 @@ Plan make_plan(int64_t M, int64_t N, int64_t k_steps, bool narrow, int sms) {
   }
   const int64_t pairs = std::max(1, sms / 2), pair_tiles = (M + 255) / 256 * ((N + 255) / 256);
   const double waves = static_cast<double>((pair_tiles + pairs - 1) / pairs);
-  if (k_steps > 0 && 4.0 + waves * (2.6 + 0.293 * static_cast<double>(k_steps) + (narrow ? 2.0 : 0.0)) < least)
+  if (k_steps > 0 && 4.0 + waves * (2.6 + 0.293 * static_cast<double>(k_steps) + (narrow ? 3.0 : 0.0)) < least)
     best.kind = Plan::kPairs;
   return best;
 }
