@@ -359,7 +359,7 @@ __global__ void __launch_bounds__(WARPS * 32, N <= 16 ? 2 : 1) moe_route_kernel(
     if (valid) ++tokens;
     if (a.renormalize) {
       const float total = lanes_sum<LANES>(w);
-      w = total > 0.0f ? __fdividef(w, total) : 0.0f;
+      w = total <= 0.0f ? 0.0f : w == total ? 1.0f : __fdividef(w, total);  // a lone choice: 1 exactly
     }
     if (sub < a.k && row < a.T) {
       a.ids[row * a.k + sub] = id;
@@ -569,9 +569,8 @@ __global__ void __launch_bounds__(WARPS * 32, N <= 16 ? 2 : 1) moe_route_backwar
           const float l = clean_logit(to_f(logits[row * a.stride + id]));
           c = SIGMOID ? sigmoid_fast(l) : exp_fast(l - shift) * inv;
         }
-        float chosen = lanes_sum<LANES>(c);
-        chosen = chosen > 0.0f ? __fdividef(1.0f, chosen) : 1.0f;
-        g = (g - lanes_sum<LANES>(g * c) * chosen) * chosen;
+        const float sum = lanes_sum<LANES>(c), chosen = sum > 0.0f ? __fdividef(1.0f, sum) : 1.0f;
+        g = (g - lanes_sum<LANES>(g * (c == sum ? 1.0f : c * chosen))) * chosen;  // nothing moves a weight of 1
       }
       if (id >= 0) atomicAdd(&sg[id], g);
       __syncwarp();

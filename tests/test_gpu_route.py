@@ -147,6 +147,16 @@ def test_route_bias_moves_the_choice_only():
         assert int(o.tokens) == valid and int(o.counts[17]) == 0 and int(o.counts[9]) == 0
 
 
+@pytest.mark.parametrize("E", [1, 5, 64, 161, 256, 700])
+@pytest.mark.parametrize("scoring", ["softmax", "sigmoid"])
+def test_route_a_lone_choice_has_the_weight_one_and_no_gradient(E, scoring):
+    z, mask = _logits(777, E, torch.float32, seed=6)
+    o = _cdg().moe_route(z, 1, scoring=scoring, token_mask=mask)
+    assert torch.equal(o.weights[:, 0], mask.float())
+    g = _cdg().moe_route_backward(z, o.ids, torch.randn(777, 1, device=DEV), scoring=scoring)
+    assert float(g.abs().max()) == 0
+
+
 def test_route_strides_streams_and_uint8_mask():
     big = torch.randn(100, 300, device=DEV)
     z = big[:, 11:211]
