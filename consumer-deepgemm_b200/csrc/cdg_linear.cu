@@ -42,12 +42,15 @@ EncodeTiledFn encode_tiled() {
 }
 
 // Copies rows of 16-bit values to rows of `out_stride` columns, zeros past `cols`; one or two
-// matrices (blockIdx.y).  1237 x 1030 and 2050 x 1030 together: 7 us, 5 us of the call they belong to.
+// matrices (blockIdx.y).  A warp takes 256 columns of a row, so that few long rows are as many warps as
+// many short ones (with a warp per row, 192 x 5729 took 27 us, now 4); a row on an odd boundary is read in the
+// words that its columns share.
 struct Repack {
   const uint16_t* in;
   int64_t in_stride, rows, cols;
   uint16_t* out;
   int64_t out_stride;
+  int64_t parts;  // of 256 columns per row
 };
 
 __global__ void __launch_bounds__(256) repack_rows_kernel(const Repack first, const Repack second) {
@@ -55,27 +58,30 @@ __global__ void __launch_bounds__(256) repack_rows_kernel(const Repack first, co
   grid_launch_dependents();
   const Repack p = blockIdx.y == 0 ? first : second;
   const int lane = threadIdx.x & 31;
-  // whole words where every row starts on a 4-byte boundary
-  const bool even = p.in_stride % 2 == 0 && reinterpret_cast<uintptr_t>(p.in) % 4 == 0;
-  for (int64_t r = (static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x) >> 5; r < p.rows;
-       r += (static_cast<int64_t>(gridDim.x) * blockDim.x) >> 5) {
-    const uint16_t* from = p.in + r * p.in_stride;
-    uint16_t* to = p.out + r * p.out_stride;
-#pragma unroll 4
-    for (int64_t c = lane * 8; c < p.out_stride; c += 256) {
-      uint32_t w[4];
-      if (even && c + 8 <= p.cols) {
+  const int64_t warps = (static_cast<int64_t>(gridDim.x) * blockDim.x) >> 5;
+  for (int64_t item = (static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x) >> 5; item < p.rows * p.parts; item += warps) {
+    const int64_t r = item / p.parts, c = (item - r * p.parts) * 256 + lane * 8;
+    if (c >= p.out_stride) continue;
+    const uint16_t* from = p.in + r * p.in_stride + c;
+    const bool odd = reinterpret_cast<uintptr_t>(from) % 4 != 0;
+    uint32_t w[4];
+    if (!odd && c + 8 <= p.cols) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) w[j] = __ldg(reinterpret_cast<const uint32_t*>(from + c) + j);
-      } else {
+      for (int j = 0; j < 4; ++j) w[j] = __ldg(reinterpret_cast<const uint32_t*>(from) + j);
+    } else if (odd && c > 0 && c + 9 <= p.cols) {
+      uint32_t shared[5];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const uint32_t lo = c + 2 * j < p.cols ? from[c + 2 * j] : 0, hi = c + 2 * j + 1 < p.cols ? from[c + 2 * j + 1] : 0;
-          w[j] = lo | (hi << 16);
-        }
+      for (int j = 0; j < 5; ++j) shared[j] = __ldg(reinterpret_cast<const uint32_t*>(from - 1) + j);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) w[j] = (shared[j] >> 16) | (shared[j + 1] << 16);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const uint32_t lo = c + 2 * j < p.cols ? from[2 * j] : 0, hi = c + 2 * j + 1 < p.cols ? from[2 * j + 1] : 0;
+        w[j] = lo | (hi << 16);
       }
-      *reinterpret_cast<uint4*>(to + c) = make_uint4(w[0], w[1], w[2], w[3]);
     }
+    *reinterpret_cast<uint4*>(p.out + r * p.out_stride + c) = make_uint4(w[0], w[1], w[2], w[3]);
   }
 }
 
@@ -189,8 +195,9 @@ int repack(Matrix* a, Matrix* b, uint8_t*& ws, cudaStream_t st) {
   for (Matrix* m : {a, b}) {
     if (!m || tma_rows(*m)) continue;
     const int64_t stride = padded(m->cols);
-    todo[n++] = Repack{static_cast<const uint16_t*>(m->p), m->stride, m->rows, m->cols, reinterpret_cast<uint16_t*>(ws), stride};
-    most = std::max(most, m->rows);
+    const int64_t parts = (stride + 255) / 256;
+    todo[n++] = Repack{static_cast<const uint16_t*>(m->p), m->stride, m->rows, m->cols, reinterpret_cast<uint16_t*>(ws), stride, parts};
+    most = std::max(most, m->rows * parts);
     const size_t bytes = repack_bytes(*m);
     m->p = ws;
     m->stride = stride;
