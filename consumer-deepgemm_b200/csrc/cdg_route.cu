@@ -14,7 +14,7 @@
 //
 // Sixteen lanes take a row (32 where the choice is long or the experts are many), lane l the experts l,
 // l + 16, ...; a row is read once and its next row's loads are in flight meanwhile.  Bound by
-// instructions (about 300 a row forward, most of them the choice), not by memory: one B200,
+// instructions (357 a row forward, most of them the choice), not by memory: one B200,
 // calls in a row, 32,768 x 256 FP32, k = 8 with the balance loss 20.8 us forward (1.7 TB/s) and 16.8 us
 // backward (4.0 TB/s); 64 x 256 4.9 us and 3.2 us.
 #include <cuda_bf16.h>
