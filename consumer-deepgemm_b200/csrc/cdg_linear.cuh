@@ -72,8 +72,8 @@ __device__ __forceinline__ float fast_sigmoid(float v) { return __fdividef(1.0f,
 
 // Phi(-|z|), the normal distribution's tail, = erfc(|z| / sqrt 2) / 2 by Abramowitz and Stegun,
 // Handbook of Mathematical Functions, formula 7.1.26 (erfc(x) = t (a1 + t (a2 + ...)) exp(-x^2),
-// t = 1 / (1 + p x), error below 1.5e-7).  The tail itself, not 1 + erf, so that nothing cancels; a
-// third of erff's instructions, which an epilogue that no product hides is bound by.
+// t = 1 / (1 + p x), error below 1.5e-7).  The tail itself, not 1 + erf, so that nothing cancels; an
+// epilogue that no product hides is bound by its instructions.
 __device__ __forceinline__ float normal_tail(float z) {
   const float a = fabsf(z);
   const float t = __fdividef(1.0f, fmaf(0.3275911f * 0.70710678f, a, 1.0f));

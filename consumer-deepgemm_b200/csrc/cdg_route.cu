@@ -54,7 +54,7 @@ __device__ __forceinline__ float key_value(uint32_t key) {
 // Fast exponential and division (errors of a few units in the last place): the gate's weights
 // and gradients stay within 1e-6 of the exact ones.
 __device__ __forceinline__ float exp_fast(float v) {
-  // 2^(v log2 e), results below the normal range taken as 0 (__expf spends three instructions on them)
+  // 2^(v log2 e), results below the normal range taken as 0: no weight or gradient needs them
   float r;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v * 1.4426950408889634f));
   return r;
