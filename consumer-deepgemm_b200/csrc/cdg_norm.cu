@@ -54,21 +54,25 @@ __device__ __forceinline__ float cta_sum(float v, float* slot, int warps) {
   return t;
 }
 
-// Scale and reciprocal factor of a 128-column block with the largest magnitude `amax`.  A NaN
-// among the values does not reach the scale (fmaxf passes over it); its own code is NaN.  The FP32
-// recipe's scale and factor are a product and a fast division (two units in the last place); the
-// power-of-two recipe needs amax / 448 exactly, since its exponent is rounded up.
-__device__ __forceinline__ float block_scale(float amax, int pow2, float& factor) {
+// Scale and factor of a 128-column block with the largest magnitude `amax`.
+// The scale is that of cdg_quant_fp8_rows bit for bit, and a code is e4m3 of y times the factor.
+// Both are correctly rounded quotients: the FP32 recipe's code can differ from e4m3(y / amax * 448) only
+// where a rounding point of e4m3 lies within 4 * 2^-24 of the value.  A NaN among the values does not
+// reach the scale (fmaxf passes over it); its own code is NaN.  With the FP32 recipe even lanes divide
+// for the scale, which is theirs alone, and odd ones for the factor: calls of 32,768 x 4096 BF16 take
+// 1.3% longer than with approximate divisions, 2.0% with two divisions a lane.
+__device__ __forceinline__ float block_scale(float amax, int pow2, int lane, float& factor) {
   amax = fmaxf(amax, 1e-12f);
   if (pow2) {
     uint32_t b = __float_as_uint(amax / 448.0f);
     if (b & 0x007FFFFFu) b = (b & 0xFF800000u) + 0x00800000u;
-    const float scale = __uint_as_float(b);
-    factor = 1.0f / scale;
-    return scale;
+    factor = 1.0f / __uint_as_float(b);
+    return __uint_as_float(b);
   }
-  factor = __fdividef(448.0f, amax);
-  return amax * (1.0f / 448.0f);
+  const bool odd = lane & 1;
+  const float quotient = (odd ? 448.0f : amax) / (odd ? amax : 448.0f);
+  factor = __shfl_sync(0xffffffffu, quotient, lane | 1);
+  return quotient;
 }
 
 struct NormFwd {
@@ -96,7 +100,7 @@ __device__ __forceinline__ void quant_chunk(const NormFwd& a, int64_t row, int64
 #pragma unroll
     for (int o = 8; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
     float f;
-    const float scale = block_scale(m, a.pow2, f);
+    const float scale = block_scale(m, a.pow2, lane, f);
     const int64_t c = column<true>(chunk, lane, 0);
     if (c >= a.H) return;
     uint32_t p[2];
@@ -118,7 +122,7 @@ __device__ __forceinline__ void quant_chunk(const NormFwd& a, int64_t row, int64
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
       float f;
-      const float scale = block_scale(m, a.pow2, f);
+      const float scale = block_scale(m, a.pow2, lane, f);
       uint8_t* to = q + column<false>(chunk, lane, 4 * b);
       const bool full = (kb + b + 1) * 128 <= a.H;
 #pragma unroll

@@ -254,3 +254,36 @@ def test_norm_refusals():
         cdg.add_rms_norm(x.cpu(), w)
     with pytest.raises(RuntimeError):
         cdg.add_rms_norm(torch.zeros(1, 32769, device=DEV), torch.ones(32769, device=DEV))
+
+
+@pytest.mark.parametrize("T,H", [(3000, 1024), (5, 4096), (300, 640)])
+@pytest.mark.parametrize("ue8m0", [False, True])
+def test_norm_codes_are_the_quantisers(T, H, ue8m0):
+    """Scales of the FP32 y bit for bit those of the framework's quantiser.  Codes: e4m3 of y * (448 / amax)
+    against e4m3 of y / amax * 448, each two roundings: equal but where a rounding point of e4m3 lies
+    within 4u of the value, and then one step apart; a power-of-two scale divides exactly."""
+    from consumer_deep_gemm import native
+
+    for offset in (0, 1):  # rows on 16-byte boundaries, or not
+        x = torch.randn(T, H + 1, device=DEV)[:, offset:offset + H]
+        w = torch.rand(H, device=DEV) + 0.5
+        o = _cdg().add_rms_norm(x, w, quantize=True, ue8m0=ue8m0)
+        q, scale = native.require().quant_fp8_rows(o.y, ue8m0)
+        assert torch.equal(o.scale.view(torch.int32), scale.view(torch.int32))
+        a, b = o.q.double(), q.view(torch.float8_e4m3fn).double()
+        if ue8m0:
+            assert torch.equal(a, b)
+            continue
+        amax = o.y.double().view(T, H // 128, 128).abs().amax(2, keepdim=True)
+        v = (o.y.double().view(T, H // 128, 128) / amax * 448).view(T, H)
+        apart = a != b
+        assert bool(((a - b).abs() <= _e4m3_steps(v))[apart].all())
+        assert bool((((a + b) / 2 - v).abs() <= 4 * U * v.abs())[apart].all())
+
+
+@pytest.mark.parametrize("T,H", [(5, 136), (700, 8), (3, 392), (4, 1), (6, 129), (3, 16392)])
+@pytest.mark.parametrize("ue8m0", [False, True])
+def test_norm_last_blocks_of_a_few_columns(T, H, ue8m0):
+    x, w, r = _inputs(T, H, torch.float32, torch.float32, True, seed=17)
+    o = _cdg().add_rms_norm(x, w, r, quantize=True, ue8m0=ue8m0)
+    _check_quant(_norm64(x, w, r, 1e-6)[1], o.q, o.scale, pow2=ue8m0)
