@@ -529,7 +529,7 @@ int cdg_rms_norm_backward(const cdg_norm_backward_args* g, void* workspace, size
   if (g->H > kNormMaxH || g->T >= int64_t(1) << 31) return CDG_ERR_UNSUPPORTED;
   if (g->T > 0 && (!g->dy || !g->h || !g->dx)) return CDG_ERR_INVALID_ARGUMENT;
   if (!workspace || workspace_bytes < cdg_rms_norm_backward_workspace_bytes(g->T, g->H)) return CDG_ERR_WORKSPACE;
-  if (reinterpret_cast<uintptr_t>(workspace) % 4) return CDG_ERR_ALIGNMENT;
+  if (reinterpret_cast<uintptr_t>(workspace) % 16) return CDG_ERR_ALIGNMENT;  // sums leave four at a time
   NormBwd a{g->dy, g->h, g->w, g->dh, g->dx, static_cast<float*>(workspace), g->dy_stride, g->h_stride, g->dh_stride,
             g->dx_stride, g->T, g->H, g->eps, g->w_dtype == CDG_DTYPE_F32};
   const int64_t e = element_size(g->dtype);

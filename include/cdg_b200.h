@@ -521,7 +521,8 @@ int cdg_add_rms_norm(const cdg_norm_args* args, cdg_stream_t stream);
  * s = 1 / sqrt(mean(h^2) + eps),
  *   dx = dh + s * (u - h * s^2 * mean(u * h)),   dw[c] = sum over rows of dy * h * s.
  * dh (the gradient that reaches h by the residual stream) may be NULL.  dx is the gradient of x
- * and of r alike.  dw is of w's type and summed in a fixed order. */
+ * and of r alike.  dw is of w's type; its sums' order is fixed by the sizes, the types, whether the rows lie on
+ * 16-byte boundaries, and the GPU's SM count.  The workspace must start on a 16-byte boundary. */
 typedef struct cdg_norm_backward_args {
   const void* dy;
   int64_t dy_stride;
@@ -553,7 +554,7 @@ int cdg_rms_norm_backward(const cdg_norm_backward_args* args, void* workspace, s
  *   *loss = E / (topk V^2) * sum over e of counts[e] * (sum over valid tokens of p[e]),
  * 1 where the experts share rows and probabilities evenly, 0 without a valid token.  The sums
  * over tokens do not depend on the order in which CTAs finish.
- * E up to 1024, topk up to 32, T up to 2^23. */
+ * E up to 1024, topk up to 32, T up to 2^23.  The workspace must start on an 8-byte boundary. */
 #define CDG_SCORE_SOFTMAX 0
 #define CDG_SCORE_SIGMOID 1
 
@@ -606,7 +607,8 @@ int cdg_moe_route_backward(const cdg_route_backward_args* args, cdg_stream_t str
  * not NULL, receives z [M, N] in `dtype` (the backward call's z).  Sums are FP32; for an F32 y no
  * running sum of the tensor cores covers more than 512 of K.  K = 0 gives act(bias) + residual.
  * The workspace holds operands whose rows do not start on 16-byte boundaries (0 bytes when both do;
- * then it may be NULL). */
+ * then it may be NULL); it must start on a 16-byte boundary.  y and z_out may not overlap each other or
+ * an input. */
 #define CDG_ACT_NONE 0
 #define CDG_ACT_RELU 1
 #define CDG_ACT_SILU 2      /* z / (1 + exp(-z)) */
@@ -637,7 +639,8 @@ int cdg_linear(const cdg_linear_args* args, void* workspace, size_t workspace_by
  *   dz = dy * act'(z),  dx = dz w,  dw = dz^T x,  db = sum over rows of dz.
  * dy, x, w, z, dx, dw are of `dtype`; db of `dtype` or F32.  dx, dw and db may each be NULL.  z (the
  * forward call's z_out) is read only with an activation; dz, an operand of both products, is held
- * in `dtype`, db sums its FP32 values in a fixed order. */
+ * in `dtype`, db sums its FP32 values in an order that the sizes, whether the rows lie on 16-byte
+ * boundaries, and the GPU's SM count fix.  The workspace, where one is needed, must start on a 16-byte boundary. */
 typedef struct cdg_linear_backward_args {
   const void* dy;
   int64_t dy_stride;

@@ -133,3 +133,13 @@ def test_normal_tail_formula():
     poly = t * (0.254829592 + t * (-0.284496736 + t * (1.421413741 + t * (-1.453152027 + t * 1.061405429))))
     tail = 0.5 * poly * torch.exp(-0.5 * a * a)
     assert float((tail - torch.special.ndtr(-a)).abs().max()) < 0.5 * 1.5e-7 + 1e-8
+
+
+def test_norm_backward_workspace_alignment():
+    """Partial sums are stored 16 bytes at a time: a workspace on a lesser boundary is refused on the host."""
+    lib = cabi.lib()
+    lib.cdg_rms_norm_backward.argtypes = [ctypes.POINTER(NormBackwardArgs), P, ctypes.c_size_t, P]
+    g = NormBackwardArgs(dy=FAKE, dy_stride=256, h=FAKE, h_stride=256, w=FAKE, dtype=BF16, w_dtype=BF16, T=4, H=256,
+                         eps=1e-6, dx=FAKE, dx_stride=256, dw=FAKE)
+    for off in (4, 8, 12, 1):
+        assert lib.cdg_rms_norm_backward(ctypes.byref(g), P(FAKE + off), 1 << 20, None) == ALIGNMENT
