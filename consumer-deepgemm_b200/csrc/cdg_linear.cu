@@ -493,6 +493,10 @@ int check_forward(const cdg_linear_args* g) {
   if (g->residual && g->residual_dtype != g->dtype && g->residual_dtype != CDG_DTYPE_F32)
     return CDG_ERR_INVALID_ARGUMENT;
   if (g->M > 0 && g->N > 0 && (!g->y || (g->K > 0 && (!g->x || !g->w)))) return CDG_ERR_INVALID_ARGUMENT;
+  if (!on_boundary(2, {g->x, g->w, g->z_out}) || !on_boundary(element_size(g->out_dtype), {g->y}) ||
+      (g->bias && !on_boundary(element_size(g->bias_dtype), {g->bias})) ||
+      (g->residual && !on_boundary(element_size(g->residual_dtype), {g->residual})))
+    return CDG_ERR_ALIGNMENT;
   return sizes_ok(g->M, g->N, g->K) ? CDG_OK : CDG_ERR_UNSUPPORTED;
 }
 
@@ -503,6 +507,8 @@ int check_backward(const cdg_linear_backward_args* g) {
   if (g->M > 0 && g->N > 0 && (!g->dy || (g->activation != CDG_ACT_NONE && !g->z))) return CDG_ERR_INVALID_ARGUMENT;
   if (g->dx && g->N > 0 && g->K > 0 && g->M > 0 && !g->w) return CDG_ERR_INVALID_ARGUMENT;
   if (g->dw && g->M > 0 && g->K > 0 && g->N > 0 && !g->x) return CDG_ERR_INVALID_ARGUMENT;
+  if (!on_boundary(2, {g->dy, g->x, g->w, g->z, g->dx, g->dw}) || (g->db && !on_boundary(element_size(g->db_dtype), {g->db})))
+    return CDG_ERR_ALIGNMENT;
   return sizes_ok(g->M, g->N, g->K) ? CDG_OK : CDG_ERR_UNSUPPORTED;
 }
 

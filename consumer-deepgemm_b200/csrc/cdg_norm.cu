@@ -500,6 +500,9 @@ int cdg_add_rms_norm(const cdg_norm_args* g, cdg_stream_t stream) {
   if (g->H > kNormMaxH || g->T >= int64_t(1) << 31) return CDG_ERR_UNSUPPORTED;
   if (g->T == 0) return CDG_OK;
   if (!g->x || !g->w || (g->q && !g->s) || (!g->y && !g->q && !g->h)) return CDG_ERR_INVALID_ARGUMENT;
+  if (!on_boundary(element_size(g->dtype), {g->x, g->r, g->h, g->y}) || !on_boundary(element_size(g->w_dtype), {g->w}) ||
+      !on_boundary(4, {g->s}))
+    return CDG_ERR_ALIGNMENT;
   NormFwd a{g->x, g->r, g->w, g->h, g->y, g->q, g->s, g->x_stride, g->r_stride, g->h_stride, g->y_stride, g->q_stride,
             g->s_stride_m, g->s_stride_k, g->T, g->H, g->eps, 1.0f / static_cast<float>(g->H), g->w_dtype == CDG_DTYPE_F32, g->scale_fmt};
   const int64_t e = element_size(g->dtype);
@@ -528,6 +531,9 @@ int cdg_rms_norm_backward(const cdg_norm_backward_args* g, void* workspace, size
   if (!(g->eps >= 0.0f) || !g->w || !g->dw) return CDG_ERR_INVALID_ARGUMENT;
   if (g->H > kNormMaxH || g->T >= int64_t(1) << 31) return CDG_ERR_UNSUPPORTED;
   if (g->T > 0 && (!g->dy || !g->h || !g->dx)) return CDG_ERR_INVALID_ARGUMENT;
+  if (!on_boundary(element_size(g->dtype), {g->dy, g->h, g->dh, g->dx}) ||
+      !on_boundary(element_size(g->w_dtype), {g->w, g->dw}))
+    return CDG_ERR_ALIGNMENT;
   if (!workspace || workspace_bytes < cdg_rms_norm_backward_workspace_bytes(g->T, g->H)) return CDG_ERR_WORKSPACE;
   if (reinterpret_cast<uintptr_t>(workspace) % 16) return CDG_ERR_ALIGNMENT;  // sums leave four at a time
   NormBwd a{g->dy, g->h, g->w, g->dh, g->dx, static_cast<float*>(workspace), g->dy_stride, g->h_stride, g->dh_stride,

@@ -712,6 +712,9 @@ int cdg_moe_route(const cdg_route_args* g, void* workspace, size_t workspace_byt
   if (g->scoring != CDG_SCORE_SOFTMAX && g->scoring != CDG_SCORE_SIGMOID) return CDG_ERR_INVALID_ARGUMENT;
   if (g->E > kRouteMaxExperts || g->topk > kRouteMaxTopk || g->T > kRouteMaxTokens) return CDG_ERR_UNSUPPORTED;
   if (!g->counts || !g->tokens || (g->T > 0 && (!g->logits || !g->weights || !g->ids))) return CDG_ERR_INVALID_ARGUMENT;
+  if (!on_boundary(element_size(g->dtype), {g->logits}) ||
+      !on_boundary(4, {g->bias, g->weights, g->ids, g->counts, g->tokens, g->loss}))
+    return CDG_ERR_ALIGNMENT;
   if (!workspace || workspace_bytes < cdg_moe_route_workspace_bytes(g->E)) return CDG_ERR_WORKSPACE;
   if (reinterpret_cast<uintptr_t>(workspace) % 8) return CDG_ERR_ALIGNMENT;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
@@ -763,6 +766,9 @@ int cdg_moe_route_backward(const cdg_route_backward_args* g, cdg_stream_t stream
   if (g->grad_loss && (!g->counts || !g->tokens)) return CDG_ERR_INVALID_ARGUMENT;
   if (g->T == 0) return CDG_OK;
   if (!g->logits || !g->ids || !g->dlogits || (!g->grad_weights && !g->grad_loss)) return CDG_ERR_INVALID_ARGUMENT;
+  if (!on_boundary(element_size(g->dtype), {g->logits, g->dlogits}) ||
+      !on_boundary(4, {g->ids, g->grad_weights, g->grad_loss, g->counts, g->tokens}))
+    return CDG_ERR_ALIGNMENT;
   RouteBwd a{g->logits, g->stride, g->ids, g->grad_weights, g->grad_loss, g->counts, g->tokens, g->T,
              static_cast<int>(g->E), static_cast<int>(g->topk), g->scoring == CDG_SCORE_SIGMOID, g->renormalize != 0,
              g->scale, g->dlogits, g->d_stride};

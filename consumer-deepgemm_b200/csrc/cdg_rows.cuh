@@ -7,6 +7,7 @@
 #include <cuda_runtime.h>
 
 #include <cstdint>
+#include <initializer_list>
 
 #include "cdg_b200.h"
 #include "cdg_ptx.cuh"
@@ -229,6 +230,14 @@ inline int element_size(int dtype) { return dtype == CDG_DTYPE_F32 ? 4 : 2; }
 
 inline bool row_dtype(int dtype) {
   return dtype == CDG_DTYPE_BF16 || dtype == CDG_DTYPE_F16 || dtype == CDG_DTYPE_F32;
+}
+
+// Whether each pointer lies on a boundary of its type's `bytes` (absent ones do): what a kernel's loads and
+// stores of single elements need.
+inline bool on_boundary(int64_t bytes, std::initializer_list<const void*> pointers) {
+  for (const void* p : pointers)
+    if (reinterpret_cast<uintptr_t>(p) % bytes) return false;
+  return true;
 }
 
 // Whether every row of a tensor starts on a 16-byte boundary (absent tensors do).

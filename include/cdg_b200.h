@@ -485,7 +485,8 @@ const char* cdg_status_string(int status);
 /* ---------------------------------------------------------------------------------------------
  * What stands around the experts in a mixture-of-experts block: the norm before them, the router
  * and dense products.  None of these exist in the reference (it ships the GEMM only).
- * Strides are in elements; last dimensions have unit stride.
+ * Strides are in elements; last dimensions have unit stride; pointers lie on their type's boundary
+ * (CDG_ERR_ALIGNMENT otherwise).
  * ------------------------------------------------------------------------------------------- */
 
 /* RMS norm with the residual's addition and an e4m3 output.  For each of T rows of H columns:

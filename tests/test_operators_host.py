@@ -143,3 +143,76 @@ def test_norm_backward_workspace_alignment():
                          eps=1e-6, dx=FAKE, dx_stride=256, dw=FAKE)
     for off in (4, 8, 12, 1):
         assert lib.cdg_rms_norm_backward(ctypes.byref(g), P(FAKE + off), 1 << 20, None) == ALIGNMENT
+
+
+class RouteBackwardArgs(ctypes.Structure):
+    _fields_ = [("logits", P), ("stride", I64), ("dtype", I32), ("scoring", I32), ("ids", P), ("grad_weights", P),
+                ("grad_loss", P), ("counts", P), ("tokens", P), ("T", I64), ("E", I64), ("topk", I64),
+                ("renormalize", I32), ("scale", F32), ("dlogits", P), ("d_stride", I64)]
+
+
+class LinearBackwardArgs(ctypes.Structure):
+    _fields_ = [("dy", P), ("dy_stride", I64), ("x", P), ("x_stride", I64), ("w", P), ("w_stride", I64), ("z", P),
+                ("z_stride", I64), ("dtype", I32), ("db_dtype", I32), ("activation", I32), ("M", I64), ("N", I64),
+                ("K", I64), ("dx", P), ("dx_stride", I64), ("dw", P), ("dw_stride", I64), ("db", P)]
+
+
+def test_pointers_off_their_types_boundary_are_refused():
+    """Each pointer in turn one byte past FAKE (16-bit types) or two bytes past it (32-bit types)."""
+    lib = cabi.lib()
+
+    def each(entry, make, names, off, rest):
+        fn = getattr(lib, entry)
+        fn.argtypes = None
+        for name in names:
+            g = make()
+            setattr(g, name, FAKE + off)
+            assert fn(ctypes.byref(g), *rest) == ALIGNMENT, (entry, name)
+
+    ws = (P(FAKE), ctypes.c_size_t(1 << 24), None)
+
+    def norm(dtype=BF16):
+        return NormArgs(x=FAKE, x_stride=256, r=FAKE, r_stride=256, w=FAKE, dtype=dtype, w_dtype=dtype, T=4, H=256,
+                        eps=1e-6, h=FAKE, h_stride=256, y=FAKE, y_stride=256, q=FAKE, q_stride=256, s=FAKE,
+                        s_stride_m=2, s_stride_k=1)
+
+    each("cdg_add_rms_norm", norm, ["x", "r", "w", "h", "y", "s"], 1, (None,))
+    each("cdg_add_rms_norm", lambda: norm(FP32), ["x", "r", "w", "h", "y", "s"], 2, (None,))
+
+    def norm_backward(dtype=F16):
+        return NormBackwardArgs(dy=FAKE, dy_stride=256, h=FAKE, h_stride=256, w=FAKE, dh=FAKE, dh_stride=256, dtype=dtype,
+                                w_dtype=FP32, T=4, H=256, eps=1e-6, dx=FAKE, dx_stride=256, dw=FAKE)
+
+    each("cdg_rms_norm_backward", norm_backward, ["dy", "h", "dh", "dx"], 1, ws)
+    each("cdg_rms_norm_backward", lambda: norm_backward(FP32), ["dy", "h", "dh", "dx", "w", "dw"], 2, ws)
+
+    def route(dtype=BF16):
+        return RouteArgs(logits=FAKE, stride=64, dtype=dtype, bias=FAKE, T=4, E=64, topk=8, renormalize=1, scale=1.0,
+                         weights=FAKE, ids=FAKE, counts=FAKE, tokens=FAKE, loss=FAKE)
+
+    each("cdg_moe_route", route, ["logits"], 1, ws)
+    each("cdg_moe_route", lambda: route(FP32), ["logits", "bias", "weights", "ids", "counts", "tokens", "loss"], 2, ws)
+
+    def route_backward(dtype=BF16):
+        return RouteBackwardArgs(logits=FAKE, stride=64, dtype=dtype, ids=FAKE, grad_weights=FAKE, grad_loss=FAKE,
+                                 counts=FAKE, tokens=FAKE, T=4, E=64, topk=8, scale=1.0, dlogits=FAKE, d_stride=64)
+
+    each("cdg_moe_route_backward", route_backward, ["logits", "dlogits"], 1, (None,))
+    each("cdg_moe_route_backward", lambda: route_backward(FP32),
+         ["logits", "dlogits", "ids", "grad_weights", "grad_loss", "counts", "tokens"], 2, (None,))
+
+    def product(out=BF16):
+        return LinearArgs(x=FAKE, x_stride=64, w=FAKE, w_stride=64, bias=FAKE, residual=FAKE, residual_stride=8,
+                          dtype=BF16, bias_dtype=out, residual_dtype=out, out_dtype=out, M=4, N=8, K=64, y=FAKE,
+                          y_stride=8, z_out=FAKE, z_stride=8)
+
+    each("cdg_linear", product, ["x", "w", "bias", "residual", "y", "z_out"], 1, ws)
+    each("cdg_linear", lambda: product(FP32), ["bias", "residual", "y"], 2, ws)
+
+    def product_backward():
+        return LinearBackwardArgs(dy=FAKE, dy_stride=8, x=FAKE, x_stride=64, w=FAKE, w_stride=64, z=FAKE, z_stride=8,
+                                  dtype=BF16, db_dtype=FP32, activation=2, M=4, N=8, K=64, dx=FAKE, dx_stride=64,
+                                  dw=FAKE, dw_stride=64, db=FAKE)
+
+    each("cdg_linear_backward", product_backward, ["dy", "x", "w", "z", "dx", "dw"], 1, ws)
+    each("cdg_linear_backward", product_backward, ["db"], 2, ws)
