@@ -421,6 +421,7 @@ int dz_groups(int64_t M, int64_t N) {
 }
 
 bool needs_dz(const cdg_linear_backward_args* g) {
+  if (g->M == 0 || g->N == 0) return false;  // no elements (and torch gives [M, 0] a row stride of 1)
   return g->activation != CDG_ACT_NONE || !tma_rows(Matrix{g->dy, g->dy_stride, g->M, g->N});
 }
 
@@ -431,7 +432,7 @@ int backward(const cdg_linear_backward_args* g, uint8_t* ws, cudaStream_t st) {
   Matrix x{g->x, g->x_stride, g->M, g->K}, w{g->w, g->w_stride, g->N, g->K};
   Matrix dz{g->dy, g->dy_stride, g->M, g->N};
   const bool store = needs_dz(g) && (g->dx || g->dw);
-  if ((store || g->db) && g->M > 0) {
+  if ((store || g->db) && g->M > 0 && g->N > 0) {
     T* out = nullptr;
     const int64_t stride = padded(g->N);
     if (store) {
@@ -461,7 +462,7 @@ int backward(const cdg_linear_backward_args* g, uint8_t* ws, cudaStream_t st) {
       dz.p = out;
       dz.stride = stride;
     }
-  } else if (g->db) {
+  } else if (g->db && g->N > 0) {
     if (cudaMemsetAsync(g->db, 0, g->N * element_size(g->db_dtype), st) != cudaSuccess) return CDG_ERR_CUDA;
   }
   if (g->dx) {
@@ -546,8 +547,8 @@ size_t cdg_linear_backward_workspace_bytes(const cdg_linear_backward_args* g) {
   using namespace cdg;
   if (check_backward(g) != CDG_OK) return 0;
   size_t n = 0;
-  if (g->M > 0 && needs_dz(g) && (g->dx || g->dw)) n += align256(static_cast<size_t>(g->M) * padded(g->N) * 2);
-  if (g->M > 0 && g->db) n += align256(static_cast<size_t>(dz_groups(g->M, g->N)) * g->N * 4);
+  if (needs_dz(g) && (g->dx || g->dw)) n += align256(static_cast<size_t>(g->M) * padded(g->N) * 2);
+  if (g->M > 0 && g->N > 0 && g->db) n += align256(static_cast<size_t>(dz_groups(g->M, g->N)) * g->N * 4);
   if (g->dx) n += repack_bytes(Matrix{g->w, g->w_stride, g->N, g->K});
   if (g->dw) n += repack_bytes(Matrix{g->x, g->x_stride, g->M, g->K});
   return n;

@@ -305,3 +305,17 @@ def test_linear_refusals():
             call()
     with pytest.raises(RuntimeError):
         cdg.linear(x.cpu(), w)
+
+
+@pytest.mark.parametrize("M,N,K", [(4, 0, 16), (1, 0, 8), (300, 0, 264), (5, 8, 0), (300, 0, 0), (0, 0, 8)])
+@pytest.mark.parametrize("act", [None, "silu"])
+@pytest.mark.parametrize("bias_grad", [False, True])
+def test_linear_backward_of_empty_products(M, N, K, act, bias_grad):
+    x, w = _operands(M, N, K, torch.bfloat16)
+    dy = torch.randn(M, N, device=DEV).bfloat16()
+    dx, dw, db = _cdg().linear_backward(dy, x, w, dy if act else None, activation=act, bias_grad=bias_grad)
+    assert dx.shape == (M, K) and dw.shape == (N, K) and float(dx.float().abs().sum()) == 0
+    assert (db is None) != bias_grad and (db is None or db.shape == (N,))
+    if bias_grad and act is None:
+        want = dy.double().sum(0)
+        assert bool(((db.double() - want).abs() <= 2.0 ** -8 * want.abs() + 2.0 ** -20 * dy.double().abs().sum(0)).all())
