@@ -7,6 +7,7 @@ layouts, plus the layout and runtime hooks vLLM calls around it
 (consumer_deep_gemm/__init__.py:11-48 of the reference, restricted to that path).
 """
 
+from .block import MoEBlock
 from .gemm import m_grouped_fp8_fp4_gemm_nt_contiguous, m_grouped_fp8_fp4_gemm_nt_masked
 from .layout import (
     get_mk_alignment_for_contiguous_layout,
@@ -37,6 +38,7 @@ __all__ = [
     "linear_backward",
     "moe_route",
     "moe_route_backward",
+    "MoEBlock",
     "get_symm_buffer_for_mega_moe",
     "fp8_fp4_mega_moe",
     "get_mn_major_tma_aligned_tensor",

@@ -216,3 +216,25 @@ def test_pointers_off_their_types_boundary_are_refused():
 
     each("cdg_linear_backward", product_backward, ["dy", "x", "w", "z", "dx", "dw"], 1, ws)
     each("cdg_linear_backward", product_backward, ["db"], 2, ws)
+
+
+def test_documented_imports():
+    """Every `from consumer_deep_gemm[.module] import ...` line of the README and the integration notes."""
+    import importlib
+    import os
+    import re
+
+    seen = set()
+    for name in ("README.md", "INTEGRATION.md"):
+        with open(os.path.join(cabi.REPO, name)) as f:
+            text = f.read()
+        for module, names in re.findall(r"^from (consumer_deep_gemm[\w.]*) import ([\w, ]+)", text, re.M):
+            for each in names.split(","):
+                assert hasattr(importlib.import_module(module), each.strip()), (name, module, each)
+                seen.add(each.strip())
+    assert {"MoEBlock", "MoELayer", "add_rms_norm", "linear", "moe_route"} <= seen
+    import consumer_deep_gemm as cdg
+
+    for each in cdg.__all__:
+        assert hasattr(cdg, each), each
+    assert "MoEBlock" in cdg.__all__
