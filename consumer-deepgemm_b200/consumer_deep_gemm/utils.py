@@ -2,12 +2,13 @@
 
 Two of them reach the kernels of libcdg_b200.so:
 
-* ``set_num_sms(n)`` limits the persistent GEMM kernels to ``n`` SMs (0 = all), e.g. to
-  leave SMs free for kernels that overlap the GEMM on another stream
+* ``set_num_sms(n)`` limits the persistent GEMM kernels, the dense product's among them, to
+  ``n`` SMs (0 = all), e.g. to leave SMs free for kernels that overlap the GEMM on another stream
   (``cdg_set_num_sms``); ``get_num_sms()`` reports the limit, or the device's SM count.
-* ``set_pdl(v)`` chooses whether the GEMM's kernels after the first are launched with
-  programmatic stream serialization (``cdg_set_pdl``; on by default in this build, where
-  every kernel waits for its predecessor on the device).
+* ``set_pdl(v)`` chooses whether the GEMM's kernels after the first, and those of the
+  norm, the router and the dense product, are launched with programmatic stream
+  serialization (``cdg_set_pdl``; on by default in this build, where every kernel waits
+  for its predecessor on the device).
 
 The reference stores all of these without reading them.  ``set_tc_util``,
 ``set_ignore_compile_dims`` and ``set_block_size_multiple_of`` tune DeepGEMM's JIT

@@ -269,8 +269,9 @@ int launch_pairs(const Matrix& A, const Matrix& B, const LinearShape& s, Epilogu
   if (rc == CDG_OK && e.staged == 1) rc = make_map(&ty, y, kOut, 32);
   if (rc == CDG_OK && e.staged == 1 && e.residual) rc = make_map(&tr, r, kOut, 32);
   if (rc != CDG_OK) return rc;
+  // The plan is made for the whole GPU, so that a limit on the SMs does not change the result's bits.
   const unsigned grid =
-      static_cast<unsigned>(2 * std::min<int64_t>(int64_t(s.m_tiles) * s.n_tiles, std::max(1, sm_count() / 2)));
+      static_cast<unsigned>(2 * std::min<int64_t>(int64_t(s.m_tiles) * s.n_tiles, std::max(1, usable_sms() / 2)));
   return launch(cdg_linear_pair_kernel<T, O, BN>, dim3(grid), PairTileSmem<BN>::kThreads, PairTileSmem<BN>::kBytes, st, ta, tb,
                 ty, tr, s, e);
 }

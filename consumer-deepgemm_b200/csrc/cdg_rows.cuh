@@ -214,6 +214,12 @@ inline int sm_count() {
   return n > 0 ? n : 148;
 }
 
+// SMs a persistent GEMM kernel may use (cdg_set_num_sms; read at every launch).
+inline int usable_sms() {
+  const int limit = cdg_get_num_sms(), all = sm_count();
+  return limit > 0 && limit < all ? limit : all;
+}
+
 constexpr int kMaxDevices = 64;
 
 // Reads a unit's device-side error record (two words) into `out`, and clears it if asked.

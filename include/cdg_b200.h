@@ -215,11 +215,11 @@ int cdg_read_device_status(const void* workspace, cdg_stream_t stream);
  * (csrc/cutlass_mxfp8_mxfp4_probe.cu:598-613, csrc/bindings.cpp:113-127). */
 int cdg_device_status(int32_t clear, int32_t* where);
 
-/* SMs the persistent GEMM kernels may use (0 = all; values above the device's count mean
- * all), e.g. to leave SMs to kernels that overlap the GEMM on another stream.  Process-wide,
- * read at every launch.  Replaces set_num_sms / get_num_sms (consumer_deep_gemm/utils.py:12-22),
- * which the reference stores without using.  cdg_get_num_sms returns the setting, or the
- * current device's SM count when it is 0. */
+/* SMs the persistent GEMM kernels, the dense product's among them (whole CTA pairs, one at least), may
+ * use (0 = all; values above the device's count mean all), e.g. to leave SMs to kernels that overlap
+ * the GEMM on another stream.  Process-wide, read at every launch.  Replaces set_num_sms / get_num_sms
+ * (consumer_deep_gemm/utils.py:12-22), which the reference stores without using.  cdg_get_num_sms
+ * returns the setting, or the current device's SM count when it is 0. */
 int cdg_set_num_sms(int32_t num_sms);
 int cdg_get_num_sms(void);
 

@@ -319,3 +319,30 @@ def test_linear_backward_of_empty_products(M, N, K, act, bias_grad):
     if bias_grad and act is None:
         want = dy.double().sum(0)
         assert bool(((db.double() - want).abs() <= 2.0 ** -8 * want.abs() + 2.0 ** -20 * dy.double().abs().sum(0)).all())
+
+
+def test_persistent_product_keeps_to_the_sm_limit():
+    """set_num_sms(2) leaves one CTA pair of the 74 a B200 has: the product of 256 tiles takes many times as long
+    (64 tiles a pair instead of four; a factor of four is asked for) and gives the same bits."""
+    cdg = _cdg()
+    x, w = _operands(4096, 4096, 1024, torch.bfloat16, seed=11)
+
+    def timed():
+        y = cdg.linear(x, w)
+        start, end = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+        torch.cuda.synchronize()
+        start.record()
+        for _ in range(5):
+            y = cdg.linear(x, w)
+        end.record()
+        end.synchronize()
+        return y, start.elapsed_time(end)
+
+    want, whole = timed()
+    cdg.set_num_sms(2)
+    try:
+        got, limited = timed()
+    finally:
+        cdg.set_num_sms(0)
+    assert torch.equal(got, want)
+    assert limited > 4 * whole, (limited, whole)
