@@ -31,7 +31,8 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] =
 
     x ``[M, K]`` and weight ``[N, K]``: both BF16 or both FP16, any row strides (rows that do not start
     on 16-byte boundaries are copied once inside the call).  bias ``[N]`` and residual ``[M, N]``:
-    x's dtype or FP32.  activation: None, ``"relu"``, ``"silu"``, ``"gelu"`` (erf) or ``"gelu_tanh"``.
+    x's dtype or FP32.  activation: None, ``"relu"``, ``"silu"``, ``"gelu"`` (erf) or ``"gelu_tanh"``,
+    in FP32 with the fast exponential (relative error 2^-19 + 2^-21 |exponent|).
     out_dtype: x's dtype (the default) or ``torch.float32``, e.g. for router logits.  Returns ``y``, or
     with ``preact=True`` ``(y, z)``, z being the value before the activation in x's dtype, which
     ``linear_backward`` takes.

@@ -346,3 +346,20 @@ def test_persistent_product_keeps_to_the_sm_limit():
         cdg.set_num_sms(0)
     assert torch.equal(got, want)
     assert limited > 4 * whole, (limited, whole)
+
+
+@pytest.mark.parametrize("rows", [1, 40, 4096])
+def test_gelu_tail_is_relatively_accurate(rows):
+    """GELU far below zero, y = z Phi(z), with z the operands' own values (x = 1, K = 1, no sum).
+
+    The tail is exp(-z^2 / 2) times a fitted factor.  The factor is within 5e-7 in FP32 and its fast division
+    within 2 units in the last place (2.4e-7); exp(x) is within 2 + 1.173 |x| units, its argument z^2 / 2 is
+    rounded once (0.25 z^2 2^-23): together within 2^-19 + z^2 2^-23.  Results below 2^-126 may be zero."""
+    z = torch.linspace(-14, 2, 2049, device=DEV).bfloat16().unique()
+    x = torch.ones(rows, 1, device=DEV).bfloat16()
+    want = z.double() * 0.5 * torch.special.erfc(-z.double() / math.sqrt(2))  # ndtr cancels below -5
+    near = (2.0 ** -19 + z.double().square() * 2.0 ** -23) * want.abs() + 2.0 ** -126
+    got = _cdg().linear(x, z[:, None].contiguous(), activation="gelu", out_dtype=torch.float32)
+    assert bool(((got.double() - want).abs() <= near).all())
+    got = _cdg().linear(x, z[:, None].contiguous(), activation="gelu")
+    assert bool(((got.double() - want).abs() <= 2.0 ** -8 * want.abs() * (1 + 2.0 ** -8) + near).all())
