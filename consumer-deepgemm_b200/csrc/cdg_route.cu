@@ -8,9 +8,14 @@
 // Over the V valid tokens: counts[e] = how often e was chosen and
 //   loss  = E / (k V^2) * sum_e counts[e] * sum_t p[t, e].
 // Gradient, with g_j = dL/dw_j * scale, a_e = dL/dloss * E counts[e] / (k V^2) (counts held fixed):
-//   renormalised: g_j <- (g_j - sum_i g_i c_i / C) / C with c the chosen scores, C their sum
-//   softmax: dl_i = p_i (d_i - sum_j d_j p_j),  d = scatter(g) + a
-//   sigmoid: dl_i = (scatter(g)_i + (a_i - sum_j a_j p_j) / S) s_i (1 - s_i),  S = sum s
+//   renormalised: G = scatter((g_j - sum_i g_i q_i) q_j) with q the shares, the chosen scores over their sum
+//     softmax: dl_i = G_i + p_i (a_i - sum_j a_j p_j)
+//     sigmoid: dl_i = (G_i + p_i (a_i - sum_j a_j p_j)) (1 - s_i)
+//   not renormalised, d = scatter(g):
+//     softmax: dl_i = p_i (d_i + a_i - sum_j (d_j + a_j) p_j)
+//     sigmoid: dl_i = (d_i s_i + p_i (a_i - sum_j a_j p_j)) (1 - s_i)
+// Scores too small for 32 bits still have shares and probabilities: sums of scores below 2^-60 are taken again
+// relative to the largest logit in them (there a sigmoid is e^l within 2^-60).
 //
 // Sixteen lanes take a row (32 where the choice is long or the experts are many), lane l the experts l,
 // l + 16, ...; a row is read once and its next row's loads are in flight meanwhile.  Bound by
@@ -25,6 +30,7 @@
 #include <atomic>
 #include <cfloat>
 #include <cstdint>
+#include <type_traits>
 
 #include "cdg_b200.h"
 #include "cdg_ptx.cuh"
@@ -59,6 +65,7 @@ __device__ __forceinline__ float exp_fast(float v) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v * 1.4426950408889634f));
   return r;
 }
+constexpr float kTiny = 8.673617e-19f;  // 2^-60
 __device__ __forceinline__ float sigmoid_fast(float v) { return __fdividef(1.0f, 1.0f + exp_fast(-v)); }
 
 // Sum and maximum over the lanes of a row.
@@ -344,21 +351,40 @@ __global__ void __launch_bounds__(WARPS * 32, N <= 16 ? 2 : 1) moe_route_kernel(
       }
       if (a.balance) {
         if (!valid) part = 0.0f;
+        if (a.sigmoid && __any_sync(kAll, valid && total < kTiny)) {  // rare: every logit below -41
+          float again = 0.0f;
+#pragma unroll
+          for (int i = 0; i < N; ++i) {
+            if (total < kTiny) {
+              const float l = row < a.T && i * LANES < left ? clean_logit(to_f(logits[row * a.stride + i * LANES + sub])) : -INFINITY;
+              score[i] = exp_fast(l - (m == -INFINITY ? 0.0f : m));
+            }
+            again += score[i];
+          }
+          again = lanes_sum<LANES>(again);
+          part = valid && again > 0.0f ? __fdividef(1.0f, again) : 0.0f;
+        }
 #pragma unroll
         for (int i = 0; i < N; ++i) psum[i] = fmaf(score[i], part, psum[i]);
       }
     }
     const int32_t id = valid ? __float_as_int(got.y) : -1;
-    float w = 0.0f;
+    float w = 0.0f, l = -INFINITY;
     if (id >= 0) {
       // the value is the logit itself, unless a bias went into it
-      const float l = BIAS ? clean_logit(to_f(logits[row * a.stride + id])) : got.x;
+      l = BIAS ? clean_logit(to_f(logits[row * a.stride + id])) : got.x;
       w = a.sigmoid ? sigmoid_fast(l) : exp_fast(l - m) * inv;
       atomicAdd(&s_counts[id], 1);
     }
     if (valid) ++tokens;
     if (a.renormalize) {
-      const float total = lanes_sum<LANES>(w);
+      float total = lanes_sum<LANES>(w);
+      // without a bias the softmax's largest score is among the chosen
+      if ((BIAS || a.sigmoid) && __any_sync(kAll, id >= 0 && total < kTiny)) {
+        const float most = lanes_max<LANES>(l);
+        if (id >= 0 && total < kTiny) w = exp_fast(l - most);
+        total = lanes_sum<LANES>(w);
+      }
       w = total <= 0.0f ? 0.0f : w == total ? 1.0f : __fdividef(w, total);  // a lone choice: 1 exactly
     }
     if (sub < a.k && row < a.T) {
@@ -553,6 +579,29 @@ __global__ void __launch_bounds__(WARPS * 32, N <= 16 ? 2 : 1) moe_route_backwar
       }
       total = lanes_sum<LANES>(total);
     }
+    float mul = 1.0f;  // the sigmoids are s times this
+    if constexpr (SIGMOID) {
+      if (__any_sync(kAll, live && total < kTiny)) {  // rare: every logit below -41
+        float top = -INFINITY, again = 0.0f;
+        auto logit = [&](int i) {
+          return row < a.T && i * LANES < left ? clean_logit(to_f(logits[row * a.stride + i * LANES + sub])) : -INFINITY;
+        };
+#pragma unroll
+        for (int i = 0; i < N; ++i) top = fmaxf(top, logit(i));
+        top = lanes_max<LANES>(top);
+        if (top == -INFINITY) top = 0.0f;
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+          if (total < kTiny) s[i] = exp_fast(logit(i) - top);
+          again += s[i];
+        }
+        again = lanes_sum<LANES>(again);
+        if (total < kTiny) {
+          mul = exp_fast(top);
+          total = again;
+        }
+      }
+    }
     // a row without a choice: all terms zero
     const float inv = live && total > 0.0f ? __fdividef(1.0f, total) : 0.0f;
 #pragma unroll
@@ -564,40 +613,56 @@ __global__ void __launch_bounds__(WARPS * 32, N <= 16 ? 2 : 1) moe_route_backwar
     }
     if (a.gw) {
       if (a.renormalize) {
-        float c = 0.0f;
+        float c = 0.0f, l = -INFINITY;
         if (id >= 0) {
-          const float l = clean_logit(to_f(logits[row * a.stride + id]));
+          l = clean_logit(to_f(logits[row * a.stride + id]));
           c = SIGMOID ? sigmoid_fast(l) : exp_fast(l - shift) * inv;
         }
-        const float sum = lanes_sum<LANES>(c), chosen = sum > 0.0f ? __fdividef(1.0f, sum) : 1.0f;
-        g = (g - lanes_sum<LANES>(g * (c == sum ? 1.0f : c * chosen))) * chosen;  // nothing moves a weight of 1
+        float sum = lanes_sum<LANES>(c);
+        if (__any_sync(kAll, id >= 0 && sum < kTiny)) {
+          const float most = lanes_max<LANES>(l);
+          if (id >= 0 && sum < kTiny && most > -INFINITY) c = exp_fast(l - most);
+          sum = lanes_sum<LANES>(c);
+        }
+        const float share = sum <= 0.0f ? 0.0f : c == sum ? 1.0f : __fdividef(c, sum);  // nothing moves a share of 1
+        g = (g - lanes_sum<LANES>(g * share)) * share;
       }
       if (id >= 0) atomicAdd(&sg[id], g);
       __syncwarp();
     }
-    float d[N];
-    float dot = 0.0f;  // of what meets the probabilities: everything (softmax) or the loss alone
+    // SHARES: what was scattered is G of the head's formulas, else d
+    auto finish = [&](auto shares) {
+      constexpr bool SHARES = decltype(shares)::value;
+      float d[N];
+      float dot = 0.0f;  // of what meets the probabilities
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-      d[i] = a.gw && i * LANES < left ? sg[i * LANES + sub] : 0.0f;
-      if constexpr (!SIGMOID) d[i] += load[i];
-      dot = fmaf(SIGMOID ? load[i] : d[i], s[i], dot);
-    }
-    dot = lanes_sum<LANES>(dot);
-    if (a.gw) {
-      __syncwarp();
-      if (id >= 0) sg[id] = 0.0f;
-      __syncwarp();
-    }
+      for (int i = 0; i < N; ++i) {
+        d[i] = a.gw && i * LANES < left ? sg[i * LANES + sub] : 0.0f;
+        if constexpr (!SIGMOID && !SHARES) d[i] += load[i];
+        dot = fmaf(SIGMOID || SHARES ? load[i] : d[i], s[i], dot);
+      }
+      dot = lanes_sum<LANES>(dot);
+      if (a.gw) {
+        __syncwarp();
+        if (id >= 0) sg[id] = 0.0f;
+        __syncwarp();
+      }
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-      float v;
-      if constexpr (SIGMOID)
-        v = (d[i] + (load[i] - dot * inv) * inv) * s[i] * (1.0f - s[i]);
-      else
-        v = s[i] * (d[i] - dot);
-      if (i * LANES < left && row < a.T) out[i * LANES] = from_f<T>(v);
-    }
+      for (int i = 0; i < N; ++i) {
+        float v;
+        if constexpr (SIGMOID) {
+          const float by_p = (load[i] - dot * inv) * inv;
+          v = (SHARES ? fmaf(s[i], by_p, d[i]) : s[i] * fmaf(d[i], mul, by_p)) * fmaf(-s[i], mul, 1.0f);
+        } else {
+          v = SHARES ? fmaf(s[i], load[i] - dot, d[i]) : s[i] * (d[i] - dot);
+        }
+        if (i * LANES < left && row < a.T) out[i * LANES] = from_f<T>(v);
+      }
+    };
+    if (a.gw && a.renormalize)
+      finish(std::true_type());
+    else
+      finish(std::false_type());
   }
 }
 

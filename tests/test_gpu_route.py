@@ -303,3 +303,57 @@ def test_route_refusals():
                  lambda: cdg.moe_route(torch.zeros(1, 64, device=DEV), 33)):
         with pytest.raises(RuntimeError):
             call()
+
+
+def _low(T, E, seed, below):
+    """Logits around `below` in every third row, around 0 in the others."""
+    z, mask = _logits(T, E, torch.float32, seed=seed, off=(3,) if E > 40 else ())
+    z[::3] += below
+    return z, mask
+
+
+def _row_error(E):
+    """_error with a row's own range: no row's logits span more than 24 here."""
+    return (2 * (4 + 2.4 * 24) + E / 32 + 16) * U
+
+
+@pytest.mark.parametrize("T,E,k", [(50, 256, 8), (4099, 161, 6), (333, 700, 24), (20000, 33, 2), (9, 16, 16)])
+@pytest.mark.parametrize("below", [-100.0, -83.0, -41.0, -600.0])
+def test_route_sigmoid_scores_below_the_normal_range(T, E, k, below):
+    """Sigmoids of logits below -87 are below 2^-126; their shares are not."""
+    z, mask = _low(T, E, seed=12, below=below)
+    o = _cdg().moe_route(z, k, scoring="sigmoid", scale=1.5, token_mask=mask, balance=True)
+    ids, w, counts, valid, loss, _ = _route64(z, k, "sigmoid", True, 1.5, mask)
+    assert torch.equal(o.ids.long(), ids) and torch.equal(o.counts.long(), counts) and int(o.tokens) == valid
+    e = _row_error(E)
+    assert bool(((o.weights.double() - w).abs() <= 2 * e * w.abs() + 1e-30).all())
+    assert abs(float(o.loss) - loss) <= (e + (T / 148 + 16) * U) * loss + 1e-30
+    gw = torch.randn(T, k, device=DEV)
+    gl = torch.tensor([0.7 * T], device=DEV)
+    for renorm in (True, False):
+        for a, b in ((gw, gl), (gw, None), (None, gl)):
+            got = _cdg().moe_route_backward(z, o.ids, a, b, o.counts, o.tokens, scoring="sigmoid", renormalize=renorm, scale=2.5)
+            want, terms = _backward64(z, o.ids, a, b, o.counts, o.tokens, "sigmoid", renorm, 2.5)
+            bad = (got.double() - want).abs() > 6 * e * terms + 1e-30
+            assert not bool(bad.any()), int(bad.sum())
+
+
+@pytest.mark.parametrize("E,k", [(64, 4), (64, 12), (600, 5)])
+@pytest.mark.parametrize("scoring", ["softmax", "sigmoid"])
+def test_route_bias_may_choose_scores_below_the_normal_range(E, k, scoring):
+    """The bias moves the choice to experts whose scores are e^-150 of the others': their shares sum to 1."""
+    T = 500
+    z, mask = _logits(T, E, torch.float32, seed=13)
+    z[:, E // 2:] -= 150.0
+    bias = -0.01 * torch.arange(E, device=DEV, dtype=torch.float32)  # decides among the low ones
+    bias[:E // 2] = -20.0
+    o = _cdg().moe_route(z, k, scoring=scoring, bias=bias, token_mask=mask)
+    want_ids = torch.where(mask[:, None], torch.arange(E // 2, E // 2 + k, device=DEV), -1)
+    assert torch.equal(o.ids.long(), want_ids)
+    c = torch.softmax(z[:, E // 2:E // 2 + k].double(), 1) * mask[:, None]
+    e = _row_error(E)
+    assert bool(((o.weights.double() - c).abs() <= 2 * e * c + 1e-30).all())
+    gw = torch.randn(T, k, device=DEV)
+    got = _cdg().moe_route_backward(z, o.ids, gw, scoring=scoring)
+    want, terms = _backward64(z, o.ids, gw, None, o.counts, o.tokens, scoring, True, 1.0)
+    assert bool(((got.double() - want).abs() <= 6 * e * terms + 1e-30).all())
