@@ -476,9 +476,13 @@ int launch_norm_backward(const NormBwd& a, const BwdShape& s, bool wide, cudaStr
     });
     return launch(rms_norm_backward_ring_kernel<T>, dim3(s.grid), s.warps * 32, slots * row, st, a, slots);
   }
-  auto kernel = a.H > kRingMaxH    ? (wide ? rms_norm_backward_kernel<T, true, 4, 1024> : rms_norm_backward_kernel<T, false, 4, 1024>)
-                : sizeof(T) == 2 ? rms_norm_backward_kernel<T, false, 1, 1024>
-                                 : rms_norm_backward_kernel<T, false, 2, 512>;
+  auto kernel = wide ? rms_norm_backward_kernel<T, true, 4, 1024> : rms_norm_backward_kernel<T, false, 4, 1024>;
+  if (a.H <= kRingMaxH) {
+    if constexpr (sizeof(T) == 2)
+      kernel = rms_norm_backward_kernel<T, false, 1, 1024>;
+    else
+      kernel = rms_norm_backward_kernel<T, false, 2, 512>;
+  }
   return launch(kernel, dim3(s.grid), s.warps * 32, 0, st, a);
 }
 
