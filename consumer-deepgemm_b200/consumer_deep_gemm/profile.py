@@ -27,6 +27,12 @@ TARGETS = (
     "m_grouped_fp8_fp4_gemm_nt_masked",
     "transform_sf_into_required_layout",
     "transform_weights_for_mega_moe",
+    "add_rms_norm",
+    "add_rms_norm_backward",
+    "linear",
+    "linear_backward",
+    "moe_route",
+    "moe_route_backward",
 )
 
 

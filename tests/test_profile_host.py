@@ -48,3 +48,17 @@ def test_gpu_calls_are_timed_with_events():
     calls, seconds = prof.stats()["m_grouped_fp8_fp4_gemm_nt_contiguous"]
     assert calls == 1 and seconds > 0
     assert torch.equal(d1.view(torch.int16), d2.view(torch.int16))
+
+
+def test_the_operators_around_the_experts_are_targets():
+    import consumer_deep_gemm as cdg
+
+    names = ("add_rms_norm", "add_rms_norm_backward", "linear", "linear_backward", "moe_route", "moe_route_backward")
+    mod = types.SimpleNamespace(**{n: getattr(cdg, n) for n in names})
+    prof = profile.install(mod, interval=1000)
+    for n in names:
+        fn = getattr(mod, n)
+        assert fn is not getattr(cdg, n) and fn.__wrapped__ is getattr(cdg, n)
+    with pytest.raises(ValueError):
+        mod.moe_route(None, 2, scoring="tanh")
+    assert prof.calls == 0  # a call that raises is not counted
