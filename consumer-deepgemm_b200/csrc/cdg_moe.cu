@@ -1507,7 +1507,7 @@ int cdg_silu_mul_quant_planes(const void* in, int64_t in_stride, int64_t M, int6
 
 int cdg_ep_unpermute_combine(const void* Y, int64_t y_stride, const int32_t* perm_pos, const int32_t* send_index,
                              const float* topk_w, int64_t T, int64_t topk, int64_t H, void* y, cdg_stream_t stream) {
-  if (!perm_pos) return CDG_ERR_INVALID_ARGUMENT;
+  if (T > 0 && !perm_pos) return CDG_ERR_INVALID_ARGUMENT;  // no tokens, no table
   return cdg::launch_combine(Y, y_stride, perm_pos, send_index, topk_w, T, topk, H, y,
                              reinterpret_cast<cudaStream_t>(stream));
 }

@@ -114,3 +114,9 @@ def test_block_refusals():
         MoEBlock(block.norm_weight, block.gate_weight[:, :128], layer, K)
     with pytest.raises(ValueError):
         MoEBlock(block.norm_weight, block.gate_weight[:4], layer, K)
+
+
+def test_block_of_no_tokens():
+    block, x, residual, _, _ = _block()
+    o = block(x[:0], residual[:0], balance=True)
+    assert o.out.shape == (0, H) and o.logits.shape == (0, E) and int(o.routing.tokens) == 0
