@@ -120,3 +120,56 @@ def test_block_of_no_tokens():
     block, x, residual, _, _ = _block()
     o = block(x[:0], residual[:0], balance=True)
     assert o.out.shape == (0, H) and o.logits.shape == (0, E) and int(o.routing.tokens) == 0
+
+
+def test_operators_without_programmatic_launches():
+    """set_pdl(False) changes when kernels start, not what they compute."""
+    import consumer_deep_gemm as cdg
+
+    x = torch.randn(700, 1000, device=DEV).bfloat16()
+    w = (torch.randn(300, 1000, device=DEV) / 32).bfloat16()
+    nw = torch.rand(1000, device=DEV) + 0.5
+    gw = torch.randn(700, 8, device=DEV)
+
+    def everything():
+        n = cdg.add_rms_norm(x, nw, x, quantize=True)
+        dh = cdg.add_rms_norm_backward(n.y, n.h, nw, n.y)
+        z = cdg.linear(n.y, w, out_dtype=torch.float32)
+        r = cdg.moe_route(z, 8, balance=True)
+        dz = cdg.moe_route_backward(z, r.ids, gw, r.loss, r.counts, r.tokens)
+        y, pre = cdg.linear(n.y, w, activation="silu", preact=True)
+        d = cdg.linear_backward(dz.bfloat16(), n.y, w, pre, activation="silu", bias_grad=True)
+        odd = cdg.linear(x[:, 1:], w[:, 1:], activation="gelu")
+        return [*n[:2], n.q.view(torch.uint8), n.scale, *dh, z, *r, dz, y, pre, *d, odd]
+
+    want = everything()
+    cdg.set_pdl(False)
+    try:
+        got = everything()
+    finally:
+        cdg.set_pdl(True)
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)
+
+
+def test_products_on_two_streams_at_once():
+    """Persistent and tile kernels beside each other: the bits of the calls one after the other."""
+    import consumer_deep_gemm as cdg
+
+    shapes = [(4096, 2048, 512), (300, 512, 2048), (1, 4096, 1024), (2593, 2307, 264), (64, 256, 4096)]
+    calls = [((torch.randn(m, k, device=DEV).bfloat16(), (torch.randn(n, k, device=DEV) / k ** 0.5).bfloat16()))
+             for m, n, k in shapes]
+    want = [cdg.linear(x, w, activation="gelu_tanh") for x, w in calls]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = [[], []]
+    for _ in range(10):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                for x, w in calls if i == 0 else calls[::-1]:
+                    got[i].append(cdg.linear(x, w, activation="gelu_tanh"))
+    torch.cuda.synchronize()
+    for i in range(2):
+        for j, y in enumerate(got[i]):
+            assert torch.equal(y, (want if i == 0 else want[::-1])[j % len(want)])
+    assert cabi.device_status() == (0, 0)

@@ -357,3 +357,18 @@ def test_route_bias_may_choose_scores_below_the_normal_range(E, k, scoring):
     got = _cdg().moe_route_backward(z, o.ids, gw, scoring=scoring)
     want, terms = _backward64(z, o.ids, gw, None, o.counts, o.tokens, scoring, True, 1.0)
     assert bool(((got.double() - want).abs() <= 6 * e * terms + 1e-30).all())
+
+
+@pytest.mark.parametrize("T,E,k", [(1000, 256, 8), (77, 7, 7), (333, 700, 24)])
+@pytest.mark.parametrize("scoring,renorm", [("softmax", True), ("sigmoid", False)])
+def test_route_backward_of_fp16_logits(T, E, k, scoring, renorm):
+    """As against 64 bits above; FP16 results below 2^-14 are rounded to a multiple of 2^-24."""
+    z, mask = _logits(T, E, torch.float16, seed=14)
+    o = _cdg().moe_route(z, k, scoring=scoring, renormalize=renorm, token_mask=mask, balance=True)
+    gw = torch.randn(T, k, device=DEV)
+    gl = torch.tensor([0.7 * T], device=DEV)
+    got = _cdg().moe_route_backward(z, o.ids, gw, gl, o.counts, o.tokens, scoring=scoring, renormalize=renorm)
+    want, terms = _backward64(z, o.ids, gw, gl, o.counts, o.tokens, scoring, renorm, 1.0)
+    assert got.dtype == torch.float16
+    slack = UNIT[torch.float16] * want.abs() + 6 * _error(z, E) * terms + 2.0 ** -25
+    assert bool(((got.double() - want).abs() <= slack).all())
