@@ -264,8 +264,10 @@ int launch_pairs(const Matrix& A, const Matrix& B, const LinearShape& s, Epilogu
   // a box of y or of the residual is one warp's 32 rows x 128 bytes
   const Matrix y{e.y, e.y_stride, M, N}, r{e.residual, e.residual_stride, M, N};
   const bool apart = M == 1 || (y.stride >= N && (!e.residual || r.stride >= N));
+  // TMA stores whole pieces of 16 bytes: where a row ends inside one, the rest of it is not this row's to write
+  const bool whole = N * static_cast<int64_t>(sizeof(O)) % 16 == 0;
   // (FP32 results have four chunks a warp and tile, and no staged residual)
-  e.staged = e.z || (e.residual && (sizeof(O) == 4 || e.residual_f32)) ? 0 : e.wide && apart ? 1 : 2;
+  e.staged = e.z || (e.residual && (sizeof(O) == 4 || e.residual_f32)) ? 0 : e.wide && apart && whole ? 1 : 2;
   if (rc == CDG_OK && e.staged == 1) rc = make_map(&ty, y, kOut, 32);
   if (rc == CDG_OK && e.staged == 1 && e.residual) rc = make_map(&tr, r, kOut, 32);
   if (rc != CDG_OK) return rc;

@@ -835,7 +835,7 @@ __global__ void __launch_bounds__(kThreadsOf<SWAP>)
 // residual where there is one, of the output's type and on 16-byte rows, z not stored): each epilogue
 // warp has the residual brought into its own shared-memory tile of 32 rows x 128 bytes by TMA, ahead
 // of the accumulator, adds it in place and has the result stored from there, so that global memory
-// sees whole tiles; clipping at M and N is TMA's.  Where rows start on other boundaries, the warp
+// sees whole tiles; clipping at M and N is TMA's.  Where rows start or end on other boundaries, the warp
 // itself copies the residual's rows in and the result's out, in whole words (10,861 x 3279 x 48 with a
 // residual: 226 us with single elements, 89 us so).  With z, or a residual of another type, its lanes turn
 // their columns and store along the rows.

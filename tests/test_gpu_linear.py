@@ -363,3 +363,33 @@ def test_gelu_tail_is_relatively_accurate(rows):
     assert bool(((got.double() - want).abs() <= near).all())
     got = _cdg().linear(x, z[:, None].contiguous(), activation="gelu")
     assert bool(((got.double() - want).abs() <= 2.0 ** -8 * want.abs() * (1 + 2.0 ** -8) + near).all())
+
+
+@pytest.mark.parametrize("M,N,stride,off", [(2626, 2239, 2240, 0), (2626, 2233, 2248, 8), (4096, 2045, 2056, 0),
+                                            (513, 1030, 1040, 16), (300, 197, 200, 0), (40, 61, 64, 0), (3, 1001, 1008, 0),
+                                            (2600, 2250, 2257, 3)])
+@pytest.mark.parametrize("out", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("with_z", [False, True])
+def test_results_into_columns_of_a_wider_matrix(M, N, stride, off, out, with_z):
+    """By the C ABI y and z may be columns of wider matrices: the others' columns keep their values."""
+    import ctypes
+
+    from test_operators_host import FP32, BF16, LinearArgs
+
+    lib = cabi.lib()
+    x, w = _operands(M, N, 136, torch.bfloat16, seed=15)
+    wide = torch.full((off + M * stride,), 7.0, device=DEV, dtype=out)
+    z_wide = torch.full((off + M * stride,), 7.0, device=DEV, dtype=torch.bfloat16)
+    y, z = (t.as_strided((M, N), (stride, 1), off) for t in (wide, z_wide))
+    g = LinearArgs(x=x.data_ptr(), x_stride=136, w=w.data_ptr(), w_stride=136, dtype=BF16,
+                   out_dtype=FP32 if out == torch.float32 else BF16, activation=2, M=M, N=N, K=136, y=y.data_ptr(),
+                   y_stride=stride, z_out=z.data_ptr() if with_z else None, z_stride=stride)
+    lib.cdg_linear.argtypes = [ctypes.POINTER(LinearArgs), ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p]
+    assert lib.cdg_linear(ctypes.byref(g), None, 0, ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)) == 0
+    torch.cuda.synchronize()
+    _check(y, x, w, None, None, "silu", out)
+    if with_z:
+        _check(z, x, w, None, None, None, torch.bfloat16)
+        z.fill_(7.0)
+    y.fill_(7.0)
+    assert bool((wide == 7.0).all()) and bool((z_wide == 7.0).all())
