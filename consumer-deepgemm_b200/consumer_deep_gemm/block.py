@@ -82,7 +82,8 @@ class MoEBlock:
     def router_gradients(self, o: BlockOutput, grad_weights: Optional[torch.Tensor] = None,
                          grad_loss: Optional[torch.Tensor] = None) -> RouterGradients:
         """Gradients from those of the gate's weights (FP32 ``[T, topk]``) and of the balance loss
-        (FP32 ``[1]``), along the router's path alone; ``h``'s is to be added to the others that reach it."""
+        (FP32 ``[1]``), along the router's path alone; ``h``'s is to be added to the others that reach it.  The
+        logits' gradient is rounded to the rows' dtype, as an operand of the gate's two products."""
         r = o.routing
         dlogits = moe_route_backward(o.logits, r.ids, grad_weights, grad_loss, r.counts, r.tokens, scoring=self.scoring,
                                      renormalize=self.renormalize, scale=self.scale)

@@ -54,6 +54,7 @@ def linear_backward(dy: torch.Tensor, x: torch.Tensor, weight: torch.Tensor, z: 
 
     dy, z: ``[M, N]`` of x's dtype; ``z`` is the forward call's (``preact=True``) and needed with an
     activation only.  The gradient of the residual is ``dy`` itself.  ``dz = dy * act'(z)`` is rounded
-    to x's dtype, as an operand of both products; ``dbias`` sums its unrounded values.
+    to x's dtype, as an operand of both products (the error of ``dx`` and ``dweight`` is sqrt 2 of what their
+    own rounding leaves); ``dbias`` has x's dtype and sums the unrounded values.
     """
     return native.require().linear_backward(dy, x, weight, z, _activation(activation), input_grad, weight_grad, bias_grad)

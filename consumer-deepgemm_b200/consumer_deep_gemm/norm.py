@@ -33,9 +33,11 @@ def add_rms_norm(x: torch.Tensor, weight: torch.Tensor, residual: Optional[torch
     x, residual: BF16, FP16 or FP32 ``[T, H]`` (any row stride, H up to 32,768); weight ``[H]`` of
     the same dtype or FP32.  The sum and the norm are held in FP32: ``h`` and ``y`` are each rounded
     once, and the codes are of the unrounded ``y``.  ``quantize=True`` adds ``q`` and ``scale`` (1x128
-    blocks, the last one shorter when H is no multiple of 128; the amax/448 recipe, or with
+    blocks, the last one shorter when H is no multiple of 128; the amax/448 recipe of the framework's
+    quantiser, whose scales these are bit for bit, or with
     ``ue8m0=True`` scales rounded up to powers of two); ``normed=False`` leaves ``y`` out.
-    A row of zeros gives zeros; a NaN keeps its place in ``y`` and ``q`` (its row is NaN).
+    A row of zeros gives zeros (with ``eps`` > 0); a NaN keeps its place in ``y`` and ``q`` (its row is NaN);
+    a row whose mean square passes FP32's range gives zeros.
     """
     return AddRMSNorm(*native.require().add_rms_norm(x, weight, residual, eps, quantize, ue8m0, normed))
 
@@ -46,8 +48,8 @@ def add_rms_norm_backward(dy: torch.Tensor, h: torch.Tensor, weight: torch.Tenso
 
     ``h`` is the forward pass's ``h`` (its ``x`` where there was no residual), ``dh`` the gradient
     that reaches it by the residual stream.  ``dx`` is the gradient of ``x`` and of ``residual``
-    alike; ``dweight`` has the weight's dtype and is summed over the rows in FP32, in an order that
-    depends on the sizes alone.
+    alike; ``dweight`` has the weight's dtype and is summed over the rows in FP32, in an order that the
+    sizes, the dtype, whether the rows lie on 16-byte boundaries, and the GPU's SM count fix.
     """
     dx, dw = native.require().rms_norm_backward(dy, h, weight, dh, eps)
     return dx, dw

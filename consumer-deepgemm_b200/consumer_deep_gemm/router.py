@@ -43,7 +43,8 @@ def moe_route(logits: torch.Tensor, topk: int, *, scoring: str = "softmax", reno
     With ``score = softmax(logits)`` or ``sigmoid(logits)`` in FP32, a token's ids are its ``topk``
     largest logits -- with ``bias`` (FP32 ``[E]``), its largest ``score + bias`` -- in falling order,
     ties to the lowest index; its weights are ``scale * score[ids]``, divided by their sum before
-    scaling with ``renormalize``.  Tokens that ``token_mask`` (bool or uint8 ``[T]``) drops and slots
+    scaling with ``renormalize`` (shares that sum to 1 also where the scores themselves are below FP32's
+    range).  Tokens that ``token_mask`` (bool or uint8 ``[T]``) drops and slots
     for which no logit above -inf is left get id -1 and weight 0, which ``MoELayer`` passes over;
     an expert is switched off by logits of -inf.  NaN counts as -inf, +inf as the largest finite value.
 

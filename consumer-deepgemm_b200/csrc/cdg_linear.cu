@@ -9,9 +9,10 @@
 // Operands whose rows do not start on 16-byte boundaries cannot be loaded by TMA: they are copied
 // once into the workspace with padded rows.
 //
-// One B200: 8192 x 4096 x 4096 with bias, GELU and residual 197 us (1.40 PFLOP/s, the power limit), the
-// bare product 217 us back to back for seconds, as the library's; gradient of 8192 x 2048 x 4096 with SiLU and
-// bias 221 us; 32,768 x 256 x 4096 with FP32 results 67 us; 1 x 4096 x 4096 10 us.
+// One B200, short replays: 8192 x 4096 x 4096 with bias, GELU and residual 200 us (1.38 PFLOP/s), gradient of
+// 8192 x 2048 x 4096 with SiLU and bias 223 us; 32,768 x 256 x 4096 with FP32 results 68 us; 1 x 4096 x 4096
+// 10 us.  Back to back for seconds the power limit lowers the clock: the first takes 233 us (1.18
+// PFLOP/s) then, the bare product 213 us, the library's 216 us.
 #include <cuda.h>
 #include <cuda_runtime.h>
 

@@ -11,8 +11,9 @@
 // Both directions are bound by memory: the forward pass reads x and r once and writes h, y, q and
 // the scales once, the backward pass reads dy, h and dh once and writes dx once.  A row stays in
 // its CTA's registers between the sum of squares and the stores.  One B200: 32,768 x 4096 BF16 with
-// residual and codes 192 us (6.3 TB/s; a plain copy 6.5), 8 x 4096 2.3 us; backward of 16,384 x 4096
-// with dh 94 us (5.7 TB/s) with the sums of dw.
+// residual and codes 194 us (6.2 TB/s; a plain copy 6.5), 8 x 4096 2.3 us; backward of 16,384 x 4096
+// with dh 94 us (5.7 TB/s) with the sums of dw.  Rows off 16-byte boundaries move by single elements: 6007 x
+// 2503 BF16 with residual and codes 44 us (3.1 TB/s), backward 55 us (2.2 TB/s).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
@@ -451,7 +452,9 @@ constexpr int64_t kRingMaxH = 8192;  // 16 warps of two chunks
 // Two chunks a warp and sixteen warps an SM (16,384 x 4096 BF16: 93 us; eight warps leave the loads
 // waiting, 128 us, 24 and more gain nothing, 96 to 122 us), but for 16-bit rows on odd boundaries, whose
 // loads of single elements want warps rather than registers: one chunk and 32 (6007 x 2503: 53 us
-// against 75).  Rows of more than 8192 columns take four chunks a warp.
+// against 75).  Rows of more than 8192 columns take four chunks a warp and spill most of them (1 to 2.4 KB
+// a thread): 8192 x 9216 BF16 1.97 ms, 0.3 TB/s.  From nine warps on, 4097 to 7680 columns, an SM holds
+// one CTA: 8192 x 4352 73 us (3.9 TB/s), 16,384 x 5120 144 us (4.7 TB/s).
 BwdShape backward_shape(int64_t T, int64_t H, bool single) {
   const int chunks = static_cast<int>((H + 255) / 256);
   BwdShape s;

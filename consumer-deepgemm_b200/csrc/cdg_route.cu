@@ -18,10 +18,11 @@
 // relative to the largest logit in them (there a sigmoid is e^l within 2^-60).
 //
 // Sixteen lanes take a row (32 where the choice is long or the experts are many), lane l the experts l,
-// l + 16, ...; a row is read once and its next row's loads are in flight meanwhile.  Bound by
-// instructions (357 a row forward, most of them the choice), not by memory: one B200,
-// calls in a row, 32,768 x 256 FP32, k = 8 with the balance loss 20.8 us forward (1.7 TB/s) and 16.8 us
-// backward (4.0 TB/s); 64 x 256 4.9 us and 3.2 us.
+// l + 16, ...; a row is read once and its next row's loads are in flight meanwhile.  Bound by the latency of
+// a row's chain (sort, list, rank, sums; 359 instructions): 116 registers a thread leave 16 warps an
+// SM, a quarter of its slots, which issue in 59% of the cycles; DRAM is 17% busy.  One B200, calls in a row,
+// 32,768 x 256 FP32, k = 8 with the balance loss 21.0 us forward (1.7 TB/s) and 17.1 us backward (4.1 TB/s),
+// 22.0 and 17.4 us with sigmoid scores; 64 x 256 4.9 us and 3.2 us; 32,768 x 512, k = 16 44 and 30 us.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>

@@ -548,7 +548,8 @@ int cdg_rms_norm_backward(const cdg_norm_backward_args* args, void* workspace, s
  * token_mask keeps and that has an expert above -inf (logit, and bias where given):
  *   score = softmax(logits) or sigmoid(logits), p = score / sum(score);
  *   ids = the topk largest logits (with a bias: the topk largest score + bias), ties to the lowest
- *   index; weights = scale * score[ids], divided by their sum before scaling if renormalize.
+ *   index; weights = scale * score[ids], divided by their sum before scaling if renormalize (shares that
+ *   sum to 1 also where the scores themselves are below FP32's range).
  * A masked token, and a slot for which no logit above -inf is left, gets id -1 and weight 0 (the
  * MoE layer's "no expert").  NaN logits count as -inf, +inf as the largest finite value.
  * counts[e] = tokens that chose e, *tokens = V = valid tokens, and, unless loss is NULL,
