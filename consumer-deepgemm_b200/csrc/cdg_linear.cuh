@@ -121,7 +121,8 @@ __device__ __forceinline__ float activate_slope(float z, int act) {
     case CDG_ACT_GELU_TANH: {
       // with s = sigmoid(2u): z s' + s, s' = s (1 - s) d(2u)/dz
       const float s = fast_sigmoid(1.5957691216057308f * (z + 0.044715f * z * z * z));
-      return s + z * s * (1.0f - s) * 1.5957691216057308f * (1.0f + 0.134145f * z * z);
+      // z^2 kept finite: far from zero s (1 - s) is 0, and so is the term
+      return s + z * s * (1.0f - s) * 1.5957691216057308f * (1.0f + 0.134145f * fminf(z * z, 1e30f));
     }
     default: return 1.0f;
   }

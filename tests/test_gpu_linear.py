@@ -393,3 +393,15 @@ def test_results_into_columns_of_a_wider_matrix(M, N, stride, off, out, with_z):
         z.fill_(7.0)
     y.fill_(7.0)
     assert bool((wide == 7.0).all()) and bool((z_wide == 7.0).all())
+
+
+@pytest.mark.parametrize("act", ACTS[1:])
+def test_activations_and_slopes_of_the_largest_values(act):
+    """Far from zero an activation is z or 0 and its slope 1 or 0, up to BF16's largest value."""
+    z = torch.tensor([3.3e38, 1e30, 2e19, 1e15, 300.0], device=DEV).bfloat16()
+    z = torch.cat([z, -z])
+    y = _cdg().linear(z[:, None].contiguous(), torch.ones(1, 1, device=DEV).bfloat16(), activation=act)
+    assert torch.equal(y[:5, 0], z[:5]) and float(y[5:].float().abs().sum()) == 0
+    dx, _, db = _cdg().linear_backward(torch.ones_like(y), torch.ones_like(y), torch.ones(1, 1, device=DEV).bfloat16(),
+                                       z[:, None].contiguous(), activation=act, bias_grad=True)
+    assert dx[:, 0].tolist() == [1.0] * 5 + [0.0] * 5 and float(db) == 5.0
